@@ -22,6 +22,8 @@ __all__ = [
     "quantize_per_tensor_fp8", "dequantize_per_tensor_fp8", "stochastic_rounding_fp8", "quantize_nvfp4", "dequantize_nvfp4",
     "quantize_mxfp8", "dequantize_mxfp8", "scaled_mm_nvfp4", "scaled_mm_mxfp8",
     "apply_rope", "apply_rope1", "apply_rope_split_half", "apply_rope_split_half1",
+    "apply_rope_axes", "apply_rope_axes1", "rope_axes_freqs",
+    "add_rmsnorm_quantize_mxfp8", "add_rmsnorm_quantize_fp8", "lora_add",
     "swap_nibbles", "to_blocked", "from_blocked",
     "list_backends", "set_backend_priority", "enable_backend", "disable_backend", "use_backend",
     "BackendError", "BackendNotFoundError", "BackendNotImplementedError", "NoCapableBackendError",
@@ -93,6 +95,44 @@ def adaln_quantize_nvfp4(x, scale, shift, per_tensor_scale, eps: float = 1e-6, h
 def adaln_quantize_mxfp8(x, scale, shift, eps: float = 1e-6):
     """``quantize_mxfp8(adaln(x, scale, shift, eps).reshape(-1, D))`` in one pass over x."""
     return _ops_ns.adaln_quantize_mxfp8(x, scale, shift, eps)
+
+
+def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+                               return_norm: bool = False, sum_out: torch.Tensor | None = None):
+    """h = x + residual; ``quantize_mxfp8(rmsnorm(h, weight, eps).reshape(-1, D))`` in one pass.
+    -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``residual`` and h
+    have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to, e.g. ``residual`` itself."""
+    if sum_out is None:
+        got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
+    else:
+        impl = registry.get_implementation("add_rmsnorm_quantize_mxfp8", kwargs={"x": x, "residual": residual, "weight": weight})
+        got = impl(x, residual, weight, eps, return_norm, sum_out)
+    return got if return_norm else got[:-1]
+
+
+def add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor,
+                             eps: float = 1e-6, output_type: torch.dtype = torch.float8_e4m3fn, return_norm: bool = False,
+                             sum_out: torch.Tensor | None = None):
+    """h = x + residual; ``quantize_per_tensor_fp8(rmsnorm(h, weight, eps), scale, output_type)`` in one pass.
+    -> (data, h), and the normalised h behind them with ``return_norm``; see ``add_rmsnorm_quantize_mxfp8``."""
+    if sum_out is None:
+        got = _ops_ns.add_rmsnorm_quantize_fp8(x, residual, weight, scale, eps, DTYPE_TO_CODE[output_type], return_norm)
+    else:
+        impl = registry.get_implementation("add_rmsnorm_quantize_fp8", kwargs={"x": x, "residual": residual, "weight": weight, "scale": scale,
+                                                                               "output_type": output_type})
+        got = impl(x, residual, weight, scale, eps, output_type, return_norm, sum_out)
+    return got if return_norm else got[:-1]
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+             scales: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y + scales[i] * (x @ a[i].T) @ b[i].T with i the row's adapter id: the low-rank adapters of many requests beside
+    a shared projection y [..., N] of x [..., K].  a: [L, R, K]; b: [L, N, R]; adapter_ids: int32 or int64, one per row
+    or per leading index (outside [0, L): no adapter); ``out`` may be y."""
+    if out is None:
+        return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
+    impl = registry.get_implementation("lora_add", kwargs={"y": y, "x": x, "a": a, "b": b, "adapter_ids": adapter_ids, "scales": scales})
+    return impl(y, x, a, b, adapter_ids, scales, out)
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, freqs_cis: torch.Tensor, heads: int,
@@ -183,6 +223,25 @@ def apply_rope_split_half(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.T
 
 def apply_rope_split_half1(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
     return _ops_ns.apply_rope_split_half1(x, freqs_cis)
+
+
+def rope_axes_freqs(axes_dim, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """Radians per unit of position for every pair, float64 [sum(axes_dim) / 2]: theta^(-2i / d) for pair i of an axis of d
+    elements.  Any other table (scaled, or one spectrum shared by the axes) can be passed to ``apply_rope_axes`` instead."""
+    return torch.cat([theta ** (-torch.arange(0, d, 2, dtype=torch.float64) / d) for d in axes_dim]).to(device)
+
+
+def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim,
+                    split_half: bool = False, tokens_dim: int = 2, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """RoPE of q and k by positions [N, A] or [B, N, A] on A axes, without a table: pair p of a head turns by
+    positions[n, axis of p] * freqs[p].  x: [B, H, N, D] (``tokens_dim`` 2) or [B, N, H, D] (1), any strides; k may have
+    fewer heads; elements behind sum(axes_dim) pass through.  ``inverse`` rotates back."""
+    return _ops_ns.apply_rope_axes(xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
+
+
+def apply_rope_axes1(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim, split_half: bool = False,
+                     tokens_dim: int = 2, inverse: bool = False) -> torch.Tensor:
+    return _ops_ns.apply_rope_axes1(x, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
 
 
 # ------------------------------------------------------------------ backend configuration

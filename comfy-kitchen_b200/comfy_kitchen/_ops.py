@@ -229,3 +229,68 @@ def _op_stochastic_rounding_fp8(x: torch.Tensor, rng: torch.Tensor, output_type:
 @_op_stochastic_rounding_fp8.register_fake
 def _(x, rng, output_type):
     return torch.empty(x.shape, dtype=output_type, device=x.device)
+
+
+@torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_mxfp8", mutates_args=())
+def _op_add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float,
+                                   return_norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _dispatch("add_rmsnorm_quantize_mxfp8", x=x, residual=residual, weight=weight, eps=eps, return_norm=return_norm)
+
+
+@_op_add_rmsnorm_quantize_mxfp8.register_fake
+def _(x, residual, weight, eps, return_norm):
+    d = x.shape[-1]
+    n = x.numel() // d
+    return (torch.empty((n, d), dtype=torch.float8_e4m3fn, device=x.device),
+            torch.empty((roundup(n, 128), roundup(d // 32, 4)), dtype=torch.float8_e8m0fnu, device=x.device),
+            torch.empty(x.shape, dtype=residual.dtype, device=x.device),
+            torch.empty(x.shape if return_norm else (0,), dtype=x.dtype, device=x.device))
+
+
+@torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_fp8", mutates_args=())
+def _op_add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor, eps: float,
+                                 output_dtype_code: int, return_norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _dispatch("add_rmsnorm_quantize_fp8", x=x, residual=residual, weight=weight, scale=scale, eps=eps,
+                     output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code], return_norm=return_norm)
+
+
+@_op_add_rmsnorm_quantize_fp8.register_fake
+def _(x, residual, weight, scale, eps, output_dtype_code, return_norm):
+    return (torch.empty(x.shape, dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code], device=x.device),
+            torch.empty(x.shape, dtype=residual.dtype, device=x.device),
+            torch.empty(x.shape if return_norm else (0,), dtype=x.dtype, device=x.device))
+
+
+@torch.library.custom_op("comfy_kitchen::apply_rope_axes", mutates_args=())
+def _op_apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim: list[int],
+                        split_half: bool, tokens_dim: int, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _dispatch("apply_rope_axes", xq=xq, xk=xk, positions=positions, freqs=freqs, axes_dim=axes_dim, split_half=split_half,
+                     tokens_dim=tokens_dim, inverse=inverse)
+
+
+@_op_apply_rope_axes.register_fake
+def _(xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse):
+    return torch.empty(xq.shape, dtype=xq.dtype, device=xq.device), torch.empty(xk.shape, dtype=xk.dtype, device=xk.device)
+
+
+@torch.library.custom_op("comfy_kitchen::apply_rope_axes1", mutates_args=())
+def _op_apply_rope_axes1(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim: list[int], split_half: bool,
+                         tokens_dim: int, inverse: bool) -> torch.Tensor:
+    return _dispatch("apply_rope_axes1", x=x, positions=positions, freqs=freqs, axes_dim=axes_dim, split_half=split_half,
+                     tokens_dim=tokens_dim, inverse=inverse)
+
+
+@_op_apply_rope_axes1.register_fake
+def _(x, positions, freqs, axes_dim, split_half, tokens_dim, inverse):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+@torch.library.custom_op("comfy_kitchen::lora_add", mutates_args=())
+def _op_lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+                 scales: torch.Tensor | None) -> torch.Tensor:
+    return _dispatch("lora_add", y=y, x=x, a=a, b=b, adapter_ids=adapter_ids, scales=scales)
+
+
+@_op_lora_add.register_fake
+def _(y, x, a, b, adapter_ids, scales):
+    return torch.empty(y.shape, dtype=y.dtype, device=y.device)

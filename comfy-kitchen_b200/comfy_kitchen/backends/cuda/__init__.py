@@ -6,7 +6,8 @@ reference's CUDA backend module (comfy_kitchen/backends/cuda/__init__.py:369-529
 unchanged.  Differences, all additive: fp32 inputs to the block quantizers, fp32
 bias in ``scaled_mm_*``, ``dequantize_mxfp8`` / ``scaled_mm_mxfp8`` on the device,
 no zero-fill pass over the scale buffers (the kernels write the padding), and the
-fused ``adaln_quantize_*`` / ``rmsnorm`` entry points.
+fused ``adaln_quantize_*`` / ``rmsnorm`` entry points, and the serving operators around a quantized linear
+(``add_rmsnorm_quantize_*``, ``apply_rope_axes``, ``lora_add``).
 
 Every output is allocated here with torch (caching allocator, CUDA-graph safe);
 the native side only launches on the current stream.  Nothing synchronises.
@@ -588,6 +589,227 @@ def rmsnorm_quantize_nvfp4(
     return qx, sx.view(torch.float8_e4m3fn)
 
 
+# ------------------------------------------------------------------ around a quantized linear, when serving
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _no_grad(what: str, *tensors) -> None:
+    """These entry points record no gradient; a call that would drop one is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def _same_device(what: str, device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _launch(device, name: str, *args) -> None:
+    """_native.call with ``device`` current, on its current stream (appended as the last argument)."""
+    if device.index == torch.cuda.current_device():
+        _native.call(name, *args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            _native.call(name, *args, _stream(device))
+
+
+def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
+    """t as [rows, width] with unit column stride, rows apart by at least their width; a copy where it has no such view."""
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, width)
+        except RuntimeError:
+            return t.reshape(-1, width).contiguous()
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm, sum_out):
+    x, residual, weight = _plain(x), _plain(residual), _plain(weight)
+    _no_grad(what, x, residual, weight)
+    _require(x.dim() >= 1 and x.shape == residual.shape, f"{what}: x {tuple(x.shape)} and residual {tuple(residual.shape)} must have the same shape")
+    _require(residual.dtype in (x.dtype, torch.float32), f"{what}: the residual has x's dtype or float32, got {residual.dtype}")
+    d = x.shape[-1]
+    n = x.numel() // d if d else 0
+    mx = scale is None
+    _require(d > 0 and (not mx or d % 32 == 0), f"{what}: last dim must be positive{' and divisible by 32' if mx else ''}, got {d}")
+    _require(weight is None or tuple(weight.shape) == (d,), f"{what}: weight must be [{d}]")
+    _same_device(what, x.device, residual, weight, sum_out)
+    if weight is not None:
+        weight = weight.to(x.dtype).contiguous()
+    if sum_out is None:
+        sum_out = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+    else:
+        _require(sum_out.shape == x.shape and sum_out.dtype == residual.dtype and sum_out.is_contiguous(),
+                 f"{what}: sum_out must be contiguous with the residual's shape and dtype")
+    norm = torch.empty(x.shape if return_norm else (0,), device=x.device, dtype=x.dtype)
+    q = torch.empty((n, d) if mx else x.shape, device=x.device, dtype=torch.uint8)
+    sx = torch.empty((roundup(n, 128), roundup(d // 32, 4)), device=x.device, dtype=torch.uint8) if mx else None
+    if n:
+        xf, rf = _rows_of(x, d), _rows_of(residual, d)
+        _launch(x.device, "launch_add_rmsnorm_quantize_kernel", _ptr(xf), _ptr(rf), _ptr(weight), _ptr(scale), _ptr(sum_out),
+                _ptr(norm if return_norm else None), _ptr(q), _ptr(sx), n, d, _row_stride(xf), _row_stride(rf), float(eps),
+                _code(x.dtype, what), _code(residual.dtype, what), DTYPE_TO_CODE[output_type])
+    return q.view(output_type), sx, sum_out, norm
+
+
+def add_rmsnorm_quantize_mxfp8(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+    return_norm: bool = False, sum_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """h = x + residual; quantize_mxfp8(rmsnorm(h, weight, eps)) in one pass -> (data, block scales, h, normalised h).
+
+    ``residual`` (and h) has x's dtype or float32; the norm is taken of h as stored and rounded to x's dtype before it
+    is quantized.  The last output is empty unless ``return_norm``.  ``sum_out``: a contiguous tensor for h, which may
+    be ``residual`` itself.
+    """
+    q, sx, h, norm = _add_rmsnorm("add_rmsnorm_quantize_mxfp8", x, residual, weight, eps, None, torch.float8_e4m3fn, return_norm, sum_out)
+    return q, sx.view(torch.float8_e8m0fnu), h, norm
+
+
+def add_rmsnorm_quantize_fp8(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor, eps: float = 1e-6,
+    output_type: torch.dtype = torch.float8_e4m3fn, return_norm: bool = False, sum_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The same with quantize_per_tensor_fp8(normalised h, scale, output_type): -> (data in x's shape, h, normalised h)."""
+    if output_type not in (torch.float8_e4m3fn, torch.float8_e5m2):
+        raise ValueError(f"Unsupported output_type: {output_type}. Expected torch.float8_e4m3fn or torch.float8_e5m2")
+    scale = _scalar_on(scale, x.device)
+    _require(scale.numel() == 1, "add_rmsnorm_quantize_fp8: scale must be a scalar tensor")
+    q, _, h, norm = _add_rmsnorm("add_rmsnorm_quantize_fp8", x, residual, weight, eps, scale, output_type, return_norm, sum_out)
+    return q, h, norm
+
+
+_POSITION_CODES = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
+
+
+def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse):
+    xq, xk = _plain(xq), _plain(xk)
+    _no_grad(what, xq, xk, positions, freqs)
+    _require(tokens_dim in (1, 2), f"{what}: tokens_dim is 2 for [B, H, N, D] or 1 for [B, N, H, D], got {tokens_dim}")
+    heads_dim = 3 - tokens_dim
+    _require(xq.dim() == 4 and (xk is None or xk.dim() == 4), f"{what}: x must have four dimensions")
+    b, n, d = xq.shape[0], xq.shape[tokens_dim], xq.shape[3]
+    _require(xk is None or (xk.dtype == xq.dtype and (xk.shape[0], xk.shape[tokens_dim], xk.shape[3]) == (b, n, d)),
+             f"{what}: q and k must agree in dtype and all dimensions but the heads")
+    axes = [int(a) for a in axes_dim]
+    _require(1 <= len(axes) <= 8 and all(a > 0 and a % 2 == 0 for a in axes) and sum(axes) <= d and d % 2 == 0,
+             f"{what}: axes_dim {axes} must be 1 to 8 positive even sizes that add up to at most the (even) head dim {d}")
+    _require(freqs.dtype == torch.float64 and tuple(freqs.shape) == (sum(axes) // 2,), f"{what}: freqs must be float64 [{sum(axes) // 2}], one per pair")
+    if positions.dim() == 2:
+        positions = positions[None]
+    _require(positions.dim() == 3 and positions.shape[0] in (1, b) and tuple(positions.shape[1:]) == (n, len(axes)),
+             f"{what}: positions must be [{n}, {len(axes)}], [1, {n}, {len(axes)}] or [{b}, {n}, {len(axes)}], got {list(positions.shape)}")
+    _require(positions.dtype in _POSITION_CODES, f"{what}: positions must be float32, float64, int32 or int64")
+    _same_device(what, xq.device, xk, positions, freqs)
+    oq = torch.empty(xq.shape, device=xq.device, dtype=xq.dtype)
+    ok = None if xk is None else torch.empty(xk.shape, device=xq.device, dtype=xq.dtype)
+    heads_q, heads_k = xq.shape[heads_dim], 0 if xk is None else xk.shape[heads_dim]
+    if oq.numel() == 0 or (ok is not None and ok.numel() == 0):
+        if oq.numel():
+            return _rope_axes(what, xq, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)[0], ok
+        if ok is not None and ok.numel():
+            return oq, _rope_axes(what, xk, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)[0]
+        return oq, ok
+
+    def order(s):
+        return (s[0], s[tokens_dim], s[heads_dim])
+
+    freqs = freqs.contiguous()
+    sq, sp = xq.stride(), positions.stride()
+    sk = sq if xk is None else xk.stride()
+    strides = (ctypes.c_int64 * 17)(*order(sq), sq[3], *order(sk), sk[3], *order(oq.stride()), *order((oq if ok is None else ok).stride()),
+                                    0 if positions.shape[0] == 1 else sp[0], sp[1], sp[2])
+    _launch(xq.device, "launch_apply_rope_axes_kernel", _ptr(xq), _ptr(xk), _ptr(positions), _ptr(freqs), _ptr(oq), _ptr(ok), strides,
+            b, n, heads_q, heads_k, d, (ctypes.c_int32 * len(axes))(*[a // 2 for a in axes]), len(axes), _code(xq.dtype, what),
+            _POSITION_CODES[positions.dtype], bool(split_half), bool(inverse))
+    return oq, ok
+
+
+def apply_rope_axes(
+    xq: torch.Tensor, xk: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim, split_half: bool = False,
+    tokens_dim: int = 2, inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary embedding of q and k by positions of several axes, the angles computed in the kernel.
+
+    xq, xk: [B, H, N, D] (``tokens_dim`` 2) or [B, N, H, D] (1), any strides; k may have fewer heads.  positions: [N, A],
+    [1, N, A] or [B, N, A], integers or fractions.  axes_dim: how many elements of a head each of the A axes turns, in
+    order; what is left of D passes through.  freqs: float64, one per pair, radians per unit of position
+    (``rope_axes_freqs``).  ``inverse`` rotates back, which is also the gradient's rotation.  Outputs are contiguous.
+    """
+    return _rope_axes("apply_rope_axes", xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
+
+
+def apply_rope_axes1(
+    x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim, split_half: bool = False, tokens_dim: int = 2,
+    inverse: bool = False,
+) -> torch.Tensor:
+    return _rope_axes("apply_rope_axes1", x, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)[0]
+
+
+def lora_add(
+    y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+    scales: torch.Tensor | None = None, out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """y + scales[i] * (x @ a[i].T) @ b[i].T, with i = adapter_ids of the row: the adapters of many requests beside a
+    shared projection.
+
+    y: [..., N], what the shared projection made of x: [..., K].  a: [L, R, K], b: [L, N, R] (adapters of a lower rank are
+    padded with zeros).  adapter_ids: int32 or int64 in the shape of x's leading dimensions, or of the first of them
+    (one per batch entry); an id outside [0, L) means no adapter, and the row of y is passed on.  scales: float32 [L].
+    ``out``: where to write, in y's shape; may be y itself.  K, N and R are multiples of 8, R at most 256.
+    """
+    what = "lora_add"
+    y, x, a, b = _plain(y), _plain(x), _plain(a), _plain(b)
+    _no_grad(what, y, x, a, b, scales)
+    _require(x.dim() >= 1 and a.dim() == 3 and b.dim() == 3, f"{what}: a must be [L, R, K] and b [L, N, R]")
+    (adapters, rank, k), n = a.shape, b.shape[1]
+    _require(tuple(b.shape) == (adapters, n, rank), f"{what}: a {list(a.shape)} and b {list(b.shape)} do not match")
+    _require(x.shape[-1] == k, f"{what}: x has {x.shape[-1]} columns, a {k}")
+    _require(y.shape == (*x.shape[:-1], n), f"{what}: y must be {[*x.shape[:-1], n]}, got {list(y.shape)}")
+    _require(x.dtype == y.dtype == a.dtype == b.dtype, f"{what}: y, x, a and b must have one dtype")
+    _require(adapters > 0 and 0 < rank <= 256 and rank % 8 == 0 and k > 0 and k % 8 == 0 and n > 0 and n % 8 == 0,
+             f"{what}: K, N and R must be multiples of 8 and R at most 256, got {k}, {n}, {rank} of {adapters} adapters")
+    _require(adapter_ids.dtype in (torch.int32, torch.int64), f"{what}: adapter_ids must be int32 or int64")
+    _require(adapter_ids.dim() < x.dim() and adapter_ids.shape == x.shape[:adapter_ids.dim()],
+             f"{what}: adapter_ids {list(adapter_ids.shape)} must have the shape of x's leading dimensions {list(x.shape[:-1])} or of the first of them")
+    _require(scales is None or (scales.dtype == torch.float32 and tuple(scales.shape) == (adapters,)), f"{what}: scales must be float32 [{adapters}]")
+    _same_device(what, x.device, y, a, b, adapter_ids, scales, out)
+    if out is None:
+        out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
+    else:
+        _require(out.shape == y.shape and out.dtype == y.dtype, f"{what}: out must have y's shape and dtype")
+    rows = x.numel() // k
+    if rows == 0:
+        return out
+
+    def aligned(t):   # the kernels move 16 bytes at a time
+        return t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) % 8 == 0)
+
+    xf, yf, of = _rows_of(x, k), _rows_of(y, n), _rows_of(out, n)
+    _require(of.data_ptr() == out.data_ptr() and aligned(of), f"{what}: out must have unit column stride, rows of one stride and 16-byte alignment")
+    xf = xf if aligned(xf) else xf.clone(memory_format=torch.contiguous_format)
+    yf = yf if aligned(yf) else yf.clone(memory_format=torch.contiguous_format)
+    a, b = a.contiguous(), b.contiguous()
+    a = a if a.data_ptr() % 16 == 0 else a.clone()
+    b = b if b.data_ptr() % 16 == 0 else b.clone()
+    ids = adapter_ids.contiguous()
+    scales = None if scales is None else scales.contiguous()
+    _launch(x.device, "launch_lora_add_kernel", _ptr(yf), _ptr(xf), _ptr(a), _ptr(b), _ptr(ids), _ptr(scales), _ptr(of), rows, k, n, rank,
+            adapters, _row_stride(yf), _row_stride(xf), _row_stride(of), rows // ids.numel(), _code(x.dtype, what), ids.dtype == torch.int64)
+    return out
+
+
 def build_constraints() -> dict:
     """What this backend accepts, per function (checked by the registry before dispatch)."""
     from comfy_kitchen.constraints import DivisibleBy, ExactDims, FunctionConstraints, ParamConstraint
@@ -606,6 +828,8 @@ def build_constraints() -> dict:
     rope2 = fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                xk=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),)))
+    positions, radians = frozenset(_POSITION_CODES), ParamConstraint(dtypes=frozenset({torch.float64}), shape_rules=(ExactDims(1),))
+    halves = ParamConstraint(dtypes=frozenset({torch.bfloat16, torch.float16}))
     norm = dict(x=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=floats), shift=ParamConstraint(dtypes=floats))
     return {
         "quantize_per_tensor_fp8": fc(x=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=frozenset({torch.float32})),
@@ -639,6 +863,15 @@ def build_constraints() -> dict:
         "stochastic_rounding_fp8": fc(x=ParamConstraint(dtypes=floats), rng=ParamConstraint(dtypes=frozenset({torch.uint8}))),
         "qk_norm_rope": fc(qkv=ParamConstraint(dtypes=frozenset({torch.bfloat16, torch.float16})),
                            freqs_cis=ParamConstraint(dtypes=frozenset({torch.float32}))),
+        "add_rmsnorm_quantize_mxfp8": fc(x=ParamConstraint(dtypes=floats), residual=ParamConstraint(dtypes=floats),
+                                         weight=ParamConstraint(dtypes=floats)),
+        "add_rmsnorm_quantize_fp8": fc(x=ParamConstraint(dtypes=floats), residual=ParamConstraint(dtypes=floats),
+                                       weight=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=frozenset({torch.float32})),
+                                       output_type=ParamConstraint(dtypes=fp8)),
+        "apply_rope_axes": fc(xq=rope2.params["xq"], xk=rope2.params["xk"], positions=ParamConstraint(dtypes=positions), freqs=radians),
+        "apply_rope_axes1": fc(x=rope.params["x"], positions=ParamConstraint(dtypes=positions), freqs=radians),
+        "lora_add": fc(y=halves, x=halves, a=halves, b=halves, adapter_ids=ParamConstraint(dtypes=frozenset({torch.int32, torch.int64})),
+                       scales=ParamConstraint(dtypes=frozenset({torch.float32}))),
         "quantize_nvfp4_gather": fc(per_tensor_scale=ParamConstraint(dtypes=frozenset({torch.float32}))),
     }
 

@@ -1,0 +1,236 @@
+// Rotary embedding by positions of several axes (time, height, width) for sm_100a, without a table.
+//
+// Pair p of a head belongs to one axis; at token n it turns by  angle = position[n, axis(p)] * freqs[p]:
+//   (a, b) -> (a cos - b sin, a sin + b cos),  (a, b) = (x[2p], x[2p+1])  or, split-half,  (x[p], x[p + P])
+// with P pairs in all; elements from 2P on pass through.  freqs is in radians per unit of position, in 64 bits:
+// at a position of 10^6 a product in 32 bits is already 0.03 rad off.  The turn is reduced to [-1/2, 1/2] in
+// 64 bits (three operations a pair) and only then rounded to fp32, so its sine and cosine are exact to fp32
+// rounding at any position; the rotation is in fp32 with one rounding to x's type.  The inverse rotation (the
+// transpose, which is the gradient's) changes the sine's sign.
+//
+// Bound by HBM: q and k are read and written once (positions are a few bytes a token; rope.cu reads 4 fp32 per
+// pair of table instead).  A thread owns 4 pairs of one token (8 with split-half), computes their sines and cosines
+// once and walks heads of q and k with them, moving 16 bytes of 16-bit data a step.
+#include "ck_common.cuh"
+
+namespace ck {
+namespace {
+
+constexpr int kMaxAxes = 8;
+enum PosType { kPosF32 = 0, kPosF64 = 1, kPosI32 = 2, kPosI64 = 3 };
+
+struct RopeAxesParams {
+    const void* x[2];          // q, k (k may be null)
+    void* o[2];                // contiguous in the order of x's dimensions
+    const void* pos;
+    const double* freqs;       // [P]
+    int64_t sx[2][4];          // element strides of batch, token, head, element
+    int64_t so[2][3];          // output strides of batch, token, head
+    int64_t sp[3];             // position strides of batch, token, axis
+    int64_t batch, tokens;
+    int heads[2];
+    int D, P, n_axes, pos_type;
+    int axis_end[kMaxAxes];    // first pair behind each axis' pairs
+    int n_vec;                 // work items per token and head chunk
+    int chunk, n_chunks;       // heads (of q, then k) one thread walks
+    float sign;                // -1: inverse
+};
+
+__device__ __forceinline__ double position(const RopeAxesParams& p, int64_t off) {
+    switch (p.pos_type) {
+    case kPosF32: return (double)__ldg(static_cast<const float*>(p.pos) + off);
+    case kPosF64: return __ldg(static_cast<const double*>(p.pos) + off);
+    case kPosI32: return (double)__ldg(static_cast<const int*>(p.pos) + off);
+    default: return (double)__ldg(static_cast<const long long*>(p.pos) + off);
+    }
+}
+
+// Cosine and sine of pair `pair` at the token whose positions start at `off`.
+__device__ __forceinline__ float2 pair_turn(const RopeAxesParams& p, int64_t off, int pair) {
+    int axis = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxAxes - 1; ++i)
+        if (i < p.n_axes - 1 && pair >= p.axis_end[i]) axis = i + 1;
+    const double turns = position(p, off + axis * p.sp[2]) * (__ldg(p.freqs + pair) * 0.15915494309189533577 /* 1 / 2 pi */);
+    float s, c;
+    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    return make_float2(c, p.sign * s);
+}
+
+__device__ __forceinline__ void rotate(float2 t, float a, float b, float& oa, float& ob) {
+    oa = fmaf(a, t.x, -__fmul_rn(b, t.y));
+    ob = fmaf(a, t.y, __fmul_rn(b, t.x));
+}
+
+// Where head `head` (q's heads first, then k's) of the item starts in the input and the output.
+template <typename T>
+__device__ __forceinline__ void head_at(const RopeAxesParams& p, int64_t b, int64_t n, int head, const T*& src, T*& dst) {
+    const int which = head < p.heads[0] ? 0 : 1;
+    const int64_t h = which ? head - p.heads[0] : head;
+    src = static_cast<const T*>(p.x[which]) + b * p.sx[which][0] + n * p.sx[which][1] + h * p.sx[which][2];
+    dst = static_cast<T*>(p.o[which]) + b * p.so[which][0] + n * p.so[which][1] + h * p.so[which][2];
+}
+
+// Vectors of 8 elements: unit stride, D (and, split-half, P) a multiple of 8, 16-byte aligned rows.
+template <typename T, bool kSplit>
+__global__ void __launch_bounds__(256) rope_axes_vec_kernel(const RopeAxesParams p) {
+    constexpr int kPairs = kSplit ? 8 : 4;
+    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t site = item / p.n_vec;
+    const int v = (int)(item - site * p.n_vec);
+    if (site >= p.tokens) return;
+    const int64_t b = blockIdx.y / p.n_chunks;
+    const int h0 = (int)(blockIdx.y % p.n_chunks) * p.chunk;
+    const int h1 = min(h0 + p.chunk, p.heads[0] + p.heads[1]);
+
+    // columns of this thread: one vector (interleaved), or the two vectors of a split-half item; behind the
+    // rotated part a split-half item is two neighbouring vectors that pass through
+    const int turning = kSplit ? p.P / 8 : (2 * p.P + 7) / 8;
+    const bool rotates = v < turning;
+    const int lo = kSplit && !rotates ? 2 * p.P + (v - turning) * 16 : v * 8;
+    const int hi = kSplit ? (rotates ? lo + p.P : lo + 8) : lo;
+    const bool second = kSplit && hi < p.D;
+    float2 t[kPairs];
+    if (rotates) {
+        const int64_t off = b * p.sp[0] + site * p.sp[1];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const int pair = v * kPairs + i;
+            t[i] = pair < p.P ? pair_turn(p, off, pair) : make_float2(1.0f, 0.0f);
+        }
+    }
+    constexpr int kBatch = kSplit ? 2 : 4;
+    for (int h = h0; h < h1; h += kBatch) {
+        Raw8<T> ra[kBatch], rb[kBatch];
+        const T* src[kBatch];
+        T* dst[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (h + i >= h1) break;
+            head_at<T>(p, b, site, h + i, src[i], dst[i]);
+            ra[i] = load_raw8<T>(src[i] + lo);
+            if (second) rb[i] = load_raw8<T>(src[i] + hi);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (h + i >= h1) break;
+            float x[8], y[8];
+            unpack8(ra[i], x);
+            if (kSplit) {
+                if (second) unpack8(rb[i], y);
+                if (rotates) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) rotate(t[j], x[j], y[j], x[j], y[j]);
+                }
+                store8<T>(dst[i] + lo, x);
+                if (second) store8<T>(dst[i] + hi, y);
+            } else {
+                if (rotates) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (v * 4 + j < p.P) rotate(t[j], x[2 * j], x[2 * j + 1], x[2 * j], x[2 * j + 1]);
+                }
+                store8<T>(dst[i] + lo, x);
+            }
+        }
+    }
+}
+
+// Any strides, any even D: one pair per thread and head; a thread behind the pairs copies two elements.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_axes_generic_kernel(const RopeAxesParams p, const bool split) {
+    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t site = item / p.n_vec;
+    const int pair = (int)(item - site * p.n_vec);
+    if (site >= p.tokens) return;
+    const int64_t b = blockIdx.y / p.n_chunks;
+    const int h0 = (int)(blockIdx.y % p.n_chunks) * p.chunk;
+    const int h1 = min(h0 + p.chunk, p.heads[0] + p.heads[1]);
+    const bool rotates = pair < p.P;
+    const int ia = split && rotates ? pair : 2 * pair, ib = split && rotates ? pair + p.P : 2 * pair + 1;
+    const float2 t = rotates ? pair_turn(p, b * p.sp[0] + site * p.sp[1], pair) : make_float2(1.0f, 0.0f);
+    for (int h = h0; h < h1; ++h) {
+        const T* src;
+        T* dst;
+        head_at<T>(p, b, site, h, src, dst);
+        const int64_t se = p.sx[h < p.heads[0] ? 0 : 1][3];
+        const T a = src[ia * se], c = src[ib * se];
+        if (rotates) {
+            float oa, oc;
+            rotate(t, Elem<T>::to_f32(a), Elem<T>::to_f32(c), oa, oc);
+            dst[ia] = Elem<T>::from_f32(oa);
+            dst[ib] = Elem<T>::from_f32(oc);
+        } else {
+            dst[ia] = a;
+            dst[ib] = c;
+        }
+    }
+}
+
+template <typename T>
+int launch(RopeAxesParams p, bool split, bool vec, cudaStream_t stream) {
+    p.n_vec = vec ? (split ? p.P / 8 + (int)ceil_div(p.D - 2 * p.P, 16) : p.D / 8) : p.D / 2;
+    const int heads = p.heads[0] + p.heads[1];
+    // Heads are split over threads until the machine is full (about 1024 threads an SM), but not below 4 a thread.
+    const int64_t sites = p.batch * p.tokens * p.n_vec;
+    int64_t chunks = ceil_div(148LL * 1024, sites);
+    if (chunks > ceil_div(heads, 4)) chunks = ceil_div(heads, 4);
+    if (chunks > 65535 / p.batch) chunks = 65535 / p.batch;   // (batch x chunks is a grid dimension)
+    if (chunks < 1) chunks = 1;
+    p.chunk = (int)ceil_div(heads, chunks);
+    p.n_chunks = (int)ceil_div(heads, p.chunk);
+    const int64_t gx = ceil_div(p.tokens * p.n_vec, 256), gy = p.batch * p.n_chunks;
+    if (gx > 0x7fffffff) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: %lld tokens are more than a grid holds", (long long)p.tokens);
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (!vec) rope_axes_generic_kernel<T><<<grid, 256, 0, stream>>>(p, split);
+    else if (split) rope_axes_vec_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+    else rope_axes_vec_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    return launch_status("apply_rope_axes");
+}
+
+}  // namespace
+}  // namespace ck
+
+extern "C" int launch_apply_rope_axes_kernel(const void* xq, const void* xk, const void* positions, const double* freqs,
+                                             void* xq_out, void* xk_out, const int64_t* strides, int64_t batch, int64_t tokens,
+                                             int64_t heads_q, int64_t heads_k, int64_t head_dim, const int32_t* axis_pairs,
+                                             int n_axes, int dtype_code, int positions_code, bool split_half, bool inverse,
+                                             cudaStream_t stream) {
+    using namespace ck;
+    if (!xq || !positions || !freqs || !xq_out || !strides || !axis_pairs) CK_FAIL(CK_ERR_NULL, "apply_rope_axes: null pointer");
+    if ((xk == nullptr) != (xk_out == nullptr) || (xk == nullptr) != (heads_k == 0))
+        CK_FAIL(CK_ERR_NULL, "apply_rope_axes: xk, xk_out and heads_k must be given together");
+    if (batch <= 0 || batch > 65535 || tokens <= 0 || tokens > (1LL << 40) || heads_q <= 0 || heads_k < 0 || heads_q > 65535 || heads_k > 65535 || head_dim <= 0 ||
+        head_dim % 2 != 0 || head_dim > 65536)
+        CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: bad shape batch=%lld tokens=%lld heads=%lld/%lld head_dim=%lld (even)", (long long)batch,
+                (long long)tokens, (long long)heads_q, (long long)heads_k, (long long)head_dim);
+    if (n_axes < 1 || n_axes > kMaxAxes) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: %d axes (1 to %d)", n_axes, kMaxAxes);
+    if (positions_code < kPosF32 || positions_code > kPosI64) CK_FAIL(CK_ERR_DTYPE, "apply_rope_axes: positions type code %d", positions_code);
+    RopeAxesParams p{};
+    int64_t pairs = 0;
+    for (int i = 0; i < n_axes; ++i) {
+        if (axis_pairs[i] <= 0) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: axis %d has %d pairs", i, (int)axis_pairs[i]);
+        pairs += axis_pairs[i];
+        if (2 * pairs > head_dim) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: the axes turn more than %lld elements", (long long)head_dim);
+        p.axis_end[i] = (int)pairs;
+    }
+    p.x[0] = xq; p.x[1] = xk; p.o[0] = xq_out; p.o[1] = xk_out;
+    p.pos = positions; p.freqs = freqs;
+    // strides: q (batch, token, head, element), k (the same), q_out (batch, token, head), k_out, positions (batch, token, axis)
+    for (int i = 0; i < 4; ++i) { p.sx[0][i] = strides[i]; p.sx[1][i] = strides[4 + i]; }
+    for (int i = 0; i < 3; ++i) { p.so[0][i] = strides[8 + i]; p.so[1][i] = strides[11 + i]; p.sp[i] = strides[14 + i]; }
+    p.batch = batch; p.tokens = tokens; p.heads[0] = (int)heads_q; p.heads[1] = (int)heads_k;
+    p.D = (int)head_dim; p.P = (int)pairs; p.n_axes = n_axes; p.pos_type = positions_code;
+    p.sign = inverse ? -1.0f : 1.0f;
+    bool vec = head_dim % 8 == 0 && (!split_half || pairs % 8 == 0);
+    for (int w = 0; w < (xk ? 2 : 1); ++w) {
+        vec = vec && aligned16(p.x[w]) && aligned16(p.o[w]) && p.sx[w][3] == 1;
+        for (int i = 0; i < 3; ++i) vec = vec && p.sx[w][i] % 8 == 0 && p.so[w][i] % 8 == 0;
+    }
+    switch (dtype_code) {
+    case CK_F32: return launch<float>(p, split_half, vec, stream);
+    case CK_F16: return launch<__half>(p, split_half, vec, stream);
+    case CK_BF16: return launch<__nv_bfloat16>(p, split_half, vec, stream);
+    default: CK_FAIL(CK_ERR_DTYPE, "apply_rope_axes: unsupported dtype code %d", dtype_code);
+    }
+}

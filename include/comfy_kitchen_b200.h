@@ -167,6 +167,19 @@ int launch_apply_rope_kernel(const void* xq, const void* xk, const void* freqs, 
                              int64_t stride_freqs_rot, int64_t stride_freqs_pair, int input_dtype_code,
                              int freqs_dtype_code, bool split_half, ck_stream_t stream);
 
+/* Rotation by positions of several axes (time, height, width), computed in the kernel instead of read from a table.
+ * No counterpart in the reference (its apply_rope reads [.., head_dim/2, 2, 2] matrices; the formula is
+ * backends/eager/rope.py:9-32 with F = [[cos, -sin], [sin, cos]]).  Pair p turns by position[axis(p)] * freqs[p] radians;
+ * axis i owns the next axis_pairs[i] pairs (1 to 8 axes); elements behind the pairs are copied.  freqs: float64
+ * [pairs].  positions_code: 0 float32, 1 float64, 2 int32, 3 int64.  strides (HOST array of 17, in elements): xq batch,
+ * token, head, element; xk the same; xq_out batch, token, head; xk_out the same (outputs have unit element stride);
+ * positions batch, token, axis.  xk / xk_out may both be NULL (heads_k = 0).  axis_pairs: HOST array.  inverse: rotate
+ * back (the transpose, i.e. the gradient's rotation). */
+int launch_apply_rope_axes_kernel(const void* xq, const void* xk, const void* positions, const double* freqs, void* xq_out,
+                                  void* xk_out, const int64_t* strides, int64_t batch, int64_t tokens, int64_t heads_q,
+                                  int64_t heads_k, int64_t head_dim, const int32_t* axis_pairs, int n_axes, int dtype_code,
+                                  int positions_code, bool split_half, bool inverse, ck_stream_t stream);
+
 /* Per-head RMSNorm of q and k + RoPE of both + relayout of q, k, v for attention, one pass.
  * No single counterpart in the reference: it composes apply_rope (backends/eager/rope.py:9-32)
  * with torch's rms_norm and the caller's permutes.  qkv: [tokens, >= 3*heads*128] with row_stride
@@ -211,10 +224,31 @@ int launch_adaln_quantize_mxfp8_kernel(const void* x, const void* scale, const v
                                        void* block_scales, int64_t N, int64_t D, int64_t scale_group,
                                        int64_t shift_group, float eps, int dtype_code, int norm_kind,
                                        ck_stream_t stream);
+/* Residual addition + RMSNorm + 8-bit output in one pass (no counterpart in the reference).  h = x + residual rounded to the
+ * residual's type and written to sum_out; y = rmsnorm(h) * weight rounded to x's type (written to norm_out unless NULL);
+ * output: block_scales given: the bytes of launch_quantize_mxfp8_kernel on y (E4M3, tiled E8M0 scales, padding
+ * written; D a multiple of 32), else those of launch_quantize_fp8_kernel on y with the device scalar scale (any D).
+ * x [N, D] and residual [N, D] have unit column stride and the given row strides; sum_out, norm_out, output are
+ * contiguous; sum_out may be the residual itself if that is contiguous.  residual_dtype_code: x's or fp32; weight [D] in x's
+ * type or NULL. */
+int launch_add_rmsnorm_quantize_kernel(const void* x, const void* residual, const void* weight, const void* scale,
+                                       void* sum_out, void* norm_out, void* output, void* block_scales, int64_t N, int64_t D,
+                                       int64_t x_row_stride, int64_t residual_row_stride, float eps, int dtype_code,
+                                       int residual_dtype_code, int output_dtype_code, ck_stream_t stream);
 /* Synchronises the device, reads and clears the norm kernels' status word.  Returns 0, or
  * CK_ERR_DEVICE_TIMEOUT when a bounded device-side wait on a row copy ran out since the last
  * call (the rows concerned were not written), or a positive cudaError_t. */
 int ck_norm_device_status(void);
+
+/* ---- low-rank adapters (no counterpart in the reference) ----
+ * out[t] = y[t] + scales[a] * B_a (A_a x[t]) for every row, a = ids[t / rows_per_id]; out[t] = y[t] where a lies outside
+ * [0, adapters).  y: [rows, N], the shared projection's output; x: [rows, K]; a: [adapters, rank, K]; b: [adapters, N, rank];
+ * all bf16 or all fp16, 16-byte aligned, row strides (elements) multiples of 8; ids: int32 or int64; scales: fp32
+ * [adapters] or NULL (ones); out may be y.  K, N, rank multiples of 8, rank at most 256. */
+int launch_lora_add_kernel(const void* y, const void* x, const void* a, const void* b, const void* ids, const float* scales,
+                           void* out, int64_t rows, int64_t K, int64_t N, int64_t rank, int64_t adapters, int64_t y_row_stride,
+                           int64_t x_row_stride, int64_t out_row_stride, int64_t rows_per_id, int dtype_code, bool ids_64bit,
+                           ck_stream_t stream);
 
 /* ---- tensor-parallel exchange (no counterpart in the reference, which has no multi-GPU code) ----
  * Stands where a tensor-parallel port would call ncclAllReduce on the row-parallel GEMM's output and
