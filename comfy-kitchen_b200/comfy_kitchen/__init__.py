@@ -102,12 +102,11 @@ def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: 
     """h = x + residual; ``quantize_mxfp8(rmsnorm(h, weight, eps).reshape(-1, D))`` in one pass.
     -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``residual`` and h
     have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to, e.g. ``residual`` itself."""
-    if sum_out is None:
+    if sum_out is None and not _Ops._plain((x, residual, weight)):
         got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
-    else:
-        impl = registry.get_implementation("add_rmsnorm_quantize_mxfp8", kwargs={"x": x, "residual": residual, "weight": weight})
-        got = impl(x, residual, weight, eps, return_norm, sum_out)
-    return got if return_norm else got[:-1]
+        return got if return_norm else got[:-1]
+    impl = registry.get_implementation("add_rmsnorm_quantize_mxfp8", kwargs={"x": x, "residual": residual, "weight": weight})
+    return impl(x, residual, weight, eps, return_norm, sum_out)
 
 
 def add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor,
@@ -115,13 +114,12 @@ def add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: to
                              sum_out: torch.Tensor | None = None):
     """h = x + residual; ``quantize_per_tensor_fp8(rmsnorm(h, weight, eps), scale, output_type)`` in one pass.
     -> (data, h), and the normalised h behind them with ``return_norm``; see ``add_rmsnorm_quantize_mxfp8``."""
-    if sum_out is None:
+    if sum_out is None and not _Ops._plain((x, residual, weight, scale)):
         got = _ops_ns.add_rmsnorm_quantize_fp8(x, residual, weight, scale, eps, DTYPE_TO_CODE[output_type], return_norm)
-    else:
-        impl = registry.get_implementation("add_rmsnorm_quantize_fp8", kwargs={"x": x, "residual": residual, "weight": weight, "scale": scale,
-                                                                               "output_type": output_type})
-        got = impl(x, residual, weight, scale, eps, output_type, return_norm, sum_out)
-    return got if return_norm else got[:-1]
+        return got if return_norm else got[:-1]
+    impl = registry.get_implementation("add_rmsnorm_quantize_fp8", kwargs={"x": x, "residual": residual, "weight": weight, "scale": scale,
+                                                                           "output_type": output_type})
+    return impl(x, residual, weight, scale, eps, output_type, return_norm, sum_out)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
@@ -129,7 +127,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """y + scales[i] * (x @ a[i].T) @ b[i].T with i the row's adapter id: the low-rank adapters of many requests beside
     a shared projection y [..., N] of x [..., K].  a: [L, R, K]; b: [L, N, R]; adapter_ids: int32 or int64, one per row
     or per leading index (outside [0, L): no adapter); ``out`` may be y."""
-    if out is None:
+    if out is None and not _Ops._plain((y, x, a, b, adapter_ids, scales)):
         return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
     impl = registry.get_implementation("lora_add", kwargs={"y": y, "x": x, "a": a, "b": b, "adapter_ids": adapter_ids, "scales": scales})
     return impl(y, x, a, b, adapter_ids, scales, out)
@@ -236,12 +234,18 @@ def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, positions: torch.Tensor,
     """RoPE of q and k by positions [N, A] or [B, N, A] on A axes, without a table: pair p of a head turns by
     positions[n, axis of p] * freqs[p].  x: [B, H, N, D] (``tokens_dim`` 2) or [B, N, H, D] (1), any strides; k may have
     fewer heads; elements behind sum(axes_dim) pass through.  ``inverse`` rotates back."""
-    return _ops_ns.apply_rope_axes(xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
+    if not _Ops._plain((xq, xk, positions, freqs)):
+        return _ops_ns.apply_rope_axes(xq, xk, positions, freqs, list(axes_dim), split_half, tokens_dim, inverse)
+    impl = registry.get_implementation("apply_rope_axes", kwargs={"xq": xq, "xk": xk, "positions": positions, "freqs": freqs})
+    return impl(xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
 
 
 def apply_rope_axes1(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes_dim, split_half: bool = False,
                      tokens_dim: int = 2, inverse: bool = False) -> torch.Tensor:
-    return _ops_ns.apply_rope_axes1(x, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
+    if not _Ops._plain((x, positions, freqs)):
+        return _ops_ns.apply_rope_axes1(x, positions, freqs, list(axes_dim), split_half, tokens_dim, inverse)
+    impl = registry.get_implementation("apply_rope_axes1", kwargs={"x": x, "positions": positions, "freqs": freqs})
+    return impl(x, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
 
 
 # ------------------------------------------------------------------ backend configuration

@@ -87,7 +87,7 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke an entry point; raise RuntimeError with the library's message on failure."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.ck_last_error().decode(errors="replace")

@@ -234,7 +234,8 @@ def _(x, rng, output_type):
 @torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_mxfp8", mutates_args=())
 def _op_add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float,
                                    return_norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _dispatch("add_rmsnorm_quantize_mxfp8", x=x, residual=residual, weight=weight, eps=eps, return_norm=return_norm)
+    got = _dispatch("add_rmsnorm_quantize_mxfp8", x=x, residual=residual, weight=weight, eps=eps, return_norm=return_norm)
+    return got if return_norm else (*got, x.new_empty(0))
 
 
 @_op_add_rmsnorm_quantize_mxfp8.register_fake
@@ -250,8 +251,9 @@ def _(x, residual, weight, eps, return_norm):
 @torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_fp8", mutates_args=())
 def _op_add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor, eps: float,
                                  output_dtype_code: int, return_norm: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _dispatch("add_rmsnorm_quantize_fp8", x=x, residual=residual, weight=weight, scale=scale, eps=eps,
-                     output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code], return_norm=return_norm)
+    got = _dispatch("add_rmsnorm_quantize_fp8", x=x, residual=residual, weight=weight, scale=scale, eps=eps,
+                    output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code], return_norm=return_norm)
+    return got if return_norm else (*got, x.new_empty(0))
 
 
 @_op_add_rmsnorm_quantize_fp8.register_fake

@@ -39,7 +39,8 @@ def _ptr(t: torch.Tensor | None):
 
 
 def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    # the raw handle: torch.cuda.current_stream builds a Stream object on the way to the same number (2.4 against 0.1 us)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index))
 
 
 def _code(dtype: torch.dtype, what: str) -> int:
@@ -50,6 +51,8 @@ def _code(dtype: torch.dtype, what: str) -> int:
 
 
 def _plain(t):
+    if type(t) is torch.Tensor:   # (the instance check of Parameter is a Python call of its own, 0.7 us)
+        return t
     return t.data if isinstance(t, torch.nn.Parameter) else t
 
 
@@ -592,15 +595,16 @@ def rmsnorm_quantize_nvfp4(
 # ------------------------------------------------------------------ around a quantized linear, when serving
 
 
-def _require(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
+# A call of these runs for a few microseconds on the GPU when one token is served, so their host side is kept short: shapes
+# are read once, addresses go to ctypes as plain integers, and the checks that format a message do so only when they fail.
 
 
 def _no_grad(what: str, *tensors) -> None:
     """These entry points record no gradient; a call that would drop one is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def _same_device(what: str, device, *tensors) -> None:
@@ -611,11 +615,12 @@ def _same_device(what: str, device, *tensors) -> None:
 
 def _launch(device, name: str, *args) -> None:
     """_native.call with ``device`` current, on its current stream (appended as the last argument)."""
-    if device.index == torch.cuda.current_device():
-        _native.call(name, *args, _stream(device))
+    index = device.index
+    if index == torch.cuda.current_device():
+        _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _native.call(name, *args, _stream(device))
+            _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -625,114 +630,131 @@ def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
             t = t.view(-1, width)
         except RuntimeError:
             return t.reshape(-1, width).contiguous()
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+    if not t.is_contiguous() and (t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width)):
         t = t.contiguous()
     return t
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _row_stride(t: torch.Tensor, width: int) -> int:
+    return t.stride(0) if t.shape[0] > 1 else width
 
 
 def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm, sum_out):
-    x, residual, weight = _plain(x), _plain(residual), _plain(weight)
-    _no_grad(what, x, residual, weight)
-    _require(x.dim() >= 1 and x.shape == residual.shape, f"{what}: x {tuple(x.shape)} and residual {tuple(residual.shape)} must have the same shape")
-    _require(residual.dtype in (x.dtype, torch.float32), f"{what}: the residual has x's dtype or float32, got {residual.dtype}")
-    d = x.shape[-1]
-    n = x.numel() // d if d else 0
-    mx = scale is None
-    _require(d > 0 and (not mx or d % 32 == 0), f"{what}: last dim must be positive{' and divisible by 32' if mx else ''}, got {d}")
-    _require(weight is None or tuple(weight.shape) == (d,), f"{what}: weight must be [{d}]")
-    _same_device(what, x.device, residual, weight, sum_out)
+    x, residual = _plain(x), _plain(residual)
+    shape, dtype, device, stream_dtype = x.shape, x.dtype, x.device, residual.dtype
+    if shape != residual.shape or not shape:
+        raise ValueError(f"{what}: x {tuple(shape)} and residual {tuple(residual.shape)} must have the same shape")
+    if stream_dtype != dtype and stream_dtype != torch.float32:
+        raise ValueError(f"{what}: the residual has x's dtype or float32, got {stream_dtype}")
+    d, mx = shape[-1], scale is None
+    if d == 0 or (mx and d % 32):
+        raise ValueError(f"{what}: last dim must be positive{' and divisible by 32' if mx else ''}, got {d}")
+    n = x.numel() // d
     if weight is not None:
-        weight = weight.to(x.dtype).contiguous()
+        weight = _plain(weight)
+        if weight.shape != (d,):
+            raise ValueError(f"{what}: weight must be [{d}], got {list(weight.shape)}")
+        if weight.dtype != dtype or not weight.is_contiguous():
+            weight = weight.to(dtype).contiguous()
+    _no_grad(what, x, residual, weight)
+    _same_device(what, device, residual, weight, sum_out)
     if sum_out is None:
-        sum_out = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
-    else:
-        _require(sum_out.shape == x.shape and sum_out.dtype == residual.dtype and sum_out.is_contiguous(),
-                 f"{what}: sum_out must be contiguous with the residual's shape and dtype")
-    norm = torch.empty(x.shape if return_norm else (0,), device=x.device, dtype=x.dtype)
-    q = torch.empty((n, d) if mx else x.shape, device=x.device, dtype=torch.uint8)
-    sx = torch.empty((roundup(n, 128), roundup(d // 32, 4)), device=x.device, dtype=torch.uint8) if mx else None
+        sum_out = torch.empty_like(residual) if residual.is_contiguous() else residual.new_empty(shape)
+    elif sum_out.shape != shape or sum_out.dtype != stream_dtype or not sum_out.is_contiguous():
+        raise ValueError(f"{what}: sum_out must be contiguous with the residual's shape and dtype")
+    norm = x.new_empty(shape) if return_norm else None
+    q = x.new_empty((n, d) if mx else shape, dtype=output_type)
+    sx = x.new_empty((roundup(n, 128), roundup(d // 32, 4)), dtype=torch.float8_e8m0fnu) if mx else None
     if n:
         xf, rf = _rows_of(x, d), _rows_of(residual, d)
-        _launch(x.device, "launch_add_rmsnorm_quantize_kernel", _ptr(xf), _ptr(rf), _ptr(weight), _ptr(scale), _ptr(sum_out),
-                _ptr(norm if return_norm else None), _ptr(q), _ptr(sx), n, d, _row_stride(xf), _row_stride(rf), float(eps),
-                _code(x.dtype, what), _code(residual.dtype, what), DTYPE_TO_CODE[output_type])
-    return q.view(output_type), sx, sum_out, norm
+        _launch(device, "launch_add_rmsnorm_quantize_kernel", xf.data_ptr(), rf.data_ptr(), 0 if weight is None else weight.data_ptr(),
+                0 if mx else scale.data_ptr(), sum_out.data_ptr(), norm.data_ptr() if return_norm else 0, q.data_ptr(),
+                sx.data_ptr() if mx else 0, n, d, _row_stride(xf, d), _row_stride(rf, d), eps, _code(dtype, what),
+                _code(stream_dtype, what), DTYPE_TO_CODE[output_type])
+    return q, sx, sum_out, norm
 
 
 def add_rmsnorm_quantize_mxfp8(
     x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
     return_norm: bool = False, sum_out: torch.Tensor | None = None,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """h = x + residual; quantize_mxfp8(rmsnorm(h, weight, eps)) in one pass -> (data, block scales, h, normalised h).
+):
+    """h = x + residual; quantize_mxfp8(rmsnorm(h, weight, eps)) in one pass -> (data, block scales, h), and with
+    ``return_norm`` the normalised h behind them.
 
     ``residual`` (and h) has x's dtype or float32; the norm is taken of h as stored and rounded to x's dtype before it
-    is quantized.  The last output is empty unless ``return_norm``.  ``sum_out``: a contiguous tensor for h, which may
-    be ``residual`` itself.
+    is quantized.  ``sum_out``: a contiguous tensor for h, which may be ``residual`` itself.
     """
     q, sx, h, norm = _add_rmsnorm("add_rmsnorm_quantize_mxfp8", x, residual, weight, eps, None, torch.float8_e4m3fn, return_norm, sum_out)
-    return q, sx.view(torch.float8_e8m0fnu), h, norm
+    return (q, sx, h, norm) if return_norm else (q, sx, h)
 
 
 def add_rmsnorm_quantize_fp8(
     x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor, eps: float = 1e-6,
     output_type: torch.dtype = torch.float8_e4m3fn, return_norm: bool = False, sum_out: torch.Tensor | None = None,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """The same with quantize_per_tensor_fp8(normalised h, scale, output_type): -> (data in x's shape, h, normalised h)."""
+):
+    """The same with quantize_per_tensor_fp8(normalised h, scale, output_type): -> (data in x's shape, h[, normalised h])."""
     if output_type not in (torch.float8_e4m3fn, torch.float8_e5m2):
         raise ValueError(f"Unsupported output_type: {output_type}. Expected torch.float8_e4m3fn or torch.float8_e5m2")
     scale = _scalar_on(scale, x.device)
-    _require(scale.numel() == 1, "add_rmsnorm_quantize_fp8: scale must be a scalar tensor")
+    if scale.numel() != 1:
+        raise ValueError("add_rmsnorm_quantize_fp8: scale must be a scalar tensor")
     q, _, h, norm = _add_rmsnorm("add_rmsnorm_quantize_fp8", x, residual, weight, eps, scale, output_type, return_norm, sum_out)
-    return q, h, norm
+    return (q, h, norm) if return_norm else (q, h)
 
 
+_Strides, _Pairs = ctypes.c_int64 * 17, ctypes.c_int32 * 8
 _POSITION_CODES = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
 
 
 def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse):
-    xq, xk = _plain(xq), _plain(xk)
-    _no_grad(what, xq, xk, positions, freqs)
-    _require(tokens_dim in (1, 2), f"{what}: tokens_dim is 2 for [B, H, N, D] or 1 for [B, N, H, D], got {tokens_dim}")
+    xq = _plain(xq)
+    if tokens_dim != 1 and tokens_dim != 2:
+        raise ValueError(f"{what}: tokens_dim is 2 for [B, H, N, D] or 1 for [B, N, H, D], got {tokens_dim}")
     heads_dim = 3 - tokens_dim
-    _require(xq.dim() == 4 and (xk is None or xk.dim() == 4), f"{what}: x must have four dimensions")
-    b, n, d = xq.shape[0], xq.shape[tokens_dim], xq.shape[3]
-    _require(xk is None or (xk.dtype == xq.dtype and (xk.shape[0], xk.shape[tokens_dim], xk.shape[3]) == (b, n, d)),
-             f"{what}: q and k must agree in dtype and all dimensions but the heads")
-    axes = [int(a) for a in axes_dim]
-    _require(1 <= len(axes) <= 8 and all(a > 0 and a % 2 == 0 for a in axes) and sum(axes) <= d and d % 2 == 0,
-             f"{what}: axes_dim {axes} must be 1 to 8 positive even sizes that add up to at most the (even) head dim {d}")
-    _require(freqs.dtype == torch.float64 and tuple(freqs.shape) == (sum(axes) // 2,), f"{what}: freqs must be float64 [{sum(axes) // 2}], one per pair")
-    if positions.dim() == 2:
-        positions = positions[None]
-    _require(positions.dim() == 3 and positions.shape[0] in (1, b) and tuple(positions.shape[1:]) == (n, len(axes)),
-             f"{what}: positions must be [{n}, {len(axes)}], [1, {n}, {len(axes)}] or [{b}, {n}, {len(axes)}], got {list(positions.shape)}")
-    _require(positions.dtype in _POSITION_CODES, f"{what}: positions must be float32, float64, int32 or int64")
-    _same_device(what, xq.device, xk, positions, freqs)
-    oq = torch.empty(xq.shape, device=xq.device, dtype=xq.dtype)
-    ok = None if xk is None else torch.empty(xk.shape, device=xq.device, dtype=xq.dtype)
-    heads_q, heads_k = xq.shape[heads_dim], 0 if xk is None else xk.shape[heads_dim]
-    if oq.numel() == 0 or (ok is not None and ok.numel() == 0):
+    q_shape, dtype, device = xq.shape, xq.dtype, xq.device
+    if len(q_shape) != 4 or (xk is not None and xk.dim() != 4):
+        raise ValueError(f"{what}: x must have four dimensions")
+    b, n, d, heads_q, heads_k = q_shape[0], q_shape[tokens_dim], q_shape[3], q_shape[heads_dim], 0
+    if xk is not None:
+        xk = _plain(xk)
+        k_shape = xk.shape
+        heads_k = k_shape[heads_dim]
+        if xk.dtype != dtype or k_shape[0] != b or k_shape[tokens_dim] != n or k_shape[3] != d:
+            raise ValueError(f"{what}: q and k must agree in dtype and all dimensions but the heads")
+    turned, count = sum(axes_dim), len(axes_dim)
+    if not 1 <= count <= 8 or turned > d or d % 2 or any(a <= 0 or a % 2 for a in axes_dim):
+        raise ValueError(f"{what}: axes_dim {list(axes_dim)} must be 1 to 8 positive even sizes that add up to at most the (even) head dim {d}")
+    if freqs.dtype != torch.float64 or freqs.shape != (turned // 2,):
+        raise ValueError(f"{what}: freqs must be float64 [{turned // 2}], one per pair")
+    p_shape = positions.shape
+    if len(p_shape) == 2:
+        p_shape = (1, *p_shape)
+    if len(p_shape) != 3 or (p_shape[0] != 1 and p_shape[0] != b) or p_shape[1] != n or p_shape[2] != count:
+        raise ValueError(f"{what}: positions must be [{n}, {count}], [1, {n}, {count}] or [{b}, {n}, {count}], got {list(positions.shape)}")
+    code = _POSITION_CODES.get(positions.dtype)
+    if code is None:
+        raise ValueError(f"{what}: positions must be float32, float64, int32 or int64")
+    _no_grad(what, xq, xk, positions, freqs)
+    _same_device(what, device, xk, positions, freqs)
+    oq = xq.new_empty(q_shape)
+    ok = None if xk is None else xk.new_empty(k_shape)
+    if b == 0 or n == 0 or d == 0 or heads_q == 0 or (xk is not None and heads_k == 0):
         if oq.numel():
-            return _rope_axes(what, xq, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)[0], ok
-        if ok is not None and ok.numel():
-            return oq, _rope_axes(what, xk, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)[0]
+            oq, _ = _rope_axes(what, xq, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
+        elif ok is not None and ok.numel():
+            ok, _ = _rope_axes(what, xk, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
         return oq, ok
-
-    def order(s):
-        return (s[0], s[tokens_dim], s[heads_dim])
-
-    freqs = freqs.contiguous()
+    if not freqs.is_contiguous():
+        freqs = freqs.contiguous()
     sq, sp = xq.stride(), positions.stride()
     sk = sq if xk is None else xk.stride()
-    strides = (ctypes.c_int64 * 17)(*order(sq), sq[3], *order(sk), sk[3], *order(oq.stride()), *order((oq if ok is None else ok).stride()),
-                                    0 if positions.shape[0] == 1 else sp[0], sp[1], sp[2])
-    _launch(xq.device, "launch_apply_rope_axes_kernel", _ptr(xq), _ptr(xk), _ptr(positions), _ptr(freqs), _ptr(oq), _ptr(ok), strides,
-            b, n, heads_q, heads_k, d, (ctypes.c_int32 * len(axes))(*[a // 2 for a in axes]), len(axes), _code(xq.dtype, what),
-            _POSITION_CODES[positions.dtype], bool(split_half), bool(inverse))
+    # contiguous outputs: [B, H, N, D] or [B, N, H, D]
+    (to, ho), (tk, hk) = ((d, n * d), (d, n * d)) if tokens_dim == 2 else ((heads_q * d, d), (heads_k * d, d))
+    strides = _Strides(sq[0], sq[tokens_dim], sq[heads_dim], sq[3], sk[0], sk[tokens_dim], sk[heads_dim], sk[3], heads_q * n * d, to, ho,
+                       heads_k * n * d, tk, hk, 0 if p_shape[0] == 1 else sp[0], sp[-2], sp[-1])
+    _launch(device, "launch_apply_rope_axes_kernel", xq.data_ptr(), 0 if xk is None else xk.data_ptr(), positions.data_ptr(), freqs.data_ptr(),
+            oq.data_ptr(), 0 if xk is None else ok.data_ptr(), strides, b, n, heads_q, heads_k, d, _Pairs(*[a // 2 for a in axes_dim]), count,
+            _code(dtype, what), code, split_half, inverse)
     return oq, ok
 
 
@@ -771,42 +793,53 @@ def lora_add(
     """
     what = "lora_add"
     y, x, a, b = _plain(y), _plain(x), _plain(a), _plain(b)
+    x_shape, y_shape, a_shape, b_shape, dtype, device = x.shape, y.shape, a.shape, b.shape, x.dtype, x.device
+    if len(a_shape) != 3 or len(b_shape) != 3 or not x_shape:
+        raise ValueError(f"{what}: a must be [L, R, K] and b [L, N, R]")
+    (adapters, rank, k), n = a_shape, b_shape[1]
+    if b_shape[0] != adapters or b_shape[2] != rank:
+        raise ValueError(f"{what}: a {list(a_shape)} and b {list(b_shape)} do not match")
+    if x_shape[-1] != k:
+        raise ValueError(f"{what}: x has {x_shape[-1]} columns, a {k}")
+    if y_shape[:-1] != x_shape[:-1] or y_shape[-1] != n:
+        raise ValueError(f"{what}: y must be {[*x_shape[:-1], n]}, got {list(y_shape)}")
+    if y.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+        raise ValueError(f"{what}: y, x, a and b must have one dtype")
+    if adapters == 0 or not 0 < rank <= 256 or rank % 8 or k == 0 or k % 8 or n == 0 or n % 8:
+        raise ValueError(f"{what}: K, N and R must be multiples of 8 and R at most 256, got {k}, {n}, {rank} of {adapters} adapters")
+    ids_dtype, ids_shape = adapter_ids.dtype, adapter_ids.shape
+    if ids_dtype != torch.int32 and ids_dtype != torch.int64:
+        raise ValueError(f"{what}: adapter_ids must be int32 or int64")
+    if len(ids_shape) >= len(x_shape) or ids_shape != x_shape[:len(ids_shape)]:
+        raise ValueError(f"{what}: adapter_ids {list(ids_shape)} must have the shape of x's leading dimensions {list(x_shape[:-1])} or of the first of them")
+    if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,)):
+        raise ValueError(f"{what}: scales must be float32 [{adapters}]")
     _no_grad(what, y, x, a, b, scales)
-    _require(x.dim() >= 1 and a.dim() == 3 and b.dim() == 3, f"{what}: a must be [L, R, K] and b [L, N, R]")
-    (adapters, rank, k), n = a.shape, b.shape[1]
-    _require(tuple(b.shape) == (adapters, n, rank), f"{what}: a {list(a.shape)} and b {list(b.shape)} do not match")
-    _require(x.shape[-1] == k, f"{what}: x has {x.shape[-1]} columns, a {k}")
-    _require(y.shape == (*x.shape[:-1], n), f"{what}: y must be {[*x.shape[:-1], n]}, got {list(y.shape)}")
-    _require(x.dtype == y.dtype == a.dtype == b.dtype, f"{what}: y, x, a and b must have one dtype")
-    _require(adapters > 0 and 0 < rank <= 256 and rank % 8 == 0 and k > 0 and k % 8 == 0 and n > 0 and n % 8 == 0,
-             f"{what}: K, N and R must be multiples of 8 and R at most 256, got {k}, {n}, {rank} of {adapters} adapters")
-    _require(adapter_ids.dtype in (torch.int32, torch.int64), f"{what}: adapter_ids must be int32 or int64")
-    _require(adapter_ids.dim() < x.dim() and adapter_ids.shape == x.shape[:adapter_ids.dim()],
-             f"{what}: adapter_ids {list(adapter_ids.shape)} must have the shape of x's leading dimensions {list(x.shape[:-1])} or of the first of them")
-    _require(scales is None or (scales.dtype == torch.float32 and tuple(scales.shape) == (adapters,)), f"{what}: scales must be float32 [{adapters}]")
-    _same_device(what, x.device, y, a, b, adapter_ids, scales, out)
+    _same_device(what, device, y, a, b, adapter_ids, scales, out)
     if out is None:
-        out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
-    else:
-        _require(out.shape == y.shape and out.dtype == y.dtype, f"{what}: out must have y's shape and dtype")
+        out = y.new_empty(y_shape)
+    elif out.shape != y_shape or out.dtype != dtype:
+        raise ValueError(f"{what}: out must have y's shape and dtype")
     rows = x.numel() // k
     if rows == 0:
         return out
 
     def aligned(t):   # the kernels move 16 bytes at a time
-        return t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) % 8 == 0)
+        return t.data_ptr() % 16 == 0 and (t.is_contiguous() or t.shape[0] == 1 or t.stride(0) % 8 == 0)
 
     xf, yf, of = _rows_of(x, k), _rows_of(y, n), _rows_of(out, n)
-    _require(of.data_ptr() == out.data_ptr() and aligned(of), f"{what}: out must have unit column stride, rows of one stride and 16-byte alignment")
+    if of.data_ptr() != out.data_ptr() or not aligned(of):
+        raise ValueError(f"{what}: out must have unit column stride, rows of one stride and 16-byte alignment")
     xf = xf if aligned(xf) else xf.clone(memory_format=torch.contiguous_format)
     yf = yf if aligned(yf) else yf.clone(memory_format=torch.contiguous_format)
-    a, b = a.contiguous(), b.contiguous()
-    a = a if a.data_ptr() % 16 == 0 else a.clone()
-    b = b if b.data_ptr() % 16 == 0 else b.clone()
-    ids = adapter_ids.contiguous()
-    scales = None if scales is None else scales.contiguous()
-    _launch(x.device, "launch_lora_add_kernel", _ptr(yf), _ptr(xf), _ptr(a), _ptr(b), _ptr(ids), _ptr(scales), _ptr(of), rows, k, n, rank,
-            adapters, _row_stride(yf), _row_stride(xf), _row_stride(of), rows // ids.numel(), _code(x.dtype, what), ids.dtype == torch.int64)
+    a = a if a.is_contiguous() and a.data_ptr() % 16 == 0 else a.clone(memory_format=torch.contiguous_format)
+    b = b if b.is_contiguous() and b.data_ptr() % 16 == 0 else b.clone(memory_format=torch.contiguous_format)
+    ids = adapter_ids if adapter_ids.is_contiguous() else adapter_ids.contiguous()
+    if scales is not None and not scales.is_contiguous():
+        scales = scales.contiguous()
+    _launch(device, "launch_lora_add_kernel", yf.data_ptr(), xf.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
+            0 if scales is None else scales.data_ptr(), of.data_ptr(), rows, k, n, rank, adapters, _row_stride(yf, n), _row_stride(xf, k),
+            _row_stride(of, n), rows // ids.numel(), _code(dtype, what), ids_dtype == torch.int64)
     return out
 
 

@@ -112,9 +112,19 @@ class ValidationResult:
         return ValidationResult(False, param, reason)
 
 
+_OK = ValidationResult.ok()
+
+
 def validate_param(name: str, value, constraint: ParamConstraint, default_devices: frozenset) -> ValidationResult:
     if value is None:
         return ValidationResult.ok()
+    if type(value) is torch.Tensor and constraint.devices is None and (
+            constraint.dtypes is None or value.dtype in constraint.dtypes) and value.device.type in default_devices:
+        for rule in constraint.shape_rules:
+            if not rule.check(value):
+                break
+        else:
+            return _OK   # the common case in one look
     if not constraint.check_dtype(value):
         shown = value.dtype if isinstance(value, torch.Tensor) else value
         return ValidationResult.fail(name, f"dtype {shown} not in {set(constraint.dtypes)}")
