@@ -23,6 +23,7 @@ SIGNATURES: dict[str, list] = {
     "ck_check_device": [],
     "ck_gemm_device_status": [],
     "ck_norm_device_status": [],
+    "ck_lora_device_status": [],
     "ck_set_option": [c_char_p, I],
     "ck_tp_device_status": [],
     "launch_tp_reduce_rows_kernel": [P, P, P, I, I, P, P, I64, I64, I64, I64, I64, I, I, P],
@@ -51,9 +52,9 @@ SIGNATURES: dict[str, list] = {
     "launch_adaln_quantize_mxfp8_kernel": [P, P, P, P, P, I64, I64, I64, I64, F, I, I, P],
     "launch_add_rmsnorm_quantize_kernel": [P, P, P, P, P, P, P, P, I64, I64, I64, I64, F, I, I, I, P],
     "launch_apply_rope_axes_kernel": [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I, I, I, B, B, P],
-    "launch_lora_add_kernel": [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I, B, P],
+    "launch_lora_add_kernel": [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I, B, P],
 }
-_RESTYPES = {"ck_last_error": c_char_p, "ck_tp_pad_bytes": c_int64}
+_RESTYPES = {"ck_last_error": c_char_p, "ck_tp_pad_bytes": c_int64, "ck_lora_workspace_bytes": c_int64}
 
 _lib = None
 
@@ -79,6 +80,8 @@ def load() -> ctypes.CDLL:
         fn.restype = c_int
     lib.ck_tp_pad_bytes.argtypes = []
     lib.ck_tp_pad_bytes.restype = c_int64
+    lib.ck_lora_workspace_bytes.argtypes = [I64, I64, I64, I64]
+    lib.ck_lora_workspace_bytes.restype = c_int64
     lib.ck_last_error.argtypes = []
     lib.ck_last_error.restype = c_char_p
     _lib = lib

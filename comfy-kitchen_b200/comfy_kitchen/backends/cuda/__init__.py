@@ -837,8 +837,11 @@ def lora_add(
     ids = adapter_ids if adapter_ids.is_contiguous() else adapter_ids.contiguous()
     if scales is not None and not scales.is_contiguous():
         scales = scales.contiguous()
+    # fp32 partial sums of the first product; the allocator's, so that streams and captured graphs keep theirs apart
+    need = _native.load().ck_lora_workspace_bytes(rows, k, rank, adapters)
+    work = x.new_empty(need, dtype=torch.uint8) if need else None
     _launch(device, "launch_lora_add_kernel", yf.data_ptr(), xf.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
-            0 if scales is None else scales.data_ptr(), of.data_ptr(), rows, k, n, rank, adapters, _row_stride(yf, n), _row_stride(xf, k),
+            0 if scales is None else scales.data_ptr(), of.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, _row_stride(yf, n), _row_stride(xf, k),
             _row_stride(of, n), rows // ids.numel(), _code(dtype, what), ids_dtype == torch.int64)
     return out
 
@@ -917,6 +920,11 @@ def set_option(name: str, value: int) -> None:
 def gemm_device_status() -> int:
     """Synchronise and return the GEMM kernels' device status word (0 = fine)."""
     return int(_native.load().ck_gemm_device_status())
+
+
+def lora_device_status() -> int:
+    """Synchronise and return (then clear) the adapter kernels' device-side status word; 0 = healthy."""
+    return int(_native.load().ck_lora_device_status())
 
 
 def norm_device_status() -> int:
