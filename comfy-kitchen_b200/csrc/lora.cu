@@ -7,9 +7,9 @@
 // Bound by HBM in either direction: x is read once, y read and out written once (2 K + 4 N bytes a row), each used adapter
 // once; the products' 2 R (K + N) flop a row stay below that up to a rank of about 128.  Two forms:
 //   few rows:   one CTA per row.
-//   many rows:  two kernels of 128-row tiles on the tensor cores (tcgen05), joined by the low-rank vectors in fp32.
-//               shrink:  low[t, :] = A x[t], the K axis split over CTAs (each split writes its own partial sums, which
-//                        the next kernel adds in order: no atomics, the same bits every time);
+//   many rows:  two kernels of 128-row tiles on the tensor cores (tcgen05), joined by the low-rank vectors.
+//               shrink:  low[t, :] = A x[t]; the K axis is split over a cluster's CTAs where there are few tiles, and
+//                        their partial sums are added in order (no atomics, the same bits every time);
 //               expand:  out = y + scale * (B low), y tiles fetched and out tiles stored by TMA while the products run.
 // Ids are looked at on the device: a tile lists the adapters that its rows ask for, computes each one's product for all 128
 // rows and keeps a row's own (a row of another request never enters a sum, whatever it holds).  Requests that lie behind
@@ -26,14 +26,11 @@ namespace {
 
 constexpr int kMaxRank = 256;
 constexpr int kTile = 128;          // rows of a tile (the MMA's M)
-constexpr int kThreads = 192;       // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue, one per 32 rows of the tile
 constexpr int kTileBytes = kTile * 128;   // 128 rows x 64 elements
 constexpr int kSmemMost = 232448;
 
-constexpr int kShrinkColumns = 256;   // two accumulators of up to 128 columns, or one of up to 256; two CTAs share an SM's TMEM
-
 __device__ int g_lora_status = 0;
-enum : int { kWaitFull = 1, kWaitEmpty = 2, kWaitAcc = 3, kWaitAccFree = 4, kWaitLow = 5, kWaitY = 6, kWaitYFree = 7, kWaitDrain = 8 };
+enum : int { kWaitFull = 1, kWaitEmpty = 2, kWaitAcc = 3, kWaitAccFree = 4, kWaitLow = 5, kWaitY = 6, kWaitYFree = 7, kWaitList = 8 };
 
 struct LoraArgs {
     const void* y;
@@ -43,12 +40,13 @@ struct LoraArgs {
     const void* ids;        // int32 or int64, one per rows_per_id rows
     const float* scales;    // [L] or null
     void* out;
-    float* low;             // [splits, rows, R] (many rows)
+    uint8_t* image;         // many rows: per tile the low-rank vectors as the second product's operand (hi blocks, lo blocks)
+    float* factor;          // [rows]: what a row's second product is multiplied by
+    float* partial;         // [splits, rows, R], where K is split
     int64_t rows, K, N, R, L;
     int64_t y_stride, x_stride, out_stride;
     int64_t rows_per_id;
     int ids64;
-    int splits;
 };
 
 __device__ __forceinline__ int adapter_of(const LoraArgs& p, int64_t row) {
@@ -65,213 +63,134 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // ------------------------------------------------------------------ few rows
 
-// One row per CTA: a warp takes one row of A at a time, then every thread one column of the output.
+constexpr int kFewCluster = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32;
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// A cluster of eight CTAs per row, one launch: each CTA sums its eighth of K for the whole low-rank vector, hands that to
+// the others through their shared memory, and computes its eighth of the output's columns.  What it costs is latency
+// (ids, A, the exchange, B), so B and y are fetched into L2 meanwhile.  Rows of one adapter read it from L2 again.
 template <typename T>
-__global__ void __launch_bounds__(256) lora_row_kernel(const LoraArgs p) {
-    __shared__ float s_low[kMaxRank];
-    const int64_t row = blockIdx.x;
-    const int id = adapter_of(p, row);
+__global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThreads)
+lora_few_kernel(const LoraArgs p) {
+    __shared__ __align__(16) float s_part[kFewWarps][kMaxRank];      // [part of this CTA's K][r]
+    __shared__ __align__(16) float s_all[kFewCluster][kMaxRank];     // [CTA][r], written by all of them
+    __shared__ __align__(16) float s_low[kMaxRank];
+    const int64_t row = blockIdx.y;
+    const int rank = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = (int)p.R;
     const T* y = static_cast<const T*>(p.y) + row * p.y_stride;
     T* out = static_cast<T*>(p.out) + row * p.out_stride;
-    if (id < 0) {
+    const int n0 = (int)(p.N / 8 * rank / kFewCluster) * 8, n1 = (int)(p.N / 8 * (rank + 1) / kFewCluster) * 8;
+    const int id = adapter_of(p, row);
+    if (id < 0) {   // (the same for the whole cluster)
         if (p.out != p.y)
-            for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) out[n] = y[n];
+            for (int n = n0 + tid * 8; n < n1; n += kFewThreads * 8) *reinterpret_cast<uint4*>(out + n) = *reinterpret_cast<const uint4*>(y + n);
         return;
     }
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    const T* a = static_cast<const T*>(p.a) + (int64_t)id * p.R * p.K;
-    const T* b = static_cast<const T*>(p.b) + (int64_t)id * p.N * p.R;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (waited for before the first store to another CTA)
+    const T* b = static_cast<const T*>(p.b) + ((int64_t)id * p.N + n0) * R;
+    for (int i = tid; i < ((n1 - n0) * R + 63) / 64; i += kFewThreads) prefetch_l2(b + (int64_t)i * 64);
+    for (int i = tid; i < (n1 - n0 + 63) / 64; i += kFewThreads) prefetch_l2(y + n0 + i * 64);
     const float scale = p.scales ? __ldg(p.scales + id) : 1.0f;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < p.R; r += blockDim.x >> 5) {
-        float sum = 0.0f;
-        for (int64_t k = lane * 8; k < p.K; k += 256) {
-            float u[8], v[8];
-            load8<T>(x + k, u);
-            load8<T>(a + r * p.K + k, v);
+
+    // four rows of A a warp at a time; where that leaves warps over, they share the K part
+    const int fours = R / 4;
+    const int parts = fours >= kFewWarps ? 1 : kFewWarps / fours;
+    const int part = warp / (kFewWarps / parts), member = warp % (kFewWarps / parts), members = kFewWarps / parts;
+    const int c0 = (int)(p.K / 8 * (rank * parts + part) / (kFewCluster * parts)), c1 = (int)(p.K / 8 * (rank * parts + part + 1) / (kFewCluster * parts));
+    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+    const T* a = static_cast<const T*>(p.a) + (int64_t)id * R * p.K;
+    for (int four = member; four < fours; four += members) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const T* ar = a + (int64_t)four * 4 * p.K;
+#pragma unroll 2
+        for (int c = c0 + lane; c < c1; c += 32) {
+            float u[8], v[4][8];
+            load8<T>(x + c * 8, u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(u[j], v[j], sum);
+            for (int i = 0; i < 4; ++i) load8<T>(ar + i * p.K + c * 8, v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[i] = fmaf(u[j], v[i][j], sum[i]);
         }
-        sum = warp_sum(sum);
-        if (lane == 0) s_low[r] = sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = warp_sum(sum[i]);
+        if (lane == 0) *reinterpret_cast<float4*>(&s_part[part][four * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     }
     __syncthreads();
-    for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
-        float sum = 0.0f;
-        for (int r = 0; r < p.R; r += 8) {
-            float v[8];
-            load8<T>(b + n * p.R + r, v);
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    for (int i = tid; i < R * kFewCluster; i += kFewThreads) {
+        const int to = i / R, r = i - to * R;
+        float v = s_part[0][r];
+        for (int k = 1; k < parts; ++k) v += s_part[k][r];
+        uint32_t addr;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tc::smem_u32(&s_all[rank][r])), "r"(to));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+    }
+    tc::cluster_sync();
+    for (int r = tid; r < R; r += kFewThreads) {
+        float v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(s_low[r + j], v[j], sum);
+        for (int k = 0; k < kFewCluster; ++k) v += s_all[k][r];
+        s_low[r] = v;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int n = tid; n < n1 - n0; n += kFewThreads) {
+        const float base = Elem<T>::to_f32(y[n0 + n]);
+        float sum = 0.0f;
+        for (int r = 0; r < R; r += 8) {
+            float v[8];
+            load8<T>(b + (int64_t)n * R + r, v);
+            const float4 lo = *reinterpret_cast<const float4*>(s_low + r), hi = *reinterpret_cast<const float4*>(s_low + r + 4);
+            sum = fmaf(lo.x, v[0], sum); sum = fmaf(lo.y, v[1], sum); sum = fmaf(lo.z, v[2], sum); sum = fmaf(lo.w, v[3], sum);
+            sum = fmaf(hi.x, v[4], sum); sum = fmaf(hi.y, v[5], sum); sum = fmaf(hi.z, v[6], sum); sum = fmaf(hi.w, v[7], sum);
         }
-        out[n] = Elem<T>::from_f32(fmaf(scale, sum, Elem<T>::to_f32(y[n])));
+        out[n0 + n] = Elem<T>::from_f32(fmaf(scale, sum, base));
     }
 }
 
 // ------------------------------------------------------------------ many rows
 
-// The adapters that the tile's rows ask for, in the order of their first rows: their number, which of them row
-// 32 * quarter + lane asks for (mine, -1: none) and, where `list` is given, their ids.  By a whole warp.
-__device__ __forceinline__ int tile_adapters(const LoraArgs& p, int64_t row0, int lane, int quarter, int& mine, int* list) {
-    int id[4];
-    uint32_t left[4];
+// The adapters that kRows rows from row0 on ask for, in the order of their first rows: their number, their ids in `list`
+// (where it is given) and,
+// in `slot`, each row's place in it (-1: none).  By a whole warp.
+template <int kRows>
+__device__ __forceinline__ int tile_adapters(const LoraArgs& p, int64_t row0, int lane, int* list, int16_t* slot) {
+    constexpr int kQ = kRows / 32;
+    int id[kQ], place[kQ];
+    uint32_t left[kQ], any = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kQ; ++q) {
         const int64_t row = row0 + 32 * q + lane;
         id[q] = row < p.rows ? adapter_of(p, row) : -1;
+        place[q] = -1;
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) left[q] = __ballot_sync(0xffffffffu, id[q] >= 0);
-    mine = -1;
+    for (int q = 0; q < kQ; ++q) any |= left[q] = __ballot_sync(0xffffffffu, id[q] >= 0);
     int count = 0;
-    while (left[0] | left[1] | left[2] | left[3]) {
+    while (any) {
         int cur = -1;
 #pragma unroll
-        for (int q = 3; q >= 0; --q) {   // (the first quarter that has rows left decides)
+        for (int q = kQ - 1; q >= 0; --q) {   // (the first 32 rows that have one left decide)
             const int first = __shfl_sync(0xffffffffu, id[q], left[q] ? __ffs(left[q]) - 1 : 0);
             if (left[q]) cur = first;
         }
+        any = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            left[q] &= ~__ballot_sync(0xffffffffu, id[q] == cur);
-            if (q == quarter && id[q] == cur) mine = count;
+        for (int q = 0; q < kQ; ++q) {
+            if (id[q] == cur) place[q] = count;
+            any |= left[q] &= ~__ballot_sync(0xffffffffu, id[q] == cur);
         }
         if (list && lane == 0) list[count] = cur;
         ++count;
     }
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) slot[32 * q + lane] = (int16_t)place[q];
     __syncwarp();
     return count;
 }
-
-struct ShrinkPlan {
-    int splits, groups;         // K parts; adapters of a tile are dealt to `groups` CTAs
-    int k_tiles, rn;            // 64-element steps of K; R rounded up to 16 (the MMA's N)
-    int stages, accs;           // ring of operand tiles; accumulators in TMEM
-    int smem;
-};
-
-// low[split][t][:] = A_{ids[t]} x[t] over this CTA's part of K.
-__global__ void __launch_bounds__(kThreads)
-lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const LoraArgs p,
-                   const ShrinkPlan plan, const bool bf16) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = kTileBytes + plan.rn * 128;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + plan.stages * stage_bytes);
-    uint64_t* empty = full + plan.stages;
-    uint64_t* acc_full = empty + plan.stages;     // [2]
-    uint64_t* acc_empty = acc_full + 2;           // [2]
-    uint64_t* drain = acc_empty + 2;
-    int* s_list = reinterpret_cast<int*>(drain + 1);
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_list + kTile);
-    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row0 = (int64_t)blockIdx.x * kTile;
-    const int split = blockIdx.y, group = blockIdx.z;
-    int mine;
-    const int count = tile_adapters(p, row0, lane, warp & 3, mine, warp == 0 ? s_list : nullptr);
-    if (group >= count) return;   // (the same for every warp)
-    const int k0 = (int)((int64_t)plan.k_tiles * split / plan.splits), k1 = (int)((int64_t)plan.k_tiles * (split + 1) / plan.splits);
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < plan.stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 4); }
-        tc::mbar_init(drain, 1);
-        *s_abort = 0;
-        tc::mbar_init_done();
-    }
-    if (warp == 1) tc::tmem_alloc(s_tmem, kShrinkColumns);
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = *s_tmem;
-
-    if (warp == 0) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (int j = group; j < count && ok; j += plan.groups) {
-            const int id = s_list[j];
-            for (int kt = k0; kt < k1; ++kt, ++it) {
-                const int s = it % plan.stages;
-                if (it >= (uint32_t)plan.stages) ok = tc::mbar_wait(&empty[s], (it / plan.stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
-                if (!ok) break;
-                if (lane == 0) {
-                    uint8_t* st = smem + s * stage_bytes;
-                    tc::mbar_expect_tx(&full[s], (uint32_t)stage_bytes);
-                    tc::tma_load_2d(st, &map_x, kt * 64, (int)row0, &full[s]);
-                    tc::tma_load_3d(st + kTileBytes, &map_a, kt * 64, 0, id, &full[s]);
-                }
-                __syncwarp();
-            }
-        }
-        if (!ok)   // copies in flight land before the CTA leaves
-            for (uint32_t i = it > (uint32_t)plan.stages ? it - plan.stages : 0; i < it; ++i)
-                for (uint32_t n = 0; n < tc::kSpinLimit && !tc::mbar_try_wait(&full[i % plan.stages], (i / plan.stages) & 1); ++n) {}
-    } else if (warp == 1) {
-        const uint32_t id = tc::idesc(bf16, plan.rn);
-        uint32_t it = 0, n = 0;
-        bool ok = true;
-        for (int j = group; j < count && ok; j += plan.groups, ++n) {
-            const uint32_t buf = n % plan.accs;
-            if (n >= (uint32_t)plan.accs) ok = tc::mbar_wait(&acc_empty[buf], (n / plan.accs - 1) & 1, s_abort, &g_lora_status, kWaitAccFree);
-            if (!ok) break;
-            tc::fence_after();
-            for (int kt = k0; kt < k1; ++kt, ++it) {
-                const int s = it % plan.stages;
-                ok = tc::mbar_wait(&full[s], (it / plan.stages) & 1, s_abort, &g_lora_status, kWaitFull);
-                if (!ok) break;
-                tc::fence_after();
-                const uint32_t da = tc::desc_lo(smem + s * stage_bytes), db = tc::desc_lo(smem + s * stage_bytes + kTileBytes);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tc::mma_16bit(tmem + buf * kTile, da + 2 * k, db + 2 * k, id, kt > k0 || k > 0);
-                tc::commit(&empty[s]);
-            }
-            if (ok) tc::commit(&acc_full[buf]);
-        }
-        if (!ok) {   // MMAs in flight end before the operands and the TMEM go
-            tc::commit(drain);
-            for (uint32_t i = 0; i < tc::kSpinLimit && !tc::mbar_try_wait(drain, 0); ++i) {}
-        }
-    } else {
-        const int64_t row = row0 + (warp & 3) * 32 + lane;
-        float* low = p.low + ((int64_t)split * p.rows + row) * p.R;
-        uint32_t n = 0;
-        for (int j = group; j < count; j += plan.groups, ++n) {
-            const uint32_t buf = n % plan.accs;
-            if (!tc::mbar_wait(&acc_full[buf], (n / plan.accs) & 1, s_abort, &g_lora_status, kWaitAcc)) break;
-            tc::fence_after();
-            if (__any_sync(0xffffffffu, mine == j)) {
-                for (int c = 0; c < plan.rn; c += 16) {
-                    uint32_t v[16];
-                    tc::ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kTile + c, v);
-                    tc::wait_ld();
-                    if (mine == j) {
-                        float4* dst = reinterpret_cast<float4*>(low + c);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (c + 4 * i < p.R)
-                                dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
-                    }
-                }
-            }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
-        }
-    }
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    if (warp == 1) tc::tmem_free(tmem, kShrinkColumns);
-}
-
-struct ExpandPlan {
-    int64_t steps, items;       // column steps of a tile; tiles x steps
-    int blocks;                 // 64-element blocks of R
-    int b_stages, y_stages;
-    int smem;
-};
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -286,225 +205,479 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The partial sums of 8 elements of a row's low-rank vector, added in the order of the splits.
-__device__ __forceinline__ void low_sum8(const LoraArgs& p, int64_t row, int r, float (&v)[8]) {
-    const float* src = p.low + row * p.R + r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    for (int s = 0; s < p.splits; ++s, src += p.rows * p.R) {
-        const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+// fp16: the power of two that brings a row of largest magnitude `most` to [1, 2), and its inverse.
+__device__ __forceinline__ void row_scale(float most, float& down, float& up) {
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;   // most is in [2^e, 2^(e+1))
+    down = up = 1.0f;
+    if (e < 127 && e > -126) {                                // (not for zeros, infinities and what fp32 itself barely holds)
+        up = __uint_as_float((uint32_t)(e + 127) << 23);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
     }
 }
 
-// Writes this thread's row of the low-rank tile as two 16-bit operands (swizzled; hi, then lo) and returns the power of
-// two that the products have to be multiplied by.
+// Elements r .. r + 7 of row `row` of a tile's image: hi and lo parts, in the swizzled order in which the MMA reads shared
+// memory, so that the second kernel fetches a tile with one bulk copy.
 template <typename T>
-__device__ __forceinline__ float put_low(const LoraArgs& p, const ExpandPlan& plan, uint8_t* s_low, int64_t row, int r_in_tile, bool has) {
-    float down = 1.0f, up = 1.0f;
-    if (sizeof(T) == 2 && Elem<T>::code == CK_F16 && has) {
-        float most = 0.0f;
-        for (int r = 0; r < p.R; r += 8) {
-            float v[8];
-            low_sum8(p, row, r, v);
+__device__ __forceinline__ void put_image(uint8_t* image, int blocks, int row, int r, const float (&v)[8], float down) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
-        }
-        const int e = (int)(__float_as_uint(most) >> 23) - 127;   // most is in [2^e, 2^(e+1))
-        if (e < 127 && e > -126) {                                // (not for zeros, infinities and what fp32 itself barely holds)
-            up = __uint_as_float((uint32_t)(e + 127) << 23);
-            down = __uint_as_float((uint32_t)(127 - e) << 23);
-        }
+    for (int i = 0; i < 4; ++i) {
+        const float a = v[2 * i] * down, b = v[2 * i + 1] * down;
+        const float ha = Elem<T>::round(a), hb = Elem<T>::round(b);
+        hi[i] = pack2<T>(ha, hb);
+        lo[i] = pack2<T>(isfinite(ha) ? a - ha : 0.0f, isfinite(hb) ? b - hb : 0.0f);   // (an infinity stays one)
     }
-    const int padded = (int)round_up(p.R, 16);
-    for (int r = 0; r < padded; r += 8) {
-        float v[8];
-        if (has && r < p.R) low_sum8(p, row, r, v);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = v[2 * i] * down, b = v[2 * i + 1] * down;
-            float ha = Elem<T>::round(a), hb = Elem<T>::round(b);
-            hi[i] = pack2<T>(ha, hb);
-            lo[i] = pack2<T>(isfinite(ha) ? a - ha : 0.0f, isfinite(hb) ? b - hb : 0.0f);   // (an infinity stays one)
-        }
-        uint8_t* dst = s_low + (r >> 6) * kTileBytes + r_in_tile * 128 + ((((r & 63) >> 3) ^ (r_in_tile & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + plan.blocks * kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    return up;
+    uint8_t* dst = image + (r >> 6) * kTileBytes + row * 128 + ((((r & 63) >> 3) ^ (row & 7)) << 4);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + blocks * kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
-// Persistent CTAs take equal runs of (tile, column step) items.  kN columns a step.
-template <typename T, int kN>
-__global__ void __launch_bounds__(kThreads, 1)
+struct ShrinkPlan {
+    int splits, groups;         // K parts (a cluster); adapters of a tile are dealt to `groups` clusters
+    int k_tiles, halves;        // 64-element steps of K; 128-row tiles of A (2 for ranks over 128)
+    int blocks;                 // 64-element blocks of R
+    int x_stages, a_stages;     // rings of x and A tiles
+    int batch;                  // adapters that share a pass over x
+    int smem;
+};
+
+constexpr int kShrinkRows = 256;           // rows of x a CTA takes (the MMA's N)
+constexpr int kShrinkThreads = 320;        // warp 0: TMA, warp 1: MMA, warps 2-9: epilogue
+constexpr int kXBytes = kShrinkRows * 128;
+
+// low[t][:] = A_{ids[t]} x[t] for 256 rows, as the image that the second product reads.
+//
+// The product is taken as A x^T: an MMA of 128 rows costs 128 clocks whether it has 64 columns or 256, so the rank is its M
+// (padded with zeros) and 256 tokens its N; with the roles the other way round the tensor cores, not HBM, were the bound.
+// The accumulator holds a token per column, and its 32 lanes store consecutive elements of a token's vector.
+// Up to `batch` adapters share a pass over x, each with an accumulator of its own: a tile in which two requests meet costs
+// the other's A tiles (from L2) and products, not a second read of x.
+// The CTAs of a cluster take parts of K.  Each leaves its sums in global memory, and after the cluster's barrier each adds
+// up a share of the tokens, in the order of the parts, and writes their image.
+template <typename T>
+__global__ void __launch_bounds__(kShrinkThreads, 1)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const LoraArgs p,
+                   const ShrinkPlan plan) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int a_bytes = plan.halves * kTileBytes;
+    uint8_t* s_x = smem;
+    uint8_t* s_a = s_x + plan.x_stages * kXBytes;
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(s_a + plan.a_stages * a_bytes);
+    uint64_t* x_empty = x_full + plan.x_stages;
+    uint64_t* a_full = x_empty + plan.x_stages;
+    uint64_t* a_empty = a_full + plan.a_stages;
+    uint64_t* acc_full = a_empty + plan.a_stages;
+    uint64_t* acc_empty = acc_full + 1;
+    uint64_t* drain = acc_empty + 1;
+    uint64_t* listed = drain + 1;
+    int* s_list = reinterpret_cast<int*>(listed + 1);
+    int16_t* s_slot = reinterpret_cast<int16_t*>(s_list + kShrinkRows);
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slot + kShrinkRows);
+    int* s_count = reinterpret_cast<int*>(s_tmem + 1);
+    volatile int* s_abort = s_count + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row0 = (int64_t)blockIdx.x * kShrinkRows;
+    const int split = blockIdx.y, group = blockIdx.z;
+    const int k0 = (int)((int64_t)plan.k_tiles * split / plan.splits), k1 = (int)((int64_t)plan.k_tiles * (split + 1) / plan.splits);
+
+    if (warp == 1) {
+        tc::tmem_alloc(s_tmem, 512);
+    } else if (threadIdx.x == 0) {
+        for (int s = 0; s < plan.x_stages; ++s) { tc::mbar_init(&x_full[s], 1); tc::mbar_init(&x_empty[s], 1); }
+        for (int s = 0; s < plan.a_stages; ++s) { tc::mbar_init(&a_full[s], 1); tc::mbar_init(&a_empty[s], 1); }
+        tc::mbar_init(acc_full, 1);
+        tc::mbar_init(acc_empty, 8);
+        tc::mbar_init(drain, 1);
+        tc::mbar_init(listed, 1);
+        *s_abort = 0;
+        tc::mbar_init_done();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    tc::launch_dependents();
+    const uint32_t tmem = *s_tmem;
+
+    // x's first tiles are on their way before the ids are known (they are wanted unless nobody asks for an adapter)
+    uint32_t ahead = 0;
+    if (warp == 0) {
+        for (; ahead < (uint32_t)min(plan.x_stages, k1 - k0) && plan.groups == 1; ++ahead) {
+            if (tc::elect_one()) {
+                tc::mbar_expect_tx(&x_full[ahead], kXBytes);
+                tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + (int)ahead) * 64, (int)row0, &x_full[ahead]);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 2) {
+        const int n = tile_adapters<kShrinkRows>(p, row0, lane, s_list, s_slot);
+        if (lane == 0) { *s_count = n; tc::mbar_arrive(listed); }
+        __syncwarp();
+    }
+    bool ok = tc::mbar_wait(listed, 0, s_abort, &g_lora_status, kWaitList);
+    const int count = ok ? *s_count : 0;   // (the same in every CTA of the cluster)
+    // a batch: adapters j, j + groups, ... below `until`
+    const int stride = plan.batch * plan.groups;
+    if (warp == 0) {
+        uint32_t xi = 0, ai = 0;
+        for (int first = group; first < count && ok; first += stride) {
+            const int until = min(count, first + stride);
+            for (int kt = k0; kt < k1 && ok; ++kt, ++xi) {
+                int s = xi % plan.x_stages;
+                if (xi >= ahead) {
+                    if (xi >= (uint32_t)plan.x_stages) ok = tc::mbar_wait(&x_empty[s], (xi / plan.x_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+                    if (!ok) break;
+                    if (tc::elect_one()) {
+                        tc::mbar_expect_tx(&x_full[s], kXBytes);
+                        tc::tma_load_2d(s_x + s * kXBytes, &map_x, kt * 64, (int)row0, &x_full[s]);
+                    }
+                    __syncwarp();
+                    ahead = xi + 1;
+                }
+                for (int j = first; j < until; j += plan.groups, ++ai) {
+                    s = ai % plan.a_stages;
+                    if (ai >= (uint32_t)plan.a_stages) ok = tc::mbar_wait(&a_empty[s], (ai / plan.a_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+                    if (!ok) break;
+                    const int which = s_list[j];
+                    if (tc::elect_one()) {
+                        tc::mbar_expect_tx(&a_full[s], (uint32_t)a_bytes);
+                        for (int h = 0; h < plan.halves; ++h)
+                            tc::tma_load_3d(s_a + s * a_bytes + h * kTileBytes, &map_a, kt * 64, h * kTile, which, &a_full[s]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (!ok || xi < ahead) {   // given up, or nobody asked: copies in flight land before the CTA leaves
+            for (uint32_t i = ahead > (uint32_t)plan.x_stages ? ahead - plan.x_stages : 0; i < ahead; ++i) tc::mbar_drain(&x_full[i % plan.x_stages], (i / plan.x_stages) & 1);
+            for (uint32_t i = ai > (uint32_t)plan.a_stages ? ai - plan.a_stages : 0; i < ai; ++i) tc::mbar_drain(&a_full[i % plan.a_stages], (i / plan.a_stages) & 1);
+        }
+    } else if (warp == 1) {
+        const uint32_t id = tc::idesc(Elem<T>::code == CK_BF16, kShrinkRows);
+        uint32_t xi = 0, ai = 0, n = 0;
+        for (int first = group; first < count && ok; first += stride, ++n) {
+            const int until = min(count, first + stride);
+            if (n > 0) ok = tc::mbar_wait(acc_empty, (n - 1) & 1, s_abort, &g_lora_status, kWaitAccFree);
+            for (int kt = k0; kt < k1 && ok; ++kt, ++xi) {
+                const int xs = xi % plan.x_stages;
+                ok = tc::mbar_wait(&x_full[xs], (xi / plan.x_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+                uint32_t d = tmem;
+                for (int j = first; j < until && ok; j += plan.groups, ++ai, d += kShrinkRows) {
+                    const int as = ai % plan.a_stages;
+                    ok = tc::mbar_wait(&a_full[as], (ai / plan.a_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (tc::elect_one()) {
+                        const uint32_t da = tc::desc_lo(s_a + as * a_bytes), db = tc::desc_lo(s_x + xs * kXBytes);
+                        for (int h = 0; h < plan.halves; ++h)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                tc::mma_16bit(d + h * kShrinkRows, da + h * (kTileBytes >> 4) + 2 * k, db + 2 * k, id, kt > k0 || k > 0);
+                        tc::commit(&a_empty[as]);
+                        if (j + plan.groups >= until) {
+                            tc::commit(&x_empty[xs]);
+                            if (kt + 1 == k1) tc::commit(acc_full);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (!ok) {
+            if (tc::elect_one()) tc::commit(drain);
+            __syncwarp();
+            tc::mbar_drain(drain, 0);
+        }
+    } else {
+        // a warp: 32 elements of the vector (its TMEM lanes) of 128 of the tokens
+        const int quarter = warp & 3, token0 = ((warp - 2) >> 2) * kTile;
+        uint32_t n = 0;
+        for (int first = group; first < count && ok; first += stride, ++n) {
+            const int until = min(count, first + stride);
+            ok = tc::mbar_wait(acc_full, n & 1, s_abort, &g_lora_status, kWaitAcc);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + token0;
+            for (int j = first; j < until; j += plan.groups, acc += kShrinkRows) {
+                for (int h = 0; h < plan.halves; ++h) {
+                    const int r = h * kTile + quarter * 32 + lane;
+                    if (r - lane >= p.R) break;
+                    float* dst = p.partial + ((int64_t)split * p.rows + row0 + token0) * p.R + r;
+                    for (int t = 0; t < kTile; t += 32) {
+                        const uint32_t asked = __ballot_sync(0xffffffffu, s_slot[token0 + t + lane] == j);
+                        if (!asked) continue;
+                        uint32_t v[2][16];
+                        tc::ld16(acc + h * kShrinkRows + t, v[0]);
+                        tc::ld16(acc + h * kShrinkRows + t + 16, v[1]);
+                        tc::wait_ld();
+                        if (r < p.R) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (asked >> i & 1) dst[(t + i) * p.R] = __uint_as_float(v[i >> 4][i & 15]);
+                        }
+                    }
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(acc_empty);
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 1) tc::tmem_free(tmem, 512);
+    tc::cluster_sync();
+
+    // the parts of K, added up: eight lanes a token, each with every eighth chunk of 8 elements
+    const int mine0 = kShrinkRows * split / plan.splits, mine1 = kShrinkRows * (split + 1) / plan.splits, sub = lane & 7;
+    for (int r0 = mine0 + warp * 4; r0 < mine1; r0 += kShrinkThreads / 8) {
+        const int r = r0 + (lane >> 3);
+        const int64_t row = row0 + r;
+        const int j = r < mine1 && count > 0 ? s_slot[r] : -1;
+        const bool wanted = j >= 0 && j % plan.groups == group;
+        float v[kMaxRank / 64][8], most = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kMaxRank / 64; ++u) {
+            const int c = (u * 8 + sub) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+            if (wanted && c < p.R) {
+                const float* src = p.partial + row * p.R + c;
+#pragma unroll 4
+                for (int k = 0; k < plan.splits; ++k, src += p.rows * p.R) {
+                    const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
+                    v[u][0] += a.x; v[u][1] += a.y; v[u][2] += a.z; v[u][3] += a.w;
+                    v[u][4] += b.x; v[u][5] += b.y; v[u][6] += b.z; v[u][7] += b.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[u][i]));
+        }
+        float down = 1.0f, up = 1.0f;
+        if (Elem<T>::code == CK_F16) {
+#pragma unroll
+            for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            row_scale(most, down, up);
+        }
+        if (!wanted) continue;
+        uint8_t* image = p.image + ((int64_t)blockIdx.x * 2 + (r >> 7)) * (2 * plan.blocks * kTileBytes);
+        const int padded = (int)round_up(p.R, 16);   // (the second product's steps)
+#pragma unroll
+        for (int u = 0; u < kMaxRank / 64; ++u)
+            if ((u * 8 + sub) * 8 < padded) put_image<T>(image, plan.blocks, r & 127, (u * 8 + sub) * 8, v[u], down);
+        if (sub == 0) p.factor[row] = p.scales ? up * __ldg(p.scales + s_list[j]) : up;
+    }
+}
+
+struct ExpandPlan {
+    int64_t steps, items;       // column steps of a tile; tiles x steps
+    int blocks;                 // 64-element blocks of R
+    int b_stages, y_stages;
+    int smem;
+};
+
+constexpr int kEpiGroups = 2;              // units of 64 columns are dealt to two groups of four epilogue warps
+constexpr int kExpandThreads = 96 + kEpiGroups * 128;   // warp 0: y's tiles, 1: MMA, 2-9: epilogue, 10: B's tiles
+
+// Persistent CTAs take equal runs of (tile, column step) items; a step is kU units of 64 columns.  The MMA of 128 rows
+// costs 128 clocks however few columns it has, and reads its 128 rows of the image from shared memory each time, so steps
+// are as wide as the number of items allows (16384 x 8192, rank 128: 225 us with 64 columns).
+template <typename T, int kU>
+__global__ void __launch_bounds__(kExpandThreads, 1)
 lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y,
                    const __grid_constant__ CUtensorMap map_out, const LoraArgs p, const ExpandPlan plan) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr int kHalves = kN / 64;
-    constexpr int kYBytes = kHalves * kTileBytes;
-    const int b_bytes = plan.blocks * kN * 128;
+    constexpr int kStep = kU * 64, kExpandColumns = 2 * kStep;
+    constexpr int b_bytes = kStep * 128;                               // 64 elements of R for a step's columns
+    const uint32_t low_bytes = 2 * plan.blocks * kTileBytes;
     uint8_t* s_low = smem;                                             // hi blocks, lo blocks
-    uint8_t* s_b = s_low + 2 * plan.blocks * kTileBytes;
+    uint8_t* s_b = s_low + low_bytes;
     uint8_t* s_y = s_b + plan.b_stages * b_bytes;
-    uint64_t* b_full = reinterpret_cast<uint64_t*>(s_y + plan.y_stages * kYBytes);
+    uint64_t* b_full = reinterpret_cast<uint64_t*>(s_y + plan.y_stages * kTileBytes);
     uint64_t* b_empty = b_full + plan.b_stages;
     uint64_t* y_full = b_empty + plan.b_stages;
     uint64_t* y_empty = y_full + plan.y_stages;
     uint64_t* acc_full = y_empty + plan.y_stages;                      // [2]
     uint64_t* acc_empty = acc_full + 2;                                // [2]
     uint64_t* low_full = acc_empty + 2;
-    uint64_t* drain = low_full + 1;
-    int* s_list = reinterpret_cast<int*>(drain + 1);
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_list + kTile);
+    uint64_t* low_done = low_full + 1;                                 // a tile's last MMA is complete
+    uint64_t* drain = low_done + 1;
+    int* s_list = reinterpret_cast<int*>(drain + 1);                   // (warp 10's)
+    int16_t* s_slots = reinterpret_cast<int16_t*>(s_list + kTile);
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slots + kExpandThreads / 32 * kTile);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t first = plan.items * blockIdx.x / gridDim.x, last = plan.items * (blockIdx.x + 1) / gridDim.x;
     const bool in_place = p.out == p.y;
+    int16_t* s_slot = s_slots + warp * kTile;                // a warp's own: the roles are at different tiles
 
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 64) {
         for (int s = 0; s < plan.b_stages; ++s) { tc::mbar_init(&b_full[s], 1); tc::mbar_init(&b_empty[s], 1); }
         for (int s = 0; s < plan.y_stages; ++s) { tc::mbar_init(&y_full[s], 1); tc::mbar_init(&y_empty[s], 4); }
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 4); }
-        tc::mbar_init(low_full, 4);
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 4 * kEpiGroups); }
+        tc::mbar_init(low_full, 1);
+        tc::mbar_init(low_done, 1);
         tc::mbar_init(drain, 1);
         *s_abort = 0;
         tc::mbar_init_done();
     }
-    if (warp == 1) tc::tmem_alloc(s_tmem, 2 * kN);
+    if (warp == 1) tc::tmem_alloc(s_tmem, kExpandColumns);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *s_tmem;
 
+    // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles
     if (warp == 0) {
-        uint32_t bi = 0, yi = 0;
+        uint32_t yi = 0;
         bool ok = true;
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            int mine;
-            const int count = tile_adapters(p, tile * kTile, lane, 0, mine, s_list);
-            if (count == 0 && in_place) continue;
-            for (int64_t step = begin; step < end && ok; ++step) {
-                {
-                    const int s = yi % plan.y_stages;
-                    if (yi >= (uint32_t)plan.y_stages) ok = tc::mbar_wait(&y_empty[s], (yi / plan.y_stages - 1) & 1, s_abort, &g_lora_status, kWaitYFree);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        tc::mbar_expect_tx(&y_full[s], kYBytes);
-#pragma unroll
-                        for (int h = 0; h < kHalves; ++h)
-                            tc::tma_load_2d(s_y + s * kYBytes + h * kTileBytes, &map_y, (int)(step * kN + h * 64), (int)(tile * kTile), &y_full[s]);
-                    }
-                    ++yi;
-                    __syncwarp();
+            if (in_place && tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot) == 0) continue;
+            for (int64_t unit = begin * kU; unit < end * kU; ++unit) {
+                const int s = yi % plan.y_stages;
+                if (yi >= (uint32_t)plan.y_stages) ok = tc::mbar_wait(&y_empty[s], (yi / plan.y_stages - 1) & 1, s_abort, &g_lora_status, kWaitYFree);
+                if (!ok) break;
+                ++yi;
+                if (tc::elect_one()) {
+                    tc::mbar_expect_tx(&y_full[s], kTileBytes);
+                    tc::tma_load_2d(s_y + s * kTileBytes, &map_y, (int)unit * 64, (int)(tile * kTile), &y_full[s]);
                 }
-                for (int j = 0; j < count; ++j, ++bi) {
-                    const int s = bi % plan.b_stages;
-                    if (bi >= (uint32_t)plan.b_stages) ok = tc::mbar_wait(&b_empty[s], (bi / plan.b_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        tc::mbar_expect_tx(&b_full[s], (uint32_t)b_bytes);
-                        for (int k = 0; k < plan.blocks; ++k)
-                            tc::tma_load_3d(s_b + s * b_bytes + k * kN * 128, &map_b, k * 64, (int)(step * kN), s_list[j], &b_full[s]);
-                    }
-                    __syncwarp();
-                }
+                __syncwarp();
             }
         }
-        if (!ok) {   // copies in flight land before the CTA leaves
-            for (uint32_t i = bi > (uint32_t)plan.b_stages ? bi - plan.b_stages : 0; i < bi; ++i)
-                for (uint32_t n = 0; n < tc::kSpinLimit && !tc::mbar_try_wait(&b_full[i % plan.b_stages], (i / plan.b_stages) & 1); ++n) {}
-            for (uint32_t i = yi > (uint32_t)plan.y_stages ? yi - plan.y_stages : 0; i < yi; ++i)
-                for (uint32_t n = 0; n < tc::kSpinLimit && !tc::mbar_try_wait(&y_full[i % plan.y_stages], (i / plan.y_stages) & 1); ++n) {}
-        }
-    } else if (warp == 1) {
-        const uint32_t id = tc::idesc(Elem<T>::code == CK_BF16, kN);
-        const int k_steps = (int)ceil_div(p.R, 16);
-        uint32_t n = 0, seg = 0;
+        if (!ok)
+            for (uint32_t i = yi > (uint32_t)plan.y_stages ? yi - plan.y_stages : 0; i < yi; ++i) tc::mbar_drain(&y_full[i % plan.y_stages], (i / plan.y_stages) & 1);
+    } else if (warp == kExpandThreads / 32 - 1) {
+        uint32_t bi = 0;
         bool ok = true;
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            int mine;
-            const int count = tile_adapters(p, tile * kTile, lane, 0, mine, nullptr);
+            const int count = tile_adapters<kTile>(p, tile * kTile, lane, s_list, s_slot);
+            for (int64_t step = begin; step < end && ok; ++step)
+                for (int j = 0; j < count && ok; ++j) {
+                    const int which = s_list[j];
+                    for (int k = 0; k < plan.blocks; ++k) {
+                        const int s = bi % plan.b_stages;
+                        if (bi >= (uint32_t)plan.b_stages) ok = tc::mbar_wait(&b_empty[s], (bi / plan.b_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+                        if (!ok) break;
+                        ++bi;
+                        if (tc::elect_one()) {
+                            tc::mbar_expect_tx(&b_full[s], (uint32_t)b_bytes);
+                            tc::tma_load_3d(s_b + s * b_bytes, &map_b, k * 64, (int)(step * kStep), which, &b_full[s]);
+                        }
+                        __syncwarp();
+                    }
+                }
+        }
+        if (!ok)
+            for (uint32_t i = bi > (uint32_t)plan.b_stages ? bi - plan.b_stages : 0; i < bi; ++i) tc::mbar_drain(&b_full[i % plan.b_stages], (i / plan.b_stages) & 1);
+    } else if (warp == 1) {
+        const uint32_t id = tc::idesc(Elem<T>::code == CK_BF16, kStep);
+        const int k_steps = (int)ceil_div(p.R, 16);
+        uint32_t bi = 0, n = 0, seg = 0;
+        bool ok = true;
+        tc::wait_for_dependency();      // the first kernel's image
+        for (int64_t item = first; item < last && ok;) {
+            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
+            item += end - begin;
+            const int count = tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot);
             if (count == 0) continue;
-            ok = tc::mbar_wait(low_full, seg++ & 1, s_abort, &g_lora_status, kWaitLow);
+            if (seg > 0) ok = tc::mbar_wait(low_done, (seg - 1) & 1, s_abort, &g_lora_status, kWaitAcc);   // nothing reads s_low any more
+            if (!ok) break;
+            if (tc::elect_one()) {
+                tc::mbar_expect_tx(low_full, low_bytes);
+                tc::bulk_load(s_low, p.image + tile * low_bytes, low_bytes, low_full);
+            }
+            __syncwarp();
+            ok = tc::mbar_wait(low_full, seg & 1, s_abort, &g_lora_status, kWaitLow);
+            ++seg;
             for (int64_t i = 0; i < (end - begin) * count && ok; ++i, ++n) {
                 const uint32_t buf = n & 1;
-                const int s = n % plan.b_stages;
                 if (n >= 2) ok = tc::mbar_wait(&acc_empty[buf], (n / 2 - 1) & 1, s_abort, &g_lora_status, kWaitAccFree);
-                if (ok) ok = tc::mbar_wait(&b_full[s], (n / plan.b_stages) & 1, s_abort, &g_lora_status, kWaitFull);
                 if (!ok) break;
-                tc::fence_after();
-                for (int part = 0; part < 2; ++part)
-                    for (int k = 0; k < k_steps; ++k)
-                        tc::mma_16bit(tmem + buf * kN, tc::desc_lo(s_low + (part * plan.blocks + (k >> 2)) * kTileBytes) + 2 * (k & 3),
-                                      tc::desc_lo(s_b + s * b_bytes + (k >> 2) * kN * 128) + 2 * (k & 3), id, part > 0 || k > 0);
-                tc::commit(&b_empty[s]);
-                tc::commit(&acc_full[buf]);
+                for (int k = 0; k < k_steps; k += 4, ++bi) {
+                    const int s = bi % plan.b_stages;
+                    ok = tc::mbar_wait(&b_full[s], (bi / plan.b_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (tc::elect_one()) {
+                        const uint32_t d = tmem + buf * kStep, to_lo = plan.blocks * (kTileBytes >> 4);
+                        const uint32_t da = tc::desc_lo(s_low) + (k >> 2) * (kTileBytes >> 4), db = tc::desc_lo(s_b + s * b_bytes);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (k + u < k_steps) {
+                                tc::mma_16bit(d, da + 2 * u, db + 2 * u, id, k + u > 0);
+                                tc::mma_16bit(d, da + to_lo + 2 * u, db + 2 * u, id, 1);
+                            }
+                        tc::commit(&b_empty[s]);
+                        if (k + 4 >= k_steps) {
+                            tc::commit(&acc_full[buf]);
+                            if (i + 1 == (end - begin) * count) tc::commit(low_done);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
         }
-        if (!ok) {   // MMAs in flight end before the operands and the TMEM go
-            tc::commit(drain);
-            for (uint32_t i = 0; i < tc::kSpinLimit && !tc::mbar_try_wait(drain, 0); ++i) {}
+        if (!ok) {
+            if (tc::elect_one()) tc::commit(drain);
+            __syncwarp();
+            tc::mbar_drain(drain, 0);
+            if (seg > 0) tc::mbar_drain(low_full, (seg - 1) & 1);
         }
     } else {
+        const uint32_t group = (warp - 2) >> 2;
         const int quarter = warp & 3, r_in_tile = quarter * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        uint32_t n = 0, yi = 0;
+        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+        uint32_t unit = 0, n = 0;       // units and accumulators so far
+        int before = -1;                // the stage whose store may still be reading
         bool ok = true;
+        tc::wait_for_dependency();      // the first kernel's factors
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            int mine;
-            const int count = tile_adapters(p, tile * kTile, lane, quarter, mine, nullptr);
+            const int count = tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot);
             if (count == 0 && in_place) continue;
-            const int64_t row = tile * kTile + r_in_tile;
-            float factor = 0.0f;
-            if (count > 0) {
-                // (the tile before has been waited for accumulator by accumulator, so its MMAs are done with s_low)
-                factor = put_low<T>(p, plan, s_low, row, r_in_tile, mine >= 0);
-                if (mine >= 0 && p.scales) factor *= __ldg(p.scales + adapter_of(p, row));
-                tc::fence_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(low_full);
-            }
-            for (int64_t step = begin; step < end && ok; ++step, ++yi) {
-                const int ys = yi % plan.y_stages;
-                uint8_t* mine_y = s_y + ys * kYBytes + r_in_tile * 128;
-                ok = tc::mbar_wait(&y_full[ys], (yi / plan.y_stages) & 1, s_abort, &g_lora_status, kWaitY);
+            const int mine = s_slot[r_in_tile];
+            const float factor = mine >= 0 ? __ldcg(p.factor + tile * kTile + r_in_tile) : 0.0f;
+            for (int64_t step = begin; step < end && ok; ++step, unit += kU) {
                 for (int j = 0; j < count && ok; ++j, ++n) {
                     const uint32_t buf = n & 1;
                     ok = tc::mbar_wait(&acc_full[buf], (n / 2) & 1, s_abort, &g_lora_status, kWaitAcc);
                     if (!ok) break;
                     tc::fence_after();
                     if (__any_sync(0xffffffffu, mine == j)) {
+#pragma unroll 1
+                        for (int u = (int)((unit ^ group) & 1); u < kU; u += kEpiGroups) {
+                            const int ys = (unit + u) % plan.y_stages;
+                            uint8_t* mine_y = s_y + ys * kTileBytes + r_in_tile * 128;
+                            uint32_t v[4][16];
 #pragma unroll
-                        for (int c = 0; c < kN; c += 16) {
-                            uint32_t v[16];
-                            tc::ld16(tmem + lanes + buf * kN + c, v);
+                            for (int c = 0; c < 4; ++c) tc::ld16(acc + buf * kStep + u * 64 + 16 * c, v[c]);
                             tc::wait_ld();
-                            if (mine == j) {
+                            ok = ok && tc::mbar_wait(&y_full[ys], ((unit + u) / plan.y_stages) & 1, s_abort, &g_lora_status, kWaitY);
+                            if (ok && mine == j) {
+                                // (all of y's row is read before any of it is written: nothing orders the eight chunks)
+                                Raw8<T> raw[8];
 #pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    uint4* at = reinterpret_cast<uint4*>(mine_y + (c >> 6) * kTileBytes + (((((c & 63) >> 3) + u) ^ (r_in_tile & 7)) << 4));
-                                    Raw8<T> raw;
-                                    raw.u = *at;
+                                for (int c = 0; c < 8; ++c) raw[c].u = *reinterpret_cast<const uint4*>(mine_y + ((c ^ (r_in_tile & 7)) << 4));
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) {
                                     float f[8];
-                                    unpack8(raw, f);
+                                    unpack8(raw[c], f);
 #pragma unroll
-                                    for (int i = 0; i < 8; ++i) f[i] = fmaf(factor, __uint_as_float(v[8 * u + i]), f[i]);
-                                    *at = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+                                    for (int i = 0; i < 8; ++i) f[i] = fmaf(factor, __uint_as_float(v[c >> 1][8 * (c & 1) + i]), f[i]);
+                                    raw[c].u = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
                                 }
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(mine_y + ((c ^ (r_in_tile & 7)) << 4)) = raw[c].u;
                             }
                         }
                     }
@@ -515,22 +688,25 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 if (!ok) break;
                 tc::fence_async_smem();
                 __syncwarp();
-                if (lane == 0) {
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h)
-                        tc::tma_store_2d(&map_out, s_y + ys * kYBytes + h * kTileBytes + quarter * 32 * 128, (int)(step * kN + h * 64),
-                                         (int)(tile * kTile) + quarter * 32);
-                    tc::tma_store_commit();
-                    // a stage is handed back when its store has read it: one step later where there are stages to spare
-                    if (plan.y_stages > 2) {
-                        tc::tma_store_wait_read<1>();
-                        if (yi > 0) tc::mbar_arrive(&y_empty[(yi - 1) % plan.y_stages]);
-                    } else {
-                        tc::tma_store_wait_read<0>();
-                        tc::mbar_arrive(&y_empty[ys]);
+                for (int u = (int)((unit ^ group) & 1); u < kU && ok; u += kEpiGroups) {
+                    const int ys = (unit + u) % plan.y_stages;
+                    ok = tc::mbar_wait(&y_full[ys], ((unit + u) / plan.y_stages) & 1, s_abort, &g_lora_status, kWaitY);
+                    if (ok && lane == 0) {
+                        tc::tma_store_2d(&map_out, s_y + ys * kTileBytes + quarter * 32 * 128, (int)(step * kStep) + u * 64, (int)(tile * kTile) + quarter * 32);
+                        tc::tma_store_commit();
+                        // a stage is handed back when its store has read it: with the group's next unit, where a whole step
+                        // fits beside the two stages that are then still out
+                        if (plan.y_stages >= kU + kEpiGroups) {
+                            tc::tma_store_wait_read<1>();
+                            if (before >= 0) tc::mbar_arrive(&y_empty[before]);
+                            before = ys;
+                        } else {
+                            tc::tma_store_wait_read<0>();
+                            tc::mbar_arrive(&y_empty[ys]);
+                        }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
         if (lane == 0) tc::tma_store_wait_read<0>();
@@ -539,7 +715,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 1) tc::tmem_free(tmem, 2 * kN);
+    if (warp == 1) tc::tmem_free(tmem, kExpandColumns);
 }
 
 // ------------------------------------------------------------------ host
@@ -557,26 +733,42 @@ int sm_count() {
     return cached[dev];
 }
 
-bool few_rows(int64_t rows) { return rows <= 16; }
+#ifndef CK_LORA_FEW
+#define CK_LORA_FEW 64
+#endif
+bool few_rows(int64_t rows) { return rows <= CK_LORA_FEW; }
 
 ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R, int64_t L) {
     ShrinkPlan s{};
-    const int64_t tiles = ceil_div(rows, kTile), slots = 2 * sm_count();   // two CTAs an SM
+    const int64_t tiles = ceil_div(rows, kShrinkRows), slots = sm_count();
     s.k_tiles = (int)ceil_div(K, 64);
-    s.rn = (int)round_up(R, 16);
-    int64_t splits = slots / tiles, most = s.k_tiles / 4;     // at least four steps of K each
-    splits = splits > most ? most : splits;
-    s.splits = (int)(splits < 1 ? 1 : splits > 65535 ? 65535 : splits);
-    int64_t groups = slots / (tiles * s.splits), asked = rows < kTile ? rows : kTile;
+    s.halves = R > kTile ? 2 : 1;
+    s.blocks = (int)ceil_div(R, 64);
+    int64_t splits = slots / tiles, most = s.k_tiles / 4;   // at least four steps of K each
+    if (splits > most) splits = most;
+    s.splits = (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
+    int64_t groups = slots / (tiles * s.splits), asked = rows < kShrinkRows ? rows : kShrinkRows;
     if (groups > asked) groups = asked;
     if (groups > L) groups = L;
     s.groups = (int)(groups < 1 ? 1 : groups);
-    const int stage = kTileBytes + s.rn * 128;
-    s.stages = (110 * 1024) / stage;
-    if (s.stages > 6) s.stages = 6;
-    s.accs = s.rn <= 128 ? 2 : 1;
-    s.smem = 1024 + s.stages * (stage + 16) + 5 * 8 + kTile * 4 + 16;
+    s.batch = s.halves == 2 ? 1 : 2;                         // (of 256 TMEM columns each)
+    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + kShrinkRows * 6 + 16;
+    s.x_stages = (kSmemMost - rest - a_bytes) / (kXBytes + a_bytes);
+    s.a_stages = s.x_stages + 1;
+    s.smem = rest + s.x_stages * kXBytes + s.a_stages * a_bytes;
     return s;
+}
+
+// Where the parts of the workspace lie.
+struct Workspace {
+    int64_t factor, partial, bytes;   // (the image is at 0)
+};
+Workspace workspace_of(const ShrinkPlan& s, int64_t rows, int64_t R) {
+    Workspace w{};
+    w.factor = ceil_div(rows, kShrinkRows) * (kShrinkRows / kTile) * 2 * s.blocks * kTileBytes;
+    w.partial = w.factor + round_up(rows * 4, 128);
+    w.bytes = w.partial + (int64_t)s.splits * rows * R * 4;
+    return w;
 }
 
 template <typename K>
@@ -591,51 +783,86 @@ int opt_in(K kernel, int which) {   // dynamic shared memory beyond 48 KB, once 
     return CK_OK;
 }
 
-template <typename T, int kN>
+int launched(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return CK_OK;
+    (void)cudaGetLastError();
+    CK_FAIL((int)e, "lora_add (%s): %s", what, cudaGetErrorString(e));
+}
+
+template <typename T, int kU>
 int launch_expand(const LoraArgs& p, cudaStream_t stream) {
+    constexpr int kStep = kU * 64, b_bytes = kStep * 128;
     ExpandPlan e{};
-    e.steps = ceil_div(p.N, kN);
+    e.steps = ceil_div(p.N, kStep);
     e.items = e.steps * ceil_div(p.rows, kTile);
     e.blocks = (int)ceil_div(p.R, 64);
-    const int b_bytes = e.blocks * kN * 128, y_bytes = kTile * kN * 2, rest = 1024 + 24 * 8 + kTile * 4 + 16;
-    int room = kSmemMost - rest - 2 * e.blocks * kTileBytes;
-    e.b_stages = e.y_stages = 2;
-    room -= 2 * (b_bytes + y_bytes);
-    for (int i = 0; i < 2; ++i) {
-        if (room >= y_bytes) { ++e.y_stages; room -= y_bytes; }
-        if (room >= b_bytes) { ++e.b_stages; room -= b_bytes; }
+    const int rest = 1024 + 40 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 16;
+    // the image, a stage of B and a step's units of y (they are freed together); then y and B in turn
+    int room = kSmemMost - rest - 2 * e.blocks * kTileBytes - b_bytes - kU * kTileBytes;
+    if (room < 0) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld does not fit", (long long)p.R);
+    e.b_stages = 1;
+    e.y_stages = kU;
+    while (e.y_stages < 8 || e.b_stages < 4) {
+        const bool y = e.y_stages < 8 && room >= kTileBytes;
+        if (y) { ++e.y_stages; room -= kTileBytes; }
+        const bool b = e.b_stages < 4 && room >= b_bytes;
+        if (b) { ++e.b_stages; room -= b_bytes; }
+        if (!b && !y) break;
     }
     e.smem = kSmemMost - room;
     CUtensorMap map_b, map_y, map_out;
     const int64_t bd[3] = {p.R, p.N, p.L}, bs[2] = {p.R * 2, p.N * p.R * 2};
     const int64_t yd[2] = {p.N, p.rows}, ys[1] = {p.y_stride * 2}, os[1] = {p.out_stride * 2};
-    if (!tc::make_map_16bit(&map_b, p.b, 3, bd, bs, kN) || !tc::make_map_16bit(&map_y, p.y, 2, yd, ys, kTile) ||
+    if (!tc::make_map_16bit(&map_b, p.b, 3, bd, bs, kStep) || !tc::make_map_16bit(&map_y, p.y, 2, yd, ys, kTile) ||
         !tc::make_map_16bit(&map_out, p.out, 2, yd, os, 32))
         CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: a tensor map could not be encoded");
-    auto kernel = lora_expand_kernel<T, kN>;
-    const int rc = opt_in(kernel, 1 + (Elem<T>::code == CK_BF16 ? 0 : 2) + (kN == 64));
+    auto kernel = lora_expand_kernel<T, kU>;
+    const int rc = opt_in(kernel, kU + (Elem<T>::code == CK_BF16 ? 0 : 4) - 1);
     if (rc != CK_OK) return rc;
-    const int64_t grid = e.items < sm_count() ? e.items : sm_count();
-    kernel<<<(unsigned)grid, kThreads, e.smem, stream>>>(map_b, map_y, map_out, p, e);
-    return launch_status("lora_add (expand)");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its beginning runs beside the first kernel's end
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(e.items < sm_count() ? e.items : sm_count()));
+    cfg.blockDim = dim3(kExpandThreads);
+    cfg.dynamicSmemBytes = e.smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return launched(cudaLaunchKernelEx(&cfg, kernel, map_b, map_y, map_out, p, e), "expand");
 }
 
 template <typename T>
-int launch_many(LoraArgs p, cudaStream_t stream) {
+int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
     const ShrinkPlan s = shrink_plan(p.rows, p.K, p.R, p.L);
-    p.splits = s.splits;
+    const Workspace w = workspace_of(s, p.rows, p.R);
+    p.image = workspace;
+    p.factor = reinterpret_cast<float*>(workspace + w.factor);
+    p.partial = reinterpret_cast<float*>(workspace + w.partial);
     CUtensorMap map_x, map_a;
     const int64_t xd[2] = {p.K, p.rows}, xs[1] = {p.x_stride * 2};
     const int64_t ad[3] = {p.K, p.R, p.L}, as[2] = {p.K * 2, p.R * p.K * 2};
-    if (!tc::make_map_16bit(&map_x, p.x, 2, xd, xs, kTile) || !tc::make_map_16bit(&map_a, p.a, 3, ad, as, s.rn))
+    if (!tc::make_map_16bit(&map_x, p.x, 2, xd, xs, kShrinkRows) || !tc::make_map_16bit(&map_a, p.a, 3, ad, as, kTile))
         CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: a tensor map could not be encoded");
-    int rc = opt_in(lora_shrink_kernel, 0);
+    int rc = opt_in(lora_shrink_kernel<T>, Elem<T>::code == CK_BF16);
     if (rc != CK_OK) return rc;
-    const dim3 grid((unsigned)ceil_div(p.rows, kTile), (unsigned)s.splits, (unsigned)s.groups);
-    lora_shrink_kernel<<<grid, kThreads, s.smem, stream>>>(map_x, map_a, p, s, Elem<T>::code == CK_BF16);
-    rc = launch_status("lora_add (shrink)");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = (unsigned)s.splits; attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ceil_div(p.rows, kShrinkRows), (unsigned)s.splits, (unsigned)s.groups);
+    cfg.blockDim = dim3(kShrinkThreads);
+    cfg.dynamicSmemBytes = s.smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    rc = launched(cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T>, map_x, map_a, p, s), "shrink");
     if (rc != CK_OK) return rc;
-    return p.R <= 64 ? launch_expand<T, 128>(p, stream) : launch_expand<T, 64>(p, stream);
+    // the widest steps that still give every SM an item (and, beside the image of a rank over 128, fit shared memory)
+    const int64_t tiles = ceil_div(p.rows, kTile);
+    if (tiles * ceil_div(p.N, 256) >= sm_count() && p.R <= 128) return launch_expand<T, 4>(p, stream);
+    if (tiles * ceil_div(p.N, 128) >= sm_count()) return launch_expand<T, 2>(p, stream);
+    return launch_expand<T, 1>(p, stream);
 }
 
 }  // namespace
@@ -644,7 +871,7 @@ int launch_many(LoraArgs p, cudaStream_t stream) {
 extern "C" int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t rank, int64_t adapters) {
     using namespace ck;
     if (rows <= 0 || K <= 0 || rank <= 0 || adapters <= 0 || few_rows(rows)) return 0;
-    return shrink_plan(rows, K, rank, adapters).splits * rows * rank * 4;
+    return workspace_of(shrink_plan(rows, K, rank, adapters), rows, rank).bytes;
 }
 
 extern "C" int ck_lora_device_status(void) {
@@ -674,13 +901,15 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
-    const LoraArgs p{y, x, a, b, ids, scales, out, static_cast<float*>(workspace), rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit, 0};
+    const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
     if (few_rows(rows)) {
-        if (dtype_code == CK_BF16) lora_row_kernel<__nv_bfloat16><<<(unsigned)rows, 256, 0, stream>>>(p);
-        else lora_row_kernel<__half><<<(unsigned)rows, 256, 0, stream>>>(p);
+        const dim3 grid(kFewCluster, (unsigned)rows);
+        if (dtype_code == CK_BF16) lora_few_kernel<__nv_bfloat16><<<grid, kFewThreads, 0, stream>>>(p);
+        else lora_few_kernel<__half><<<grid, kFewThreads, 0, stream>>>(p);
         return launch_status("lora_add");
     }
     if (!workspace) CK_FAIL(CK_ERR_NULL, "lora_add: a workspace of ck_lora_workspace_bytes() is needed");
     if (!aligned16(workspace)) CK_FAIL(CK_ERR_ALIGN, "lora_add: the workspace must be 16-byte aligned");
-    return dtype_code == CK_BF16 ? launch_many<__nv_bfloat16>(p, stream) : launch_many<__half>(p, stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    return dtype_code == CK_BF16 ? launch_many<__nv_bfloat16>(p, ws, stream) : launch_many<__half>(p, ws, stream);
 }

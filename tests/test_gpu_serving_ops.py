@@ -322,6 +322,7 @@ LORAS = [
     (31, 200, 136, 8, 2, "runs"), (33, 1024, 512, 64, 4, "mixed"), (64, 2048, 1032, 32, 20, "mixed"), (65, 264, 520, 128, 3, "runs"), (127, 320, 64, 16, 300, "mixed"),
     (128, 640, 256, 256, 2, "mixed"), (129, 1032, 392, 72, 7, "runs"), (300, 4096, 24, 64, 40, "mixed"), (511, 136, 2056, 16, 3, "runs"),
     (1000, 768, 776, 200, 6, "runs"), (2049, 256, 512, 64, 9, "runs"), (4100, 512, 1544, 32, 4, "runs"),
+    (9473, 200, 136, 72, 9, "mixed"), (9728, 1032, 264, 128, 5, "runs"), (19200, 520, 72, 16, 3, "runs"),
 ]
 
 
