@@ -67,9 +67,27 @@ __device__ __forceinline__ bool mbar_wait_one(uint64_t* bar, uint32_t parity, vo
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     return __all_sync(0xffffffffu, mbar_wait_one(bar, parity, abort_flag, status, code));
 }
+// A place in a ring of stages and the parity of its current round (kept by counting: dividing a running number by a
+// stage count that is known at run time only costs more than the rest of a loop's step).  A consumer waits for parity
+// `round`, a producer for the other one, which a fresh barrier grants at once.
+struct Ring {
+    int at = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++at == stages) { at = 0; round ^= 1u; }
+    }
+};
+
 // What a role that gives up does for its copies and MMAs in flight: they end before shared memory and TMEM go.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(bar, parity); ++i) {}
+}
+// The copies of the last `issued` (at most all) stages before `ring`'s place.
+__device__ __forceinline__ void ring_drain(uint64_t* full, Ring ring, uint32_t issued, int stages) {
+    for (uint32_t i = 0; i < issued && i < (uint32_t)stages; ++i) {
+        if (--ring.at < 0) { ring.at = stages - 1; ring.round ^= 1u; }
+        mbar_drain(&full[ring.at], ring.round);
+    }
 }
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {

@@ -153,37 +153,42 @@ lora_few_kernel(const LoraArgs p) {
 
 // ------------------------------------------------------------------ many rows
 
-// The adapters that kRows rows from row0 on ask for, in the order of their first rows: their number, their ids in `list`
-// (where it is given) and,
-// in `slot`, each row's place in it (-1: none).  By a whole warp.
+// The ids that kRows rows from row0 on ask for (-1: none): lane l has rows l, l + 32, ...
 template <int kRows>
-__device__ __forceinline__ int tile_adapters(const LoraArgs& p, int64_t row0, int lane, int* list, int16_t* slot) {
-    constexpr int kQ = kRows / 32;
-    int id[kQ], place[kQ];
-    uint32_t left[kQ], any = 0;
+__device__ __forceinline__ void tile_ids(const LoraArgs& p, int64_t row0, int lane, int (&id)[kRows / 32]) {
 #pragma unroll
-    for (int q = 0; q < kQ; ++q) {
+    for (int q = 0; q < kRows / 32; ++q) {
         const int64_t row = row0 + 32 * q + lane;
         id[q] = row < p.rows ? adapter_of(p, row) : -1;
-        place[q] = -1;
     }
+}
+
+// The different adapters among them, in the order of their first rows: calls each(place, id, first row, last row) with
+// every lane, leaves each row's place in `slot` (-1: none) and returns their number.  By a whole warp.
+template <int kRows, typename Each>
+__device__ __forceinline__ int tile_adapters(const int (&id)[kRows / 32], int lane, int16_t* slot, Each each) {
+    constexpr int kQ = kRows / 32;
+    int place[kQ];
+    uint32_t left[kQ], any = 0;
 #pragma unroll
-    for (int q = 0; q < kQ; ++q) any |= left[q] = __ballot_sync(0xffffffffu, id[q] >= 0);
+    for (int q = 0; q < kQ; ++q) { any |= left[q] = __ballot_sync(0xffffffffu, id[q] >= 0); place[q] = -1; }
     int count = 0;
     while (any) {
-        int cur = -1;
+        int cur = -1, lo = 0, hi = 0;
 #pragma unroll
         for (int q = kQ - 1; q >= 0; --q) {   // (the first 32 rows that have one left decide)
             const int first = __shfl_sync(0xffffffffu, id[q], left[q] ? __ffs(left[q]) - 1 : 0);
-            if (left[q]) cur = first;
+            if (left[q]) { cur = first; lo = 32 * q + __ffs(left[q]) - 1; }
         }
         any = 0;
 #pragma unroll
         for (int q = 0; q < kQ; ++q) {
+            const uint32_t same = __ballot_sync(0xffffffffu, id[q] == cur);
+            if (same) hi = 32 * q + 31 - __clz(same);
             if (id[q] == cur) place[q] = count;
-            any |= left[q] &= ~__ballot_sync(0xffffffffu, id[q] == cur);
+            any |= left[q] &= ~same;
         }
-        if (list && lane == 0) list[count] = cur;
+        each(count, cur, lo, hi);
         ++count;
     }
 #pragma unroll
@@ -237,21 +242,22 @@ struct ShrinkPlan {
     int k_tiles, halves;        // 64-element steps of K; 128-row tiles of A (2 for ranks over 128)
     int blocks;                 // 64-element blocks of R
     int x_stages, a_stages;     // rings of x and A tiles
-    int batch;                  // adapters that share a pass over x
     int smem;
 };
 
 constexpr int kShrinkRows = 256;           // rows of x a CTA takes (the MMA's N)
 constexpr int kShrinkThreads = 320;        // warp 0: TMA, warp 1: MMA, warps 2-9: epilogue
 constexpr int kXBytes = kShrinkRows * 128;
+constexpr int kShrinkColumns = 512;        // all of TMEM
 
 // low[t][:] = A_{ids[t]} x[t] for 256 rows, as the image that the second product reads.
 //
 // The product is taken as A x^T: an MMA of 128 rows costs 128 clocks whether it has 64 columns or 256, so the rank is its M
 // (padded with zeros) and 256 tokens its N; with the roles the other way round the tensor cores, not HBM, were the bound.
 // The accumulator holds a token per column, and its 32 lanes store consecutive elements of a token's vector.
-// Up to `batch` adapters share a pass over x, each with an accumulator of its own: a tile in which two requests meet costs
-// the other's A tiles (from L2) and products, not a second read of x.
+// Adapters share a pass over x as long as their accumulators fit TMEM.  An adapter's product is taken only for the tokens
+// from the first to the last that asks for it, so requests that lie behind one another fit by the dozen: a tile in which
+// some meet costs their A tiles (from L2), not a second read of x, and no tile holds up the launch.
 // The CTAs of a cluster take parts of K.  Each leaves its sums in global memory, and after the cluster's barrier each adds
 // up a share of the tokens, in the order of the parts, and writes their image.
 template <typename T>
@@ -271,8 +277,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* acc_empty = acc_full + 1;
     uint64_t* drain = acc_empty + 1;
     uint64_t* listed = drain + 1;
-    int* s_list = reinterpret_cast<int*>(listed + 1);
-    int16_t* s_slot = reinterpret_cast<int16_t*>(s_list + kShrinkRows);
+    int* s_list = reinterpret_cast<int*>(listed + 1);                        // [adapter]: id,
+    int16_t* s_from = reinterpret_cast<int16_t*>(s_list + kShrinkRows);      // first token (a multiple of 8)
+    int16_t* s_wide = s_from + kShrinkRows;                                  // and number of tokens (of 16)
+    int16_t* s_slot = s_wide + kShrinkRows;                                  // [token]: which adapter
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slot + kShrinkRows);
     int* s_count = reinterpret_cast<int*>(s_tmem + 1);
     volatile int* s_abort = s_count + 1;
@@ -282,8 +290,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     const int split = blockIdx.y, group = blockIdx.z;
     const int k0 = (int)((int64_t)plan.k_tiles * split / plan.splits), k1 = (int)((int64_t)plan.k_tiles * (split + 1) / plan.splits);
 
+    int id[kShrinkRows / 32];
+    if (warp == 2) tile_ids<kShrinkRows>(p, row0, lane, id);   // (before the flood of x)
     if (warp == 1) {
-        tc::tmem_alloc(s_tmem, 512);
+        tc::tmem_alloc(s_tmem, kShrinkColumns);
     } else if (threadIdx.x == 0) {
         for (int s = 0; s < plan.x_stages; ++s) { tc::mbar_init(&x_full[s], 1); tc::mbar_init(&x_empty[s], 1); }
         for (int s = 0; s < plan.a_stages; ++s) { tc::mbar_init(&a_full[s], 1); tc::mbar_init(&a_empty[s], 1); }
@@ -301,86 +311,97 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     const uint32_t tmem = *s_tmem;
 
     // x's first tiles are on their way before the ids are known (they are wanted unless nobody asks for an adapter)
-    uint32_t ahead = 0;
+    tc::Ring xr, ar;
+    int ahead = 0;
     if (warp == 0) {
-        for (; ahead < (uint32_t)min(plan.x_stages, k1 - k0) && plan.groups == 1; ++ahead) {
+        for (; ahead < min(plan.x_stages, k1 - k0) && plan.groups == 1; ++ahead) {
             if (tc::elect_one()) {
                 tc::mbar_expect_tx(&x_full[ahead], kXBytes);
-                tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + (int)ahead) * 64, (int)row0, &x_full[ahead]);
+                tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + ahead) * 64, (int)row0, &x_full[ahead]);
             }
             __syncwarp();
         }
     } else if (warp == 2) {
-        const int n = tile_adapters<kShrinkRows>(p, row0, lane, s_list, s_slot);
+        const int n = tile_adapters<kShrinkRows>(id, lane, s_slot, [&](int j, int which, int lo, int hi) {
+            const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
+            if (lane == 0) { s_list[j] = which; s_wide[j] = (int16_t)wide; s_from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
+        });
         if (lane == 0) { *s_count = n; tc::mbar_arrive(listed); }
         __syncwarp();
     }
     bool ok = tc::mbar_wait(listed, 0, s_abort, &g_lora_status, kWaitList);
     const int count = ok ? *s_count : 0;   // (the same in every CTA of the cluster)
-    // a batch: adapters j, j + groups, ... below `until`
-    const int stride = plan.batch * plan.groups;
+    // a batch: adapters first, first + groups, ... below `until`, their accumulators side by side
+    auto batch_end = [&](int first) {
+        int until = first, columns = 0;
+        while (until < count && (columns += plan.halves * s_wide[until]) <= kShrinkColumns) until += plan.groups;
+        return until;
+    };
     if (warp == 0) {
-        uint32_t xi = 0, ai = 0;
-        for (int first = group; first < count && ok; first += stride) {
-            const int until = min(count, first + stride);
-            for (int kt = k0; kt < k1 && ok; ++kt, ++xi) {
-                int s = xi % plan.x_stages;
-                if (xi >= ahead) {
-                    if (xi >= (uint32_t)plan.x_stages) ok = tc::mbar_wait(&x_empty[s], (xi / plan.x_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+        uint32_t xs = 0, as = 0;           // tiles issued
+        for (int first = group, until; first < count && ok; first = until) {
+            until = batch_end(first);
+            for (int kt = k0; kt < k1 && ok; ++kt) {
+                if (--ahead < 0) {
+                    ok = tc::mbar_wait(&x_empty[xr.at], xr.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
                     if (!ok) break;
                     if (tc::elect_one()) {
-                        tc::mbar_expect_tx(&x_full[s], kXBytes);
-                        tc::tma_load_2d(s_x + s * kXBytes, &map_x, kt * 64, (int)row0, &x_full[s]);
+                        tc::mbar_expect_tx(&x_full[xr.at], kXBytes);
+                        tc::tma_load_2d(s_x + xr.at * kXBytes, &map_x, kt * 64, (int)row0, &x_full[xr.at]);
                     }
                     __syncwarp();
-                    ahead = xi + 1;
                 }
-                for (int j = first; j < until; j += plan.groups, ++ai) {
-                    s = ai % plan.a_stages;
-                    if (ai >= (uint32_t)plan.a_stages) ok = tc::mbar_wait(&a_empty[s], (ai / plan.a_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+                ++xs;
+                xr.next(plan.x_stages);
+                for (int j = first; j < until; j += plan.groups) {
+                    ok = tc::mbar_wait(&a_empty[ar.at], ar.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
                     if (!ok) break;
                     const int which = s_list[j];
                     if (tc::elect_one()) {
-                        tc::mbar_expect_tx(&a_full[s], (uint32_t)a_bytes);
+                        tc::mbar_expect_tx(&a_full[ar.at], (uint32_t)a_bytes);
                         for (int h = 0; h < plan.halves; ++h)
-                            tc::tma_load_3d(s_a + s * a_bytes + h * kTileBytes, &map_a, kt * 64, h * kTile, which, &a_full[s]);
+                            tc::tma_load_3d(s_a + ar.at * a_bytes + h * kTileBytes, &map_a, kt * 64, h * kTile, which, &a_full[ar.at]);
                     }
                     __syncwarp();
+                    ++as;
+                    ar.next(plan.a_stages);
                 }
             }
         }
-        if (!ok || xi < ahead) {   // given up, or nobody asked: copies in flight land before the CTA leaves
-            for (uint32_t i = ahead > (uint32_t)plan.x_stages ? ahead - plan.x_stages : 0; i < ahead; ++i) tc::mbar_drain(&x_full[i % plan.x_stages], (i / plan.x_stages) & 1);
-            for (uint32_t i = ai > (uint32_t)plan.a_stages ? ai - plan.a_stages : 0; i < ai; ++i) tc::mbar_drain(&a_full[i % plan.a_stages], (i / plan.a_stages) & 1);
+        // given up, or nobody asked: copies in flight land before the CTA leaves
+        if (!ok || ahead > 0) {
+            for (; ahead > 0; --ahead, ++xs) xr.next(plan.x_stages);
+            tc::ring_drain(x_full, xr, xs, plan.x_stages);
+            tc::ring_drain(a_full, ar, as, plan.a_stages);
         }
     } else if (warp == 1) {
-        const uint32_t id = tc::idesc(Elem<T>::code == CK_BF16, kShrinkRows);
-        uint32_t xi = 0, ai = 0, n = 0;
-        for (int first = group; first < count && ok; first += stride, ++n) {
-            const int until = min(count, first + stride);
-            if (n > 0) ok = tc::mbar_wait(acc_empty, (n - 1) & 1, s_abort, &g_lora_status, kWaitAccFree);
-            for (int kt = k0; kt < k1 && ok; ++kt, ++xi) {
-                const int xs = xi % plan.x_stages;
-                ok = tc::mbar_wait(&x_full[xs], (xi / plan.x_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+        uint32_t n = 0;
+        for (int first = group, until; first < count && ok; first = until, ++n) {
+            until = batch_end(first);
+            ok = tc::mbar_wait(acc_empty, (n & 1) ^ 1, s_abort, &g_lora_status, kWaitAccFree);
+            for (int kt = k0; kt < k1 && ok; ++kt, xr.next(plan.x_stages)) {
+                ok = tc::mbar_wait(&x_full[xr.at], xr.round, s_abort, &g_lora_status, kWaitFull);
                 uint32_t d = tmem;
-                for (int j = first; j < until && ok; j += plan.groups, ++ai, d += kShrinkRows) {
-                    const int as = ai % plan.a_stages;
-                    ok = tc::mbar_wait(&a_full[as], (ai / plan.a_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+                for (int j = first; j < until && ok; j += plan.groups, ar.next(plan.a_stages)) {
+                    ok = tc::mbar_wait(&a_full[ar.at], ar.round, s_abort, &g_lora_status, kWaitFull);
                     if (!ok) break;
                     tc::fence_after();
+                    const int wide = s_wide[j];
+                    const uint32_t tokens = s_from[j], desc = tc::idesc(Elem<T>::code == CK_BF16, wide);
                     if (tc::elect_one()) {
-                        const uint32_t da = tc::desc_lo(s_a + as * a_bytes), db = tc::desc_lo(s_x + xs * kXBytes);
+                        const uint32_t da = tc::desc_lo(s_a + ar.at * a_bytes), db = tc::desc_lo(s_x + xr.at * kXBytes + tokens * 128);
                         for (int h = 0; h < plan.halves; ++h)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                tc::mma_16bit(d + h * kShrinkRows, da + h * (kTileBytes >> 4) + 2 * k, db + 2 * k, id, kt > k0 || k > 0);
-                        tc::commit(&a_empty[as]);
+                                tc::mma_16bit(d + h * wide, da + h * (kTileBytes >> 4) + 2 * k, db + 2 * k, desc, kt > k0 || k > 0);
+                        tc::commit(&a_empty[ar.at]);
                         if (j + plan.groups >= until) {
-                            tc::commit(&x_empty[xs]);
+                            tc::commit(&x_empty[xr.at]);
                             if (kt + 1 == k1) tc::commit(acc_full);
                         }
                     }
                     __syncwarp();
+                    d += plan.halves * wide;
                 }
             }
         }
@@ -390,31 +411,30 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             tc::mbar_drain(drain, 0);
         }
     } else {
-        // a warp: 32 elements of the vector (its TMEM lanes) of 128 of the tokens
-        const int quarter = warp & 3, token0 = ((warp - 2) >> 2) * kTile;
+        // a warp: 32 elements of the vector (its TMEM lanes) of every other 16 tokens
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
         uint32_t n = 0;
-        for (int first = group; first < count && ok; first += stride, ++n) {
-            const int until = min(count, first + stride);
+        for (int first = group, until; first < count && ok; first = until, ++n) {
+            until = batch_end(first);
             ok = tc::mbar_wait(acc_full, n & 1, s_abort, &g_lora_status, kWaitAcc);
             if (!ok) break;
             tc::fence_after();
-            uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + token0;
-            for (int j = first; j < until; j += plan.groups, acc += kShrinkRows) {
-                for (int h = 0; h < plan.halves; ++h) {
+            uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+            for (int j = first; j < until; j += plan.groups) {
+                const int wide = s_wide[j], from = s_from[j];
+                for (int h = 0; h < plan.halves; ++h, acc += wide) {
                     const int r = h * kTile + quarter * 32 + lane;
-                    if (r - lane >= p.R) break;
-                    float* dst = p.partial + ((int64_t)split * p.rows + row0 + token0) * p.R + r;
-                    for (int t = 0; t < kTile; t += 32) {
-                        const uint32_t asked = __ballot_sync(0xffffffffu, s_slot[token0 + t + lane] == j);
+                    float* dst = p.partial + ((int64_t)split * p.rows + row0 + from) * p.R + r;
+                    for (int t = half * 16; t < wide && r - lane < p.R; t += 32) {
+                        const uint32_t asked = __ballot_sync(0xffffffffu, lane < 16 && s_slot[from + t + (lane & 15)] == j);
                         if (!asked) continue;
-                        uint32_t v[2][16];
-                        tc::ld16(acc + h * kShrinkRows + t, v[0]);
-                        tc::ld16(acc + h * kShrinkRows + t + 16, v[1]);
+                        uint32_t v[16];
+                        tc::ld16(acc + t, v);
                         tc::wait_ld();
                         if (r < p.R) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (asked >> i & 1) dst[(t + i) * p.R] = __uint_as_float(v[i >> 4][i & 15]);
+                            for (int i = 0; i < 16; ++i)
+                                if (asked >> i & 1) dst[(t + i) * p.R] = __uint_as_float(v[i]);
                         }
                     }
                 }
@@ -427,47 +447,58 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 1) tc::tmem_free(tmem, 512);
+    if (warp == 1) tc::tmem_free(tmem, kShrinkColumns);
     tc::cluster_sync();
 
-    // the parts of K, added up: eight lanes a token, each with every eighth chunk of 8 elements
+    // the parts of K, added up: eight lanes a token, each with every eighth chunk of 8 elements; two tokens in flight
     const int mine0 = kShrinkRows * split / plan.splits, mine1 = kShrinkRows * (split + 1) / plan.splits, sub = lane & 7;
-    for (int r0 = mine0 + warp * 4; r0 < mine1; r0 += kShrinkThreads / 8) {
-        const int r = r0 + (lane >> 3);
-        const int64_t row = row0 + r;
-        const int j = r < mine1 && count > 0 ? s_slot[r] : -1;
-        const bool wanted = j >= 0 && j % plan.groups == group;
-        float v[kMaxRank / 64][8], most = 0.0f;
+    const int padded = (int)round_up(p.R, 16);   // (the second product's steps)
+    constexpr int kAtOnce = kShrinkThreads / 8;
+    for (int r0 = mine0 + warp * 4; r0 < mine1; r0 += 2 * kAtOnce) {
+        bool wanted[2];
+        float v[2][kMaxRank / 64][8];
 #pragma unroll
-        for (int u = 0; u < kMaxRank / 64; ++u) {
-            const int c = (u * 8 + sub) * 8;
+        for (int w = 0; w < 2; ++w) {
+            const int r = r0 + w * kAtOnce + (lane >> 3);
+            const int j = r < mine1 && count > 0 ? s_slot[r] : -1;
+            wanted[w] = j >= 0 && j % plan.groups == group;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
-            if (wanted && c < p.R) {
-                const float* src = p.partial + row * p.R + c;
+            for (int u = 0; u < kMaxRank / 64; ++u) {
+                const int c = (u * 8 + sub) * 8;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[w][u][i] = 0.0f;
+                if (wanted[w] && c < p.R) {
+                    const float* src = p.partial + (row0 + r) * p.R + c;
 #pragma unroll 4
-                for (int k = 0; k < plan.splits; ++k, src += p.rows * p.R) {
-                    const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
-                    v[u][0] += a.x; v[u][1] += a.y; v[u][2] += a.z; v[u][3] += a.w;
-                    v[u][4] += b.x; v[u][5] += b.y; v[u][6] += b.z; v[u][7] += b.w;
+                    for (int k = 0; k < plan.splits; ++k, src += p.rows * p.R) {
+                        const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
+                        v[w][u][0] += a.x; v[w][u][1] += a.y; v[w][u][2] += a.z; v[w][u][3] += a.w;
+                        v[w][u][4] += b.x; v[w][u][5] += b.y; v[w][u][6] += b.z; v[w][u][7] += b.w;
+                    }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[u][i]));
         }
-        float down = 1.0f, up = 1.0f;
-        if (Elem<T>::code == CK_F16) {
 #pragma unroll
-            for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            row_scale(most, down, up);
+        for (int w = 0; w < 2; ++w) {
+            const int r = r0 + w * kAtOnce + (lane >> 3);
+            float down = 1.0f, up = 1.0f;
+            if (Elem<T>::code == CK_F16) {
+                float most = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kMaxRank / 64; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[w][u][i]));
+#pragma unroll
+                for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                row_scale(most, down, up);
+            }
+            if (!wanted[w]) continue;
+            uint8_t* image = p.image + ((int64_t)blockIdx.x * 2 + (r >> 7)) * (2 * plan.blocks * kTileBytes);
+#pragma unroll
+            for (int u = 0; u < kMaxRank / 64; ++u)
+                if ((u * 8 + sub) * 8 < padded) put_image<T>(image, plan.blocks, r & 127, (u * 8 + sub) * 8, v[w][u], down);
+            if (sub == 0) p.factor[row0 + r] = p.scales ? up * __ldg(p.scales + s_list[s_slot[r]]) : up;
         }
-        if (!wanted) continue;
-        uint8_t* image = p.image + ((int64_t)blockIdx.x * 2 + (r >> 7)) * (2 * plan.blocks * kTileBytes);
-        const int padded = (int)round_up(p.R, 16);   // (the second product's steps)
-#pragma unroll
-        for (int u = 0; u < kMaxRank / 64; ++u)
-            if ((u * 8 + sub) * 8 < padded) put_image<T>(image, plan.blocks, r & 127, (u * 8 + sub) * 8, v[u], down);
-        if (sub == 0) p.factor[row] = p.scales ? up * __ldg(p.scales + s_list[j]) : up;
     }
 }
 
@@ -531,65 +562,72 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     tc::fence_after();
     const uint32_t tmem = *s_tmem;
 
+    int id[kTile / 32];
+    auto tile_count = [&](int64_t tile) {
+        tile_ids<kTile>(p, tile * kTile, lane, id);
+        return tile_adapters<kTile>(id, lane, s_slot, [](int, int, int, int) {});
+    };
     // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles
     if (warp == 0) {
-        uint32_t yi = 0;
+        tc::Ring yr;
+        uint32_t issued = 0;
         bool ok = true;
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            if (in_place && tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot) == 0) continue;
-            for (int64_t unit = begin * kU; unit < end * kU; ++unit) {
-                const int s = yi % plan.y_stages;
-                if (yi >= (uint32_t)plan.y_stages) ok = tc::mbar_wait(&y_empty[s], (yi / plan.y_stages - 1) & 1, s_abort, &g_lora_status, kWaitYFree);
+            if (in_place && tile_count(tile) == 0) continue;
+            for (int unit = (int)begin * kU; unit < (int)end * kU; ++unit) {
+                ok = tc::mbar_wait(&y_empty[yr.at], yr.round ^ 1u, s_abort, &g_lora_status, kWaitYFree);
                 if (!ok) break;
-                ++yi;
                 if (tc::elect_one()) {
-                    tc::mbar_expect_tx(&y_full[s], kTileBytes);
-                    tc::tma_load_2d(s_y + s * kTileBytes, &map_y, (int)unit * 64, (int)(tile * kTile), &y_full[s]);
+                    tc::mbar_expect_tx(&y_full[yr.at], kTileBytes);
+                    tc::tma_load_2d(s_y + yr.at * kTileBytes, &map_y, unit * 64, (int)(tile * kTile), &y_full[yr.at]);
                 }
                 __syncwarp();
+                ++issued;
+                yr.next(plan.y_stages);
             }
         }
-        if (!ok)
-            for (uint32_t i = yi > (uint32_t)plan.y_stages ? yi - plan.y_stages : 0; i < yi; ++i) tc::mbar_drain(&y_full[i % plan.y_stages], (i / plan.y_stages) & 1);
+        if (!ok) tc::ring_drain(y_full, yr, issued, plan.y_stages);
     } else if (warp == kExpandThreads / 32 - 1) {
-        uint32_t bi = 0;
+        tc::Ring br;
+        uint32_t issued = 0;
         bool ok = true;
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            const int count = tile_adapters<kTile>(p, tile * kTile, lane, s_list, s_slot);
-            for (int64_t step = begin; step < end && ok; ++step)
+            tile_ids<kTile>(p, tile * kTile, lane, id);
+            const int count = tile_adapters<kTile>(id, lane, s_slot, [&](int j, int which, int, int) { if (lane == 0) s_list[j] = which; });
+            for (int step = (int)begin; step < (int)end && ok; ++step)
                 for (int j = 0; j < count && ok; ++j) {
                     const int which = s_list[j];
                     for (int k = 0; k < plan.blocks; ++k) {
-                        const int s = bi % plan.b_stages;
-                        if (bi >= (uint32_t)plan.b_stages) ok = tc::mbar_wait(&b_empty[s], (bi / plan.b_stages - 1) & 1, s_abort, &g_lora_status, kWaitEmpty);
+                        ok = tc::mbar_wait(&b_empty[br.at], br.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
                         if (!ok) break;
-                        ++bi;
                         if (tc::elect_one()) {
-                            tc::mbar_expect_tx(&b_full[s], (uint32_t)b_bytes);
-                            tc::tma_load_3d(s_b + s * b_bytes, &map_b, k * 64, (int)(step * kStep), which, &b_full[s]);
+                            tc::mbar_expect_tx(&b_full[br.at], (uint32_t)b_bytes);
+                            tc::tma_load_3d(s_b + br.at * b_bytes, &map_b, k * 64, step * kStep, which, &b_full[br.at]);
                         }
                         __syncwarp();
+                        ++issued;
+                        br.next(plan.b_stages);
                     }
                 }
         }
-        if (!ok)
-            for (uint32_t i = bi > (uint32_t)plan.b_stages ? bi - plan.b_stages : 0; i < bi; ++i) tc::mbar_drain(&b_full[i % plan.b_stages], (i / plan.b_stages) & 1);
+        if (!ok) tc::ring_drain(b_full, br, issued, plan.b_stages);
     } else if (warp == 1) {
-        const uint32_t id = tc::idesc(Elem<T>::code == CK_BF16, kStep);
+        const uint32_t desc = tc::idesc(Elem<T>::code == CK_BF16, kStep);
         const int k_steps = (int)ceil_div(p.R, 16);
-        uint32_t bi = 0, n = 0, seg = 0;
+        tc::Ring br;
+        uint32_t n = 0, seg = 0;
         bool ok = true;
         tc::wait_for_dependency();      // the first kernel's image
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            const int count = tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot);
+            const int count = tile_count(tile);
             if (count == 0) continue;
-            if (seg > 0) ok = tc::mbar_wait(low_done, (seg - 1) & 1, s_abort, &g_lora_status, kWaitAcc);   // nothing reads s_low any more
+            ok = tc::mbar_wait(low_done, (seg & 1) ^ 1, s_abort, &g_lora_status, kWaitAcc);   // nothing reads s_low any more
             if (!ok) break;
             if (tc::elect_one()) {
                 tc::mbar_expect_tx(low_full, low_bytes);
@@ -598,28 +636,28 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
             __syncwarp();
             ok = tc::mbar_wait(low_full, seg & 1, s_abort, &g_lora_status, kWaitLow);
             ++seg;
-            for (int64_t i = 0; i < (end - begin) * count && ok; ++i, ++n) {
+            const int products = (int)(end - begin) * count;
+            for (int i = 0; i < products && ok; ++i, ++n) {
                 const uint32_t buf = n & 1;
-                if (n >= 2) ok = tc::mbar_wait(&acc_empty[buf], (n / 2 - 1) & 1, s_abort, &g_lora_status, kWaitAccFree);
+                ok = tc::mbar_wait(&acc_empty[buf], (n >> 1 & 1) ^ 1, s_abort, &g_lora_status, kWaitAccFree);
                 if (!ok) break;
-                for (int k = 0; k < k_steps; k += 4, ++bi) {
-                    const int s = bi % plan.b_stages;
-                    ok = tc::mbar_wait(&b_full[s], (bi / plan.b_stages) & 1, s_abort, &g_lora_status, kWaitFull);
+                for (int k = 0; k < k_steps; k += 4, br.next(plan.b_stages)) {
+                    ok = tc::mbar_wait(&b_full[br.at], br.round, s_abort, &g_lora_status, kWaitFull);
                     if (!ok) break;
                     tc::fence_after();
                     if (tc::elect_one()) {
                         const uint32_t d = tmem + buf * kStep, to_lo = plan.blocks * (kTileBytes >> 4);
-                        const uint32_t da = tc::desc_lo(s_low) + (k >> 2) * (kTileBytes >> 4), db = tc::desc_lo(s_b + s * b_bytes);
+                        const uint32_t da = tc::desc_lo(s_low) + (k >> 2) * (kTileBytes >> 4), db = tc::desc_lo(s_b + br.at * b_bytes);
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             if (k + u < k_steps) {
-                                tc::mma_16bit(d, da + 2 * u, db + 2 * u, id, k + u > 0);
-                                tc::mma_16bit(d, da + to_lo + 2 * u, db + 2 * u, id, 1);
+                                tc::mma_16bit(d, da + 2 * u, db + 2 * u, desc, k + u > 0);
+                                tc::mma_16bit(d, da + to_lo + 2 * u, db + 2 * u, desc, 1);
                             }
-                        tc::commit(&b_empty[s]);
+                        tc::commit(&b_empty[br.at]);
                         if (k + 4 >= k_steps) {
                             tc::commit(&acc_full[buf]);
-                            if (i + 1 == (end - begin) * count) tc::commit(low_done);
+                            if (i + 1 == products) tc::commit(low_done);
                         }
                     }
                     __syncwarp();
@@ -636,33 +674,36 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         const uint32_t group = (warp - 2) >> 2;
         const int quarter = warp & 3, r_in_tile = quarter * 32 + lane;
         const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-        uint32_t unit = 0, n = 0;       // units and accumulators so far
+        tc::Ring yr;                    // the step's first unit
+        uint32_t n = 0;                 // accumulators so far
+        uint32_t odd = 0;               // the parity of the step's first unit: which group takes it
         int before = -1;                // the stage whose store may still be reading
         bool ok = true;
         tc::wait_for_dependency();      // the first kernel's factors
         for (int64_t item = first; item < last && ok;) {
             const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
             item += end - begin;
-            const int count = tile_adapters<kTile>(p, tile * kTile, lane, nullptr, s_slot);
+            const int count = tile_count(tile);
             if (count == 0 && in_place) continue;
             const int mine = s_slot[r_in_tile];
             const float factor = mine >= 0 ? __ldcg(p.factor + tile * kTile + r_in_tile) : 0.0f;
-            for (int64_t step = begin; step < end && ok; ++step, unit += kU) {
+            for (int step = (int)begin; step < (int)end && ok; ++step) {
                 for (int j = 0; j < count && ok; ++j, ++n) {
                     const uint32_t buf = n & 1;
-                    ok = tc::mbar_wait(&acc_full[buf], (n / 2) & 1, s_abort, &g_lora_status, kWaitAcc);
+                    ok = tc::mbar_wait(&acc_full[buf], n >> 1 & 1, s_abort, &g_lora_status, kWaitAcc);
                     if (!ok) break;
                     tc::fence_after();
                     if (__any_sync(0xffffffffu, mine == j)) {
+                        tc::Ring r = yr;
 #pragma unroll 1
-                        for (int u = (int)((unit ^ group) & 1); u < kU; u += kEpiGroups) {
-                            const int ys = (unit + u) % plan.y_stages;
-                            uint8_t* mine_y = s_y + ys * kTileBytes + r_in_tile * 128;
+                        for (uint32_t u = 0; u < kU; ++u, r.next(plan.y_stages)) {
+                            if (((u + odd) & 1) != group) continue;
+                            uint8_t* mine_y = s_y + r.at * kTileBytes + r_in_tile * 128;
                             uint32_t v[4][16];
 #pragma unroll
                             for (int c = 0; c < 4; ++c) tc::ld16(acc + buf * kStep + u * 64 + 16 * c, v[c]);
                             tc::wait_ld();
-                            ok = ok && tc::mbar_wait(&y_full[ys], ((unit + u) / plan.y_stages) & 1, s_abort, &g_lora_status, kWaitY);
+                            ok = ok && tc::mbar_wait(&y_full[r.at], r.round, s_abort, &g_lora_status, kWaitY);
                             if (ok && mine == j) {
                                 // (all of y's row is read before any of it is written: nothing orders the eight chunks)
                                 Raw8<T> raw[8];
@@ -688,25 +729,26 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 if (!ok) break;
                 tc::fence_async_smem();
                 __syncwarp();
-                for (int u = (int)((unit ^ group) & 1); u < kU && ok; u += kEpiGroups) {
-                    const int ys = (unit + u) % plan.y_stages;
-                    ok = tc::mbar_wait(&y_full[ys], ((unit + u) / plan.y_stages) & 1, s_abort, &g_lora_status, kWaitY);
+                for (uint32_t u = 0; u < kU; ++u, yr.next(plan.y_stages)) {
+                    if (((u + odd) & 1) != group) continue;
+                    ok = ok && tc::mbar_wait(&y_full[yr.at], yr.round, s_abort, &g_lora_status, kWaitY);
                     if (ok && lane == 0) {
-                        tc::tma_store_2d(&map_out, s_y + ys * kTileBytes + quarter * 32 * 128, (int)(step * kStep) + u * 64, (int)(tile * kTile) + quarter * 32);
+                        tc::tma_store_2d(&map_out, s_y + yr.at * kTileBytes + quarter * 32 * 128, step * kStep + (int)u * 64, (int)(tile * kTile) + quarter * 32);
                         tc::tma_store_commit();
                         // a stage is handed back when its store has read it: with the group's next unit, where a whole step
                         // fits beside the two stages that are then still out
                         if (plan.y_stages >= kU + kEpiGroups) {
                             tc::tma_store_wait_read<1>();
                             if (before >= 0) tc::mbar_arrive(&y_empty[before]);
-                            before = ys;
+                            before = yr.at;
                         } else {
                             tc::tma_store_wait_read<0>();
-                            tc::mbar_arrive(&y_empty[ys]);
+                            tc::mbar_arrive(&y_empty[yr.at]);
                         }
                     }
                     __syncwarp();
                 }
+                odd ^= kU & 1;
             }
         }
         if (lane == 0) tc::tma_store_wait_read<0>();
@@ -738,24 +780,65 @@ int sm_count() {
 #endif
 bool few_rows(int64_t rows) { return rows <= CK_LORA_FEW; }
 
+template <typename K>
+int opt_in(K kernel, int which) {   // dynamic shared memory beyond 48 KB, once per kernel and device
+    static bool done[8][64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && done[which][dev]) return CK_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e != cudaSuccess) CK_FAIL((int)e, "lora_add: cannot reserve %d bytes of shared memory: %s", kSmemMost, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) done[which][dev] = true;
+    return CK_OK;
+}
+
+// How many clusters of 2^log_size CTAs of the first kernel, one CTA an SM, the current device holds at once (clusters do
+// not cross its groups of SMs: 16 of 8 CTAs, not 18, on a device of 148 SMs).
+int resident_clusters(int log_size, int smem) {
+    static int cached[64][4] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const bool known = dev >= 0 && dev < 64;
+    if (known && cached[dev][log_size]) return cached[dev][log_size];
+    const int size = 1 << log_size;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, size, 1024);
+    cfg.blockDim = dim3(kShrinkThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1; attr.val.clusterDim.y = size; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (opt_in(lora_shrink_kernel<__nv_bfloat16>, 1) != CK_OK ||
+        cudaOccupancyMaxActiveClusters(&n, lora_shrink_kernel<__nv_bfloat16>, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        n = sm_count() / size;
+    }
+    if (known) cached[dev][log_size] = n;
+    return n;
+}
+
 ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R, int64_t L) {
     ShrinkPlan s{};
-    const int64_t tiles = ceil_div(rows, kShrinkRows), slots = sm_count();
+    const int64_t tiles = ceil_div(rows, kShrinkRows);
     s.k_tiles = (int)ceil_div(K, 64);
     s.halves = R > kTile ? 2 : 1;
     s.blocks = (int)ceil_div(R, 64);
-    int64_t splits = slots / tiles, most = s.k_tiles / 4;   // at least four steps of K each
-    if (splits > most) splits = most;
-    s.splits = (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
-    int64_t groups = slots / (tiles * s.splits), asked = rows < kShrinkRows ? rows : kShrinkRows;
-    if (groups > asked) groups = asked;
-    if (groups > L) groups = L;
-    s.groups = (int)(groups < 1 ? 1 : groups);
-    s.batch = s.halves == 2 ? 1 : 2;                         // (of 256 TMEM columns each)
-    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + kShrinkRows * 6 + 16;
+    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + kShrinkRows * 10 + 16;
     s.x_stages = (kSmemMost - rest - a_bytes) / (kXBytes + a_bytes);
     s.a_stages = s.x_stages + 1;
     s.smem = rest + s.x_stages * kXBytes + s.a_stages * a_bytes;
+    // K is split as far as all tiles' clusters run at once and every part keeps four steps
+    int log_splits = 3;
+    while (log_splits > 0 && (tiles > resident_clusters(log_splits, s.smem) || (4 << log_splits) > s.k_tiles)) --log_splits;
+    s.splits = 1 << log_splits;
+    // and what is then left of the machine shares out a tile's adapters
+    int64_t groups = resident_clusters(log_splits, s.smem) / tiles, asked = rows < kShrinkRows ? rows : kShrinkRows;
+    if (groups > asked) groups = asked;
+    if (groups > L) groups = L;
+    s.groups = (int)(groups < 1 ? 1 : groups);
     return s;
 }
 
@@ -769,18 +852,6 @@ Workspace workspace_of(const ShrinkPlan& s, int64_t rows, int64_t R) {
     w.partial = w.factor + round_up(rows * 4, 128);
     w.bytes = w.partial + (int64_t)s.splits * rows * R * 4;
     return w;
-}
-
-template <typename K>
-int opt_in(K kernel, int which) {   // dynamic shared memory beyond 48 KB, once per kernel and device
-    static bool done[8][64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && done[which][dev]) return CK_OK;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
-    if (e != cudaSuccess) CK_FAIL((int)e, "lora_add: cannot reserve %d bytes of shared memory: %s", kSmemMost, cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) done[which][dev] = true;
-    return CK_OK;
 }
 
 int launched(cudaError_t e, const char* what) {
@@ -797,14 +868,16 @@ int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     e.items = e.steps * ceil_div(p.rows, kTile);
     e.blocks = (int)ceil_div(p.R, 64);
     const int rest = 1024 + 40 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 16;
-    // the image, a stage of B and a step's units of y (they are freed together); then y and B in turn
-    int room = kSmemMost - rest - 2 * e.blocks * kTileBytes - b_bytes - kU * kTileBytes;
-    if (room < 0) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld does not fit", (long long)p.R);
+    // The image, a stage of B and a step's units of y (at least two: their number is even, so that a stage always serves
+    // the same group of epilogue warps; a group that waited for a stage whose last load it had not seen might mistake that
+    // one's end for its own); then y and B in turn.
     e.b_stages = 1;
-    e.y_stages = kU;
+    e.y_stages = kU > 2 ? kU : 2;
+    int room = kSmemMost - rest - 2 * e.blocks * kTileBytes - b_bytes - e.y_stages * kTileBytes;
+    if (room < 0) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld does not fit", (long long)p.R);
     while (e.y_stages < 8 || e.b_stages < 4) {
-        const bool y = e.y_stages < 8 && room >= kTileBytes;
-        if (y) { ++e.y_stages; room -= kTileBytes; }
+        const bool y = e.y_stages < 8 && room >= 2 * kTileBytes;
+        if (y) { e.y_stages += 2; room -= 2 * kTileBytes; }
         const bool b = e.b_stages < 4 && room >= b_bytes;
         if (b) { ++e.b_stages; room -= b_bytes; }
         if (!b && !y) break;
@@ -894,7 +967,7 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     if (!y || !x || !a || !b || !ids || !out) CK_FAIL(CK_ERR_NULL, "lora_add: null pointer");
     if (dtype_code != CK_F16 && dtype_code != CK_BF16) CK_FAIL(CK_ERR_DTYPE, "lora_add: dtype code %d (bf16 or fp16)", dtype_code);
     // (tiles are addressed with 32-bit coordinates; 2^27 rows keep the grid of the first product within its bounds)
-    if (rows <= 0 || rows > (1 << 27) || K <= 0 || K > (1 << 30) || N <= 0 || N > (1 << 30) || adapters <= 0 || adapters > 0x7fffffff ||
+    if (rows <= 0 || rows > (1 << 27) || K <= 0 || K > (1 << 24) || N <= 0 || N > (1 << 24) || adapters <= 0 || adapters > 0x7fffffff ||
         K % 8 != 0 || N % 8 != 0 || rows_per_id <= 0 || x_row_stride < K || y_row_stride < N || out_row_stride < N)
         CK_FAIL(CK_ERR_SHAPE, "lora_add: bad shape rows=%lld K=%lld N=%lld adapters=%lld (K and N multiples of 8)", (long long)rows,
                 (long long)K, (long long)N, (long long)adapters);

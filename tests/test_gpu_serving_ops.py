@@ -339,15 +339,31 @@ def test_lora(ck, case, dtype):
     assert ck.lora_add(own, x, a, b, ids, scales, out=own) is own and torch.equal(own, got)
 
 
-@pytest.mark.parametrize("rows", [3, 40, 200])
-def test_lora_nothing_to_add(ck, rows):
-    x, y, a, b, _, scales = _lora_case(rows, 128, 96, 16, 4, BF16, 8, "one")
+@pytest.mark.parametrize("rows,n,rank", [(3, 96, 16), (40, 96, 16), (200, 96, 16), (300, 4104, 256), (16500, 520, 128), (20000, 264, 64)])
+def test_lora_nothing_to_add(ck, rows, n, rank):
+    x, y, a, b, _, scales = _lora_case(rows, 512, n, rank, 4, BF16, 8, "one")
     for value in (-1, 4, -2 ** 31, 2 ** 31 - 1):
         ids = torch.full((rows,), value, device="cuda", dtype=torch.int32)
         assert torch.equal(_bytes(ck.lora_add(y, x, a, b, ids, scales)), _bytes(y))
     for value in (2 ** 32, -2 ** 63, 2 ** 63 - 1):
         ids = torch.full((rows,), value, device="cuda")
         assert torch.equal(_bytes(ck.lora_add(y, x, a, b, ids, scales)), _bytes(y))
+
+
+@pytest.mark.parametrize("rows,rank", [(700, 64), (5000, 128), (17000, 24), (3000, 256)])
+def test_lora_some_tiles_without_adapters(ck, rows, rank):
+    """Whole tiles that are copied between tiles that are not, in place and not, again and again."""
+    x, y, a, b, _, scales = _lora_case(rows, 264, 1032, rank, 4, BF16, rows, "one")
+    ids = (torch.arange(rows, device="cuda") // 150 * 7) % 11 - 3
+    first = ck.lora_add(y, x, a, b, ids, scales)
+    _check_lora(first, y, x, a, b, ids, scales)
+    for _ in range(20):
+        own = y.clone()
+        ck.lora_add(own, x, a, b, ids, scales, out=own)
+        assert torch.equal(ck.lora_add(y, x, a, b, ids, scales), first) and torch.equal(own, first)
+    from comfy_kitchen.backends import cuda
+
+    assert cuda.lora_device_status() == 0
 
 
 @pytest.mark.parametrize("rows", [5, 70, 300])
