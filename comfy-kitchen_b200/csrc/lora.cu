@@ -7,9 +7,10 @@
 // Bound by HBM in either direction: x is read once, y read and out written once (2 K + 4 N bytes a row), each used adapter
 // once; the products' 2 R (K + N) flop a row stay below that up to a rank of about 128.  Two forms:
 //   few rows:   one CTA per row.
-//   many rows:  two kernels of 128-row tiles on the tensor cores (tcgen05), joined by the low-rank vectors.
-//               shrink:  low[t, :] = A x[t]; the K axis is split over a cluster's CTAs where there are few tiles, and
-//                        their partial sums are added in order (no atomics, the same bits every time);
+//   many rows:  three kernels, the first and the last on the tensor cores (tcgen05):
+//               shrink:  low[t, :] = A x[t], equal shares of all tiles' K steps for every SM, partial sums in fp32;
+//               join:    the partial sums added in order (no atomics, the same bits every time) and laid out as the
+//                        next product's operand;
 //               expand:  out = y + scale * (B low), y tiles fetched and out tiles stored by TMA while the products run.
 // Ids are looked at on the device: a tile lists the adapters that its rows ask for, computes each one's product for all 128
 // rows and keeps a row's own (a row of another request never enters a sum, whatever it holds).  Requests that lie behind
@@ -30,7 +31,7 @@ constexpr int kTileBytes = kTile * 128;   // 128 rows x 64 elements
 constexpr int kSmemMost = 232448;
 
 __device__ int g_lora_status = 0;
-enum : int { kWaitFull = 1, kWaitEmpty = 2, kWaitAcc = 3, kWaitAccFree = 4, kWaitLow = 5, kWaitY = 6, kWaitYFree = 7, kWaitList = 8 };
+enum : int { kWaitFull = 1, kWaitEmpty = 2, kWaitAcc = 3, kWaitAccFree = 4, kWaitLow = 5, kWaitY = 6, kWaitYFree = 7, kWaitList = 8, kWaitDone = 9 };
 
 struct LoraArgs {
     const void* y;
@@ -42,7 +43,7 @@ struct LoraArgs {
     void* out;
     uint8_t* image;         // many rows: per tile the low-rank vectors as the second product's operand (hi blocks, lo blocks)
     float* factor;          // [rows]: what a row's second product is multiplied by
-    float* partial;         // [splits, rows, R], where K is split
+    float* partial;         // [parts, tiles of 256 rows, 256, R]
     int64_t rows, K, N, R, L;
     int64_t y_stride, x_stride, out_stride;
     int64_t rows_per_id;
@@ -238,28 +239,46 @@ __device__ __forceinline__ void put_image(uint8_t* image, int blocks, int row, i
 }
 
 struct ShrinkPlan {
-    int splits, groups;         // K parts (a cluster); adapters of a tile are dealt to `groups` clusters
     int k_tiles, halves;        // 64-element steps of K; 128-row tiles of A (2 for ranks over 128)
     int blocks;                 // 64-element blocks of R
+    int tiles, ctas;            // tiles of 256 rows; CTAs that share the tiles x k_tiles units,
+    int each, more;             // `each` units a CTA, and one more for the first `more` of them
+    int parts;                  // most CTAs that meet in one tile
     int x_stages, a_stages;     // rings of x and A tiles
     int smem;
 };
 
-constexpr int kShrinkRows = 256;           // rows of x a CTA takes (the MMA's N)
-constexpr int kShrinkThreads = 320;        // warp 0: TMA, warp 1: MMA, warps 2-9: epilogue
+constexpr int kShrinkRows = 256;           // rows of x in a tile (the MMA's N)
+constexpr int kShrinkThreads = 352;        // warp 0: TMA, warp 1: MMA, warps 2-9: epilogue, warp 10: the tiles' lists
 constexpr int kXBytes = kShrinkRows * 128;
 constexpr int kShrinkColumns = 512;        // all of TMEM
 
-// low[t][:] = A_{ids[t]} x[t] for 256 rows, as the image that the second product reads.
+// What the rows of a tile ask for.
+struct TileList {
+    int id[kShrinkRows];            // [adapter]: its id,
+    int16_t from[kShrinkRows];      // the first token (a multiple of 8)
+    int16_t wide[kShrinkRows];      // and the number of tokens (of 16) that its product is taken for
+    int16_t slot[kShrinkRows];      // [token]: which adapter (-1: none)
+    int count, unused;
+};
+
+// First unit (tile x K step) of a CTA's share, and the CTA whose share holds a unit.
+__device__ __forceinline__ int share(const ShrinkPlan& plan, int cta) { return plan.each * cta + min(cta, plan.more); }
+__device__ __forceinline__ int owner(const ShrinkPlan& plan, int unit) {
+    const int longer = plan.more * (plan.each + 1);
+    return unit < longer ? unit / (plan.each + 1) : plan.more + (unit - longer) / plan.each;
+}
+
+// low[t][:] = A_{ids[t]} x[t] as partial sums over parts of K: every CTA takes an equal run of (tile, K step) units, so that
+// all SMs are busy whatever the number of rows, and leaves one part for each tile that it meets.
 //
 // The product is taken as A x^T: an MMA of 128 rows costs 128 clocks whether it has 64 columns or 256, so the rank is its M
-// (padded with zeros) and 256 tokens its N; with the roles the other way round the tensor cores, not HBM, were the bound.
-// The accumulator holds a token per column, and its 32 lanes store consecutive elements of a token's vector.
+// (what lies behind it in shared memory only fills accumulator rows that nobody reads) and 256 tokens its N; with the roles
+// the other way round the tensor cores, not memory, were the bound.  The accumulator holds a token per column, and its 32
+// lanes store consecutive elements of a token's vector.
 // Adapters share a pass over x as long as their accumulators fit TMEM.  An adapter's product is taken only for the tokens
 // from the first to the last that asks for it, so requests that lie behind one another fit by the dozen: a tile in which
-// some meet costs their A tiles (from L2), not a second read of x, and no tile holds up the launch.
-// The CTAs of a cluster take parts of K.  Each leaves its sums in global memory, and after the cluster's barrier each adds
-// up a share of the tokens, in the order of the parts, and writes their image.
+// some meet costs their A tiles (from L2), not a second read of x.
 template <typename T>
 __global__ void __launch_bounds__(kShrinkThreads, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const LoraArgs p,
@@ -267,6 +286,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int a_bytes = plan.halves * kTileBytes;
+    const uint32_t a_tx = (uint32_t)p.R * 128;                                // (rows of A behind the rank are not fetched)
     uint8_t* s_x = smem;
     uint8_t* s_a = s_x + plan.x_stages * kXBytes;
     uint64_t* x_full = reinterpret_cast<uint64_t*>(s_a + plan.a_stages * a_bytes);
@@ -276,22 +296,16 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* acc_full = a_empty + plan.a_stages;
     uint64_t* acc_empty = acc_full + 1;
     uint64_t* drain = acc_empty + 1;
-    uint64_t* listed = drain + 1;
-    int* s_list = reinterpret_cast<int*>(listed + 1);                        // [adapter]: id,
-    int16_t* s_from = reinterpret_cast<int16_t*>(s_list + kShrinkRows);      // first token (a multiple of 8)
-    int16_t* s_wide = s_from + kShrinkRows;                                  // and number of tokens (of 16)
-    int16_t* s_slot = s_wide + kShrinkRows;                                  // [token]: which adapter
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slot + kShrinkRows);
-    int* s_count = reinterpret_cast<int*>(s_tmem + 1);
-    volatile int* s_abort = s_count + 1;
+    uint64_t* listed = drain + 1;                                             // [2] a tile's lists are there
+    uint64_t* unlisted = listed + 2;                                          // [2] nobody needs them any more
+    TileList* s_lists = reinterpret_cast<TileList*>(unlisted + 2);            // [2]
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_lists + 2);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row0 = (int64_t)blockIdx.x * kShrinkRows;
-    const int split = blockIdx.y, group = blockIdx.z;
-    const int k0 = (int)((int64_t)plan.k_tiles * split / plan.splits), k1 = (int)((int64_t)plan.k_tiles * (split + 1) / plan.splits);
+    const int unit0 = share(plan, blockIdx.x), unit1 = share(plan, blockIdx.x + 1);
+    const int tile0 = unit0 / plan.k_tiles, tile1 = (unit1 - 1) / plan.k_tiles;
 
-    int id[kShrinkRows / 32];
-    if (warp == 2) tile_ids<kShrinkRows>(p, row0, lane, id);   // (before the flood of x)
     if (warp == 1) {
         tc::tmem_alloc(s_tmem, kShrinkColumns);
     } else if (threadIdx.x == 0) {
@@ -300,7 +314,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         tc::mbar_init(acc_full, 1);
         tc::mbar_init(acc_empty, 8);
         tc::mbar_init(drain, 1);
-        tc::mbar_init(listed, 1);
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&listed[i], 1); tc::mbar_init(&unlisted[i], 10); }
         *s_abort = 0;
         tc::mbar_init_done();
     }
@@ -310,196 +324,231 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     tc::launch_dependents();
     const uint32_t tmem = *s_tmem;
 
-    // x's first tiles are on their way before the ids are known (they are wanted unless nobody asks for an adapter)
+    if (warp == 10) {
+        // lists, a tile ahead of the other warps
+        bool ok = true;
+        for (int tile = tile0; tile <= tile1 && ok; ++tile) {
+            const int at = (tile - tile0) & 1;
+            TileList& l = s_lists[at];
+            int id[kShrinkRows / 32];
+            tile_ids<kShrinkRows>(p, (int64_t)tile * kShrinkRows, lane, id);
+            ok = tc::mbar_wait(&unlisted[at], ((tile - tile0) >> 1 & 1) ^ 1, s_abort, &g_lora_status, kWaitList);
+            if (!ok) break;
+            const int found = tile_adapters<kShrinkRows>(id, lane, l.slot, [&](int j, int which, int lo, int hi) {
+                const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
+                if (lane == 0) { l.id[j] = which; l.wide[j] = (int16_t)wide; l.from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
+            });
+            if (lane == 0) { l.count = found; tc::mbar_arrive(&listed[at]); }
+            __syncwarp();
+        }
+    }
     tc::Ring xr, ar;
+    uint32_t xs = 0, as = 0, n = 0;     // tiles issued (warp 0); accumulator rounds
+    // x's first tiles are on their way before the ids are known (they are wanted unless nobody asks for an adapter)
     int ahead = 0;
     if (warp == 0) {
-        for (; ahead < min(plan.x_stages, k1 - k0) && plan.groups == 1; ++ahead) {
+        const int k0 = unit0 - tile0 * plan.k_tiles, k1 = min(plan.k_tiles, unit1 - tile0 * plan.k_tiles);
+        for (; ahead < min(plan.x_stages, k1 - k0); ++ahead) {
             if (tc::elect_one()) {
                 tc::mbar_expect_tx(&x_full[ahead], kXBytes);
-                tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + ahead) * 64, (int)row0, &x_full[ahead]);
+                tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + ahead) * 64, tile0 * kShrinkRows, &x_full[ahead]);
             }
             __syncwarp();
         }
-    } else if (warp == 2) {
-        const int n = tile_adapters<kShrinkRows>(id, lane, s_slot, [&](int j, int which, int lo, int hi) {
-            const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
-            if (lane == 0) { s_list[j] = which; s_wide[j] = (int16_t)wide; s_from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
-        });
-        if (lane == 0) { *s_count = n; tc::mbar_arrive(listed); }
-        __syncwarp();
     }
-    bool ok = tc::mbar_wait(listed, 0, s_abort, &g_lora_status, kWaitList);
-    const int count = ok ? *s_count : 0;   // (the same in every CTA of the cluster)
-    // a batch: adapters first, first + groups, ... below `until`, their accumulators side by side
-    auto batch_end = [&](int first) {
-        int until = first, columns = 0;
-        while (until < count && (columns += plan.halves * s_wide[until]) <= kShrinkColumns) until += plan.groups;
-        return until;
-    };
-    if (warp == 0) {
-        uint32_t xs = 0, as = 0;           // tiles issued
-        for (int first = group, until; first < count && ok; first = until) {
-            until = batch_end(first);
-            for (int kt = k0; kt < k1 && ok; ++kt) {
-                if (--ahead < 0) {
-                    ok = tc::mbar_wait(&x_empty[xr.at], xr.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
-                    if (!ok) break;
-                    if (tc::elect_one()) {
-                        tc::mbar_expect_tx(&x_full[xr.at], kXBytes);
-                        tc::tma_load_2d(s_x + xr.at * kXBytes, &map_x, kt * 64, (int)row0, &x_full[xr.at]);
+    bool ok = true;
+    for (int tile = tile0; tile <= tile1 && ok && warp < 10; ++tile) {
+        const int base = tile * plan.k_tiles, at = (tile - tile0) & 1;
+        const int k0 = max(0, unit0 - base), k1 = min(plan.k_tiles, unit1 - base);
+        ok = tc::mbar_wait(&listed[at], (tile - tile0) >> 1 & 1, s_abort, &g_lora_status, kWaitList);
+        const TileList& l = s_lists[at];
+        const int count = ok ? l.count : 0;
+        // a batch: adapters `first` to `until`, their accumulators side by side
+        auto batch_end = [&](int first) {
+            int until = first, columns = 0;
+            while (until < count && (columns += plan.halves * l.wide[until]) <= kShrinkColumns) ++until;
+            return until;
+        };
+        if (warp == 0) {
+            for (int first = 0, until; first < count && ok; first = until) {
+                until = batch_end(first);
+                for (int kt = k0; kt < k1 && ok; ++kt) {
+                    if (ahead > 0) --ahead;
+                    else {
+                        ok = tc::mbar_wait(&x_empty[xr.at], xr.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
+                        if (!ok) break;
+                        if (tc::elect_one()) {
+                            tc::mbar_expect_tx(&x_full[xr.at], kXBytes);
+                            tc::tma_load_2d(s_x + xr.at * kXBytes, &map_x, kt * 64, tile * kShrinkRows, &x_full[xr.at]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                }
-                ++xs;
-                xr.next(plan.x_stages);
-                for (int j = first; j < until; j += plan.groups) {
-                    ok = tc::mbar_wait(&a_empty[ar.at], ar.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
-                    if (!ok) break;
-                    const int which = s_list[j];
-                    if (tc::elect_one()) {
-                        tc::mbar_expect_tx(&a_full[ar.at], (uint32_t)a_bytes);
-                        for (int h = 0; h < plan.halves; ++h)
-                            tc::tma_load_3d(s_a + ar.at * a_bytes + h * kTileBytes, &map_a, kt * 64, h * kTile, which, &a_full[ar.at]);
+                    ++xs;
+                    xr.next(plan.x_stages);
+                    for (int j = first; j < until; ++j) {
+                        ok = tc::mbar_wait(&a_empty[ar.at], ar.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
+                        if (!ok) break;
+                        const int which = l.id[j];
+                        if (tc::elect_one()) {
+                            tc::mbar_expect_tx(&a_full[ar.at], a_tx);
+                            tc::tma_load_3d(s_a + ar.at * a_bytes, &map_a, kt * 64, 0, which, &a_full[ar.at]);
+                        }
+                        __syncwarp();
+                        ++as;
+                        ar.next(plan.a_stages);
                     }
-                    __syncwarp();
-                    ++as;
-                    ar.next(plan.a_stages);
                 }
             }
+            // a first tile in which nobody asked for an adapter: its x tiles are taken out of the ring again
+            for (; ahead > 0 && ok; --ahead) {
+                ok = tc::mbar_wait(&x_full[xr.at], xr.round, s_abort, &g_lora_status, kWaitFull);
+                if (lane == 0) tc::mbar_arrive(&x_empty[xr.at]);
+                __syncwarp();
+                ++xs;
+                xr.next(plan.x_stages);
+            }
+        } else if (warp == 1) {
+            for (int first = 0, until; first < count && ok; first = until, ++n) {
+                until = batch_end(first);
+                ok = tc::mbar_wait(acc_empty, (n & 1) ^ 1, s_abort, &g_lora_status, kWaitAccFree);
+                for (int kt = k0; kt < k1 && ok; ++kt, xr.next(plan.x_stages)) {
+                    ok = tc::mbar_wait(&x_full[xr.at], xr.round, s_abort, &g_lora_status, kWaitFull);
+                    uint32_t d = tmem;
+                    for (int j = first; j < until && ok; ++j, ar.next(plan.a_stages)) {
+                        ok = tc::mbar_wait(&a_full[ar.at], ar.round, s_abort, &g_lora_status, kWaitFull);
+                        if (!ok) break;
+                        tc::fence_after();
+                        const int wide = l.wide[j];
+                        const uint32_t tokens = l.from[j], desc = tc::idesc(Elem<T>::code == CK_BF16, wide);
+                        if (tc::elect_one()) {
+                            const uint32_t da = tc::desc_lo(s_a + ar.at * a_bytes), db = tc::desc_lo(s_x + xr.at * kXBytes + tokens * 128);
+                            for (int h = 0; h < plan.halves; ++h)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    tc::mma_16bit(d + h * wide, da + h * (kTileBytes >> 4) + 2 * k, db + 2 * k, desc, kt > k0 || k > 0);
+                            tc::commit(&a_empty[ar.at]);
+                            if (j + 1 == until) {
+                                tc::commit(&x_empty[xr.at]);
+                                if (kt + 1 == k1) tc::commit(acc_full);
+                            }
+                        }
+                        __syncwarp();
+                        d += plan.halves * wide;
+                    }
+                }
+            }
+            if (tile == tile0 && count == 0)   // (warp 0 takes the first tiles out)
+                for (int i = 0; i < min(plan.x_stages, k1 - k0); ++i) xr.next(plan.x_stages);
+        } else {
+            // a warp: 32 elements of the vector (its TMEM lanes) of every other 16 tokens
+            const int quarter = warp & 3, half = (warp - 2) >> 2;
+            float* part = p.partial + ((int64_t)((int)blockIdx.x - owner(plan, base)) * plan.tiles + tile) * kShrinkRows * p.R;
+            const int R = (int)p.R;
+            for (int first = 0, until; first < count && ok; first = until, ++n) {
+                until = batch_end(first);
+                ok = tc::mbar_wait(acc_full, n & 1, s_abort, &g_lora_status, kWaitAcc);
+                if (!ok) break;
+                tc::fence_after();
+                uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+                for (int j = first; j < until; ++j) {
+                    const int wide = l.wide[j], from = l.from[j];
+                    for (int h = 0; h < plan.halves; ++h, acc += wide) {
+                        const int r = h * kTile + quarter * 32 + lane;
+                        if (r - lane >= R) continue;
+                        float* dst = part + (from + half * 16) * R + r;
+                        for (int t = half * 16; t < wide; t += 32, dst += 32 * R) {
+                            const uint32_t asked = __ballot_sync(0xffffffffu, lane < 16 && l.slot[from + t + (lane & 15)] == j);
+                            if (!asked) continue;
+                            uint32_t v[16];
+                            tc::ld16(acc + t, v);
+                            tc::wait_ld();
+                            float* to = dst;
+                            if (asked == 0xffffu) {
+                                if (r < R) {
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i, to += R) *to = __uint_as_float(v[i]);
+                                }
+                            } else if (r < R) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i, to += R)
+                                    if (asked >> i & 1) *to = __uint_as_float(v[i]);
+                            }
+                        }
+                    }
+                }
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(acc_empty);
+            }
         }
-        // given up, or nobody asked: copies in flight land before the CTA leaves
-        if (!ok || ahead > 0) {
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&unlisted[at]);
+    }
+    if (!ok) {   // given up: copies and MMAs in flight end before shared memory and TMEM go
+        if (warp == 0) {
             for (; ahead > 0; --ahead, ++xs) xr.next(plan.x_stages);
             tc::ring_drain(x_full, xr, xs, plan.x_stages);
             tc::ring_drain(a_full, ar, as, plan.a_stages);
-        }
-    } else if (warp == 1) {
-        uint32_t n = 0;
-        for (int first = group, until; first < count && ok; first = until, ++n) {
-            until = batch_end(first);
-            ok = tc::mbar_wait(acc_empty, (n & 1) ^ 1, s_abort, &g_lora_status, kWaitAccFree);
-            for (int kt = k0; kt < k1 && ok; ++kt, xr.next(plan.x_stages)) {
-                ok = tc::mbar_wait(&x_full[xr.at], xr.round, s_abort, &g_lora_status, kWaitFull);
-                uint32_t d = tmem;
-                for (int j = first; j < until && ok; j += plan.groups, ar.next(plan.a_stages)) {
-                    ok = tc::mbar_wait(&a_full[ar.at], ar.round, s_abort, &g_lora_status, kWaitFull);
-                    if (!ok) break;
-                    tc::fence_after();
-                    const int wide = s_wide[j];
-                    const uint32_t tokens = s_from[j], desc = tc::idesc(Elem<T>::code == CK_BF16, wide);
-                    if (tc::elect_one()) {
-                        const uint32_t da = tc::desc_lo(s_a + ar.at * a_bytes), db = tc::desc_lo(s_x + xr.at * kXBytes + tokens * 128);
-                        for (int h = 0; h < plan.halves; ++h)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                tc::mma_16bit(d + h * wide, da + h * (kTileBytes >> 4) + 2 * k, db + 2 * k, desc, kt > k0 || k > 0);
-                        tc::commit(&a_empty[ar.at]);
-                        if (j + plan.groups >= until) {
-                            tc::commit(&x_empty[xr.at]);
-                            if (kt + 1 == k1) tc::commit(acc_full);
-                        }
-                    }
-                    __syncwarp();
-                    d += plan.halves * wide;
-                }
-            }
-        }
-        if (!ok) {
+        } else if (warp == 1) {
             if (tc::elect_one()) tc::commit(drain);
             __syncwarp();
             tc::mbar_drain(drain, 0);
-        }
-    } else {
-        // a warp: 32 elements of the vector (its TMEM lanes) of every other 16 tokens
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        uint32_t n = 0;
-        for (int first = group, until; first < count && ok; first = until, ++n) {
-            until = batch_end(first);
-            ok = tc::mbar_wait(acc_full, n & 1, s_abort, &g_lora_status, kWaitAcc);
-            if (!ok) break;
-            tc::fence_after();
-            uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-            for (int j = first; j < until; j += plan.groups) {
-                const int wide = s_wide[j], from = s_from[j];
-                for (int h = 0; h < plan.halves; ++h, acc += wide) {
-                    const int r = h * kTile + quarter * 32 + lane;
-                    float* dst = p.partial + ((int64_t)split * p.rows + row0 + from) * p.R + r;
-                    for (int t = half * 16; t < wide && r - lane < p.R; t += 32) {
-                        const uint32_t asked = __ballot_sync(0xffffffffu, lane < 16 && s_slot[from + t + (lane & 15)] == j);
-                        if (!asked) continue;
-                        uint32_t v[16];
-                        tc::ld16(acc + t, v);
-                        tc::wait_ld();
-                        if (r < p.R) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (asked >> i & 1) dst[(t + i) * p.R] = __uint_as_float(v[i]);
-                        }
-                    }
-                }
-            }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(acc_empty);
         }
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     if (warp == 1) tc::tmem_free(tmem, kShrinkColumns);
-    tc::cluster_sync();
+}
 
-    // the parts of K, added up: eight lanes a token, each with every eighth chunk of 8 elements; two tokens in flight
-    const int mine0 = kShrinkRows * split / plan.splits, mine1 = kShrinkRows * (split + 1) / plan.splits, sub = lane & 7;
-    const int padded = (int)round_up(p.R, 16);   // (the second product's steps)
-    constexpr int kAtOnce = kShrinkThreads / 8;
-    for (int r0 = mine0 + warp * 4; r0 < mine1; r0 += 2 * kAtOnce) {
-        bool wanted[2];
-        float v[2][kMaxRank / 64][8];
+// The parts of K, added up in their order and written as the image that the second product reads: eight lanes a token, each
+// with every eighth chunk of 8 elements.
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs p, const ShrinkPlan plan) {
+    tc::launch_dependents();
+    const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 8) + (threadIdx.x >> 3);
+    const int sub = threadIdx.x & 7;
+    const int id = row < p.rows ? adapter_of(p, row) : -1;
+    const int base = (int)(row / kShrinkRows) * plan.k_tiles;
+    const int parts = owner(plan, base + plan.k_tiles - 1) - owner(plan, base) + 1;
+    const float scale = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.0f;
+    tc::wait_for_dependency();
+    float v[kMaxRank / 64][8];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const int r = r0 + w * kAtOnce + (lane >> 3);
-            const int j = r < mine1 && count > 0 ? s_slot[r] : -1;
-            wanted[w] = j >= 0 && j % plan.groups == group;
+    for (int u = 0; u < kMaxRank / 64; ++u) {
+        const int c = (u * 8 + sub) * 8;
 #pragma unroll
-            for (int u = 0; u < kMaxRank / 64; ++u) {
-                const int c = (u * 8 + sub) * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[w][u][i] = 0.0f;
-                if (wanted[w] && c < p.R) {
-                    const float* src = p.partial + (row0 + r) * p.R + c;
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+        if (id >= 0 && c < p.R) {
+            const float* src = p.partial + row * p.R + c;   // (row = tile * 256 + row in tile)
 #pragma unroll 4
-                    for (int k = 0; k < plan.splits; ++k, src += p.rows * p.R) {
-                        const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
-                        v[w][u][0] += a.x; v[w][u][1] += a.y; v[w][u][2] += a.z; v[w][u][3] += a.w;
-                        v[w][u][4] += b.x; v[w][u][5] += b.y; v[w][u][6] += b.z; v[w][u][7] += b.w;
-                    }
-                }
+            for (int k = 0; k < parts; ++k, src += (int64_t)plan.tiles * kShrinkRows * p.R) {
+                const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
+                v[u][0] += a.x; v[u][1] += a.y; v[u][2] += a.z; v[u][3] += a.w;
+                v[u][4] += b.x; v[u][5] += b.y; v[u][6] += b.z; v[u][7] += b.w;
             }
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const int r = r0 + w * kAtOnce + (lane >> 3);
-            float down = 1.0f, up = 1.0f;
-            if (Elem<T>::code == CK_F16) {
-                float most = 0.0f;
-#pragma unroll
-                for (int u = 0; u < kMaxRank / 64; ++u)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[w][u][i]));
-#pragma unroll
-                for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                row_scale(most, down, up);
-            }
-            if (!wanted[w]) continue;
-            uint8_t* image = p.image + ((int64_t)blockIdx.x * 2 + (r >> 7)) * (2 * plan.blocks * kTileBytes);
-#pragma unroll
-            for (int u = 0; u < kMaxRank / 64; ++u)
-                if ((u * 8 + sub) * 8 < padded) put_image<T>(image, plan.blocks, r & 127, (u * 8 + sub) * 8, v[w][u], down);
-            if (sub == 0) p.factor[row0 + r] = p.scales ? up * __ldg(p.scales + s_list[s_slot[r]]) : up;
         }
     }
+    float down = 1.0f, up = 1.0f;
+    if (Elem<T>::code == CK_F16) {
+        float most = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kMaxRank / 64; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[u][i]));
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        row_scale(most, down, up);
+    }
+    if (id < 0) return;
+    uint8_t* image = p.image + row / kTile * (2 * plan.blocks * kTileBytes);
+    const int padded = (int)round_up(p.R, 16);   // (the second product's steps)
+#pragma unroll
+    for (int u = 0; u < kMaxRank / 64; ++u)
+        if ((u * 8 + sub) * 8 < padded) put_image<T>(image, plan.blocks, (int)(row % kTile), (u * 8 + sub) * 8, v[u], down);
+    if (sub == 0) p.factor[row] = scale * up;
 }
 
 struct ExpandPlan {
@@ -510,11 +559,12 @@ struct ExpandPlan {
 };
 
 constexpr int kEpiGroups = 2;              // units of 64 columns are dealt to two groups of four epilogue warps
-constexpr int kExpandThreads = 96 + kEpiGroups * 128;   // warp 0: y's tiles, 1: MMA, 2-9: epilogue, 10: B's tiles
+constexpr int kExpandThreads = 128 + kEpiGroups * 128;  // warp 0: y's tiles, 1: MMA, 2-9: epilogue, 10: B's tiles, 11: stores
 
 // Persistent CTAs take equal runs of (tile, column step) items; a step is kU units of 64 columns.  The MMA of 128 rows
 // costs 128 clocks however few columns it has, and reads its 128 rows of the image from shared memory each time, so steps
-// are as wide as the number of items allows (16384 x 8192, rank 128: 225 us with 64 columns).
+// have two units (16384 x 8192, rank 128: 150 us; one unit 229 us, four units, whose tiles leave no room to fetch y ahead, 195)
+// unless that leaves SMs without an item.
 template <typename T, int kU>
 __global__ void __launch_bounds__(kExpandThreads, 1)
 lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y,
@@ -531,7 +581,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     uint64_t* b_empty = b_full + plan.b_stages;
     uint64_t* y_full = b_empty + plan.b_stages;
     uint64_t* y_empty = y_full + plan.y_stages;
-    uint64_t* acc_full = y_empty + plan.y_stages;                      // [2]
+    uint64_t* y_done = y_empty + plan.y_stages;                        // a unit's result is in its stage
+    uint64_t* acc_full = y_done + plan.y_stages;                       // [2]
     uint64_t* acc_empty = acc_full + 2;                                // [2]
     uint64_t* low_full = acc_empty + 2;
     uint64_t* low_done = low_full + 1;                                 // a tile's last MMA is complete
@@ -548,7 +599,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < plan.b_stages; ++s) { tc::mbar_init(&b_full[s], 1); tc::mbar_init(&b_empty[s], 1); }
-        for (int s = 0; s < plan.y_stages; ++s) { tc::mbar_init(&y_full[s], 1); tc::mbar_init(&y_empty[s], 4); }
+        for (int s = 0; s < plan.y_stages; ++s) { tc::mbar_init(&y_full[s], 1); tc::mbar_init(&y_empty[s], 1); tc::mbar_init(&y_done[s], 4); }
         for (int i = 0; i < 2; ++i) { tc::mbar_init(&acc_full[i], 1); tc::mbar_init(&acc_empty[i], 4 * kEpiGroups); }
         tc::mbar_init(low_full, 1);
         tc::mbar_init(low_done, 1);
@@ -589,7 +640,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
             }
         }
         if (!ok) tc::ring_drain(y_full, yr, issued, plan.y_stages);
-    } else if (warp == kExpandThreads / 32 - 1) {
+    } else if (warp == 10) {
         tc::Ring br;
         uint32_t issued = 0;
         bool ok = true;
@@ -670,6 +721,30 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
             tc::mbar_drain(drain, 0);
             if (seg > 0) tc::mbar_drain(low_full, (seg - 1) & 1);
         }
+    } else if (warp == 11) {
+        // stores in the units' order; a stage is handed back one store later, when its own has read it
+        tc::Ring yr;
+        int before = -1;
+        bool ok = true;
+        for (int64_t item = first; item < last && ok;) {
+            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
+            item += end - begin;
+            if (in_place && tile_count(tile) == 0) continue;
+            for (int unit = (int)begin * kU; unit < (int)end * kU; ++unit, yr.next(plan.y_stages)) {
+                ok = tc::mbar_wait(&y_done[yr.at], yr.round, s_abort, &g_lora_status, kWaitDone);
+                if (!ok) break;
+                if (lane == 0) {
+                    tc::tma_store_2d(&map_out, s_y + yr.at * kTileBytes, unit * 64, (int)(tile * kTile));
+                    tc::tma_store_commit();
+                    tc::tma_store_wait_read<1>();
+                    if (before >= 0) tc::mbar_arrive(&y_empty[before]);
+                }
+                __syncwarp();
+                before = yr.at;
+            }
+        }
+        if (lane == 0) tc::tma_store_wait_read<0>();
+        __syncwarp();
     } else {
         const uint32_t group = (warp - 2) >> 2;
         const int quarter = warp & 3, r_in_tile = quarter * 32 + lane;
@@ -677,7 +752,6 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::Ring yr;                    // the step's first unit
         uint32_t n = 0;                 // accumulators so far
         uint32_t odd = 0;               // the parity of the step's first unit: which group takes it
-        int before = -1;                // the stage whose store may still be reading
         bool ok = true;
         tc::wait_for_dependency();      // the first kernel's factors
         for (int64_t item = first; item < last && ok;) {
@@ -732,27 +806,11 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 for (uint32_t u = 0; u < kU; ++u, yr.next(plan.y_stages)) {
                     if (((u + odd) & 1) != group) continue;
                     ok = ok && tc::mbar_wait(&y_full[yr.at], yr.round, s_abort, &g_lora_status, kWaitY);
-                    if (ok && lane == 0) {
-                        tc::tma_store_2d(&map_out, s_y + yr.at * kTileBytes + quarter * 32 * 128, step * kStep + (int)u * 64, (int)(tile * kTile) + quarter * 32);
-                        tc::tma_store_commit();
-                        // a stage is handed back when its store has read it: with the group's next unit, where a whole step
-                        // fits beside the two stages that are then still out
-                        if (plan.y_stages >= kU + kEpiGroups) {
-                            tc::tma_store_wait_read<1>();
-                            if (before >= 0) tc::mbar_arrive(&y_empty[before]);
-                            before = yr.at;
-                        } else {
-                            tc::tma_store_wait_read<0>();
-                            tc::mbar_arrive(&y_empty[yr.at]);
-                        }
-                    }
-                    __syncwarp();
+                    if (ok && lane == 0) tc::mbar_arrive(&y_done[yr.at]);
                 }
                 odd ^= kU & 1;
             }
         }
-        if (lane == 0) tc::tma_store_wait_read<0>();
-        __syncwarp();
     }
     tc::fence_before();
     __syncthreads();
@@ -792,53 +850,22 @@ int opt_in(K kernel, int which) {   // dynamic shared memory beyond 48 KB, once 
     return CK_OK;
 }
 
-// How many clusters of 2^log_size CTAs of the first kernel, one CTA an SM, the current device holds at once (clusters do
-// not cross its groups of SMs: 16 of 8 CTAs, not 18, on a device of 148 SMs).
-int resident_clusters(int log_size, int smem) {
-    static int cached[64][4] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const bool known = dev >= 0 && dev < 64;
-    if (known && cached[dev][log_size]) return cached[dev][log_size];
-    const int size = 1 << log_size;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, size, 1024);
-    cfg.blockDim = dim3(kShrinkThreads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 1; attr.val.clusterDim.y = size; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (opt_in(lora_shrink_kernel<__nv_bfloat16>, 1) != CK_OK ||
-        cudaOccupancyMaxActiveClusters(&n, lora_shrink_kernel<__nv_bfloat16>, &cfg) != cudaSuccess || n <= 0) {
-        (void)cudaGetLastError();
-        n = sm_count() / size;
-    }
-    if (known) cached[dev][log_size] = n;
-    return n;
-}
-
-ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R, int64_t L) {
+ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R) {
     ShrinkPlan s{};
-    const int64_t tiles = ceil_div(rows, kShrinkRows);
     s.k_tiles = (int)ceil_div(K, 64);
     s.halves = R > kTile ? 2 : 1;
     s.blocks = (int)ceil_div(R, 64);
-    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + kShrinkRows * 10 + 16;
+    s.tiles = (int)ceil_div(rows, kShrinkRows);
+    const int units = s.tiles * s.k_tiles, most = (int)ceil_div(units, 4);   // at least four steps of K for a CTA
+    s.ctas = most < sm_count() ? most : sm_count();
+    s.each = units / s.ctas;
+    s.more = units % s.ctas;
+    s.parts = (int)ceil_div(s.k_tiles - 1, s.each) + 1;      // a run of k_tiles units touches at most this many shares
+    if (s.parts > s.ctas) s.parts = s.ctas;
+    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + 2 * (int)sizeof(TileList) + 16;
     s.x_stages = (kSmemMost - rest - a_bytes) / (kXBytes + a_bytes);
     s.a_stages = s.x_stages + 1;
     s.smem = rest + s.x_stages * kXBytes + s.a_stages * a_bytes;
-    // K is split as far as all tiles' clusters run at once and every part keeps four steps
-    int log_splits = 3;
-    while (log_splits > 0 && (tiles > resident_clusters(log_splits, s.smem) || (4 << log_splits) > s.k_tiles)) --log_splits;
-    s.splits = 1 << log_splits;
-    // and what is then left of the machine shares out a tile's adapters
-    int64_t groups = resident_clusters(log_splits, s.smem) / tiles, asked = rows < kShrinkRows ? rows : kShrinkRows;
-    if (groups > asked) groups = asked;
-    if (groups > L) groups = L;
-    s.groups = (int)(groups < 1 ? 1 : groups);
     return s;
 }
 
@@ -848,9 +875,9 @@ struct Workspace {
 };
 Workspace workspace_of(const ShrinkPlan& s, int64_t rows, int64_t R) {
     Workspace w{};
-    w.factor = ceil_div(rows, kShrinkRows) * (kShrinkRows / kTile) * 2 * s.blocks * kTileBytes;
+    w.factor = (int64_t)s.tiles * (kShrinkRows / kTile) * 2 * s.blocks * kTileBytes;
     w.partial = w.factor + round_up(rows * 4, 128);
-    w.bytes = w.partial + (int64_t)s.splits * rows * R * 4;
+    w.bytes = w.partial + (int64_t)s.parts * s.tiles * kShrinkRows * R * 4;
     return w;
 }
 
@@ -860,6 +887,22 @@ int launched(cudaError_t e, const char* what) {
     CK_FAIL((int)e, "lora_add (%s): %s", what, cudaGetErrorString(e));
 }
 
+// A launch; `chained`: its beginning may run beside the end of the kernel before it (wait_for_dependency()).
+struct Launch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = {};
+    Launch(unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, bool chained) {
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = chained ? 1 : 0;
+    }
+};
+
 template <typename T, int kU>
 int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     constexpr int kStep = kU * 64, b_bytes = kStep * 128;
@@ -867,12 +910,12 @@ int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     e.steps = ceil_div(p.N, kStep);
     e.items = e.steps * ceil_div(p.rows, kTile);
     e.blocks = (int)ceil_div(p.R, 64);
-    const int rest = 1024 + 40 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 16;
-    // The image, a stage of B and a step's units of y (at least two: their number is even, so that a stage always serves
+    const int rest = 1024 + 48 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 16;
+    // The image, a stage of B and four units of y (their number is even, so that a stage always serves
     // the same group of epilogue warps; a group that waited for a stage whose last load it had not seen might mistake that
     // one's end for its own); then y and B in turn.
     e.b_stages = 1;
-    e.y_stages = kU > 2 ? kU : 2;
+    e.y_stages = 4;
     int room = kSmemMost - rest - 2 * e.blocks * kTileBytes - b_bytes - e.y_stages * kTileBytes;
     if (room < 0) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld does not fit", (long long)p.R);
     while (e.y_stages < 8 || e.b_stages < 4) {
@@ -887,27 +930,18 @@ int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     const int64_t bd[3] = {p.R, p.N, p.L}, bs[2] = {p.R * 2, p.N * p.R * 2};
     const int64_t yd[2] = {p.N, p.rows}, ys[1] = {p.y_stride * 2}, os[1] = {p.out_stride * 2};
     if (!tc::make_map_16bit(&map_b, p.b, 3, bd, bs, kStep) || !tc::make_map_16bit(&map_y, p.y, 2, yd, ys, kTile) ||
-        !tc::make_map_16bit(&map_out, p.out, 2, yd, os, 32))
+        !tc::make_map_16bit(&map_out, p.out, 2, yd, os, kTile))
         CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: a tensor map could not be encoded");
     auto kernel = lora_expand_kernel<T, kU>;
     const int rc = opt_in(kernel, kU + (Elem<T>::code == CK_BF16 ? 0 : 4) - 1);
     if (rc != CK_OK) return rc;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its beginning runs beside the first kernel's end
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(e.items < sm_count() ? e.items : sm_count()));
-    cfg.blockDim = dim3(kExpandThreads);
-    cfg.dynamicSmemBytes = e.smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return launched(cudaLaunchKernelEx(&cfg, kernel, map_b, map_y, map_out, p, e), "expand");
+    Launch l((unsigned)(e.items < sm_count() ? e.items : sm_count()), kExpandThreads, e.smem, stream, true);
+    return launched(cudaLaunchKernelEx(&l.cfg, kernel, map_b, map_y, map_out, p, e), "expand");
 }
 
 template <typename T>
 int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
-    const ShrinkPlan s = shrink_plan(p.rows, p.K, p.R, p.L);
+    const ShrinkPlan s = shrink_plan(p.rows, p.K, p.R);
     const Workspace w = workspace_of(s, p.rows, p.R);
     p.image = workspace;
     p.factor = reinterpret_cast<float*>(workspace + w.factor);
@@ -915,27 +949,17 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
     CUtensorMap map_x, map_a;
     const int64_t xd[2] = {p.K, p.rows}, xs[1] = {p.x_stride * 2};
     const int64_t ad[3] = {p.K, p.R, p.L}, as[2] = {p.K * 2, p.R * p.K * 2};
-    if (!tc::make_map_16bit(&map_x, p.x, 2, xd, xs, kShrinkRows) || !tc::make_map_16bit(&map_a, p.a, 3, ad, as, kTile))
+    if (!tc::make_map_16bit(&map_x, p.x, 2, xd, xs, kShrinkRows) || !tc::make_map_16bit(&map_a, p.a, 3, ad, as, (int)p.R))
         CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: a tensor map could not be encoded");
     int rc = opt_in(lora_shrink_kernel<T>, Elem<T>::code == CK_BF16);
     if (rc != CK_OK) return rc;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = (unsigned)s.splits; attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ceil_div(p.rows, kShrinkRows), (unsigned)s.splits, (unsigned)s.groups);
-    cfg.blockDim = dim3(kShrinkThreads);
-    cfg.dynamicSmemBytes = s.smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    rc = launched(cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T>, map_x, map_a, p, s), "shrink");
+    Launch shrink((unsigned)s.ctas, kShrinkThreads, s.smem, stream, false);
+    rc = launched(cudaLaunchKernelEx(&shrink.cfg, lora_shrink_kernel<T>, map_x, map_a, p, s), "shrink");
     if (rc != CK_OK) return rc;
-    // the widest steps that still give every SM an item (and, beside the image of a rank over 128, fit shared memory)
-    const int64_t tiles = ceil_div(p.rows, kTile);
-    if (tiles * ceil_div(p.N, 256) >= sm_count() && p.R <= 128) return launch_expand<T, 4>(p, stream);
-    if (tiles * ceil_div(p.N, 128) >= sm_count()) return launch_expand<T, 2>(p, stream);
-    return launch_expand<T, 1>(p, stream);
+    Launch join((unsigned)ceil_div(p.rows, kJoinThreads / 8), kJoinThreads, 0, stream, true);
+    rc = launched(cudaLaunchKernelEx(&join.cfg, lora_join_kernel<T>, p, s), "join");
+    if (rc != CK_OK) return rc;
+    return ceil_div(p.rows, kTile) * ceil_div(p.N, 128) >= sm_count() ? launch_expand<T, 2>(p, stream) : launch_expand<T, 1>(p, stream);
 }
 
 }  // namespace
@@ -943,8 +967,9 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
 
 extern "C" int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t rank, int64_t adapters) {
     using namespace ck;
-    if (rows <= 0 || K <= 0 || rank <= 0 || adapters <= 0 || few_rows(rows)) return 0;
-    return workspace_of(shrink_plan(rows, K, rank, adapters), rows, rank).bytes;
+    if (rows <= 0 || rows > (1 << 27) || K <= 0 || K > (1 << 24) || rank <= 0 || adapters <= 0 || few_rows(rows)) return 0;
+    if (ceil_div(rows, kShrinkRows) * ceil_div(K, 64) > 0x3fffffff) return 0;   // (refused)
+    return workspace_of(shrink_plan(rows, K, rank), rows, rank).bytes;
 }
 
 extern "C" int ck_lora_device_status(void) {
@@ -971,6 +996,8 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
         K % 8 != 0 || N % 8 != 0 || rows_per_id <= 0 || x_row_stride < K || y_row_stride < N || out_row_stride < N)
         CK_FAIL(CK_ERR_SHAPE, "lora_add: bad shape rows=%lld K=%lld N=%lld adapters=%lld (K and N multiples of 8)", (long long)rows,
                 (long long)K, (long long)N, (long long)adapters);
+    if (ceil_div(rows, kShrinkRows) * ceil_div(K, 64) > 0x3fffffff)
+        CK_FAIL(CK_ERR_SHAPE, "lora_add: %lld rows of %lld are too many", (long long)rows, (long long)K);
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
