@@ -51,7 +51,7 @@ SIGNATURES: dict[str, list] = {
     "launch_adaln_quantize_nvfp4_rows_kernel": [P, P, P, P, P, P, I64, I64, I64, I64, F, I, B, I, I64, I64, P],
     "launch_adaln_quantize_mxfp8_kernel": [P, P, P, P, P, I64, I64, I64, I64, F, I, I, P],
     "launch_add_rmsnorm_quantize_kernel": [P, P, P, P, P, P, P, P, I64, I64, I64, I64, F, I, I, I, P],
-    "launch_apply_rope_axes_kernel": [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I, I, I, B, B, P],
+    "launch_apply_rope_axes_kernel": [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I, I, I, B, B, B, P],
     "launch_lora_add_kernel": [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I, B, P],
 }
 _RESTYPES = {"ck_last_error": c_char_p, "ck_tp_pad_bytes": c_int64, "ck_lora_workspace_bytes": c_int64}

@@ -15,6 +15,7 @@ the native side only launches on the current stream.  Nothing synchronises.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -639,6 +640,14 @@ def _row_stride(t: torch.Tensor, width: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else width
 
 
+def _empty(like: torch.Tensor, shape, dtype) -> torch.Tensor:
+    """A contiguous tensor on ``like``'s device; torch.empty_like is the cheapest way to one where it fits (1.4 against 2.6 us)."""
+    if shape is like.shape or shape == like.shape:
+        if like.is_contiguous():
+            return torch.empty_like(like) if dtype == like.dtype else torch.empty_like(like, dtype=dtype)
+    return like.new_empty(shape, dtype=dtype)
+
+
 def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm, sum_out):
     x, residual = _plain(x), _plain(residual)
     shape, dtype, device, stream_dtype = x.shape, x.dtype, x.device, residual.dtype
@@ -659,12 +668,15 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
     _no_grad(what, x, residual, weight)
     _same_device(what, device, residual, weight, sum_out)
     if sum_out is None:
-        sum_out = torch.empty_like(residual) if residual.is_contiguous() else residual.new_empty(shape)
+        sum_out = _empty(residual, shape, stream_dtype)
     elif sum_out.shape != shape or sum_out.dtype != stream_dtype or not sum_out.is_contiguous():
         raise ValueError(f"{what}: sum_out must be contiguous with the residual's shape and dtype")
-    norm = x.new_empty(shape) if return_norm else None
-    q = x.new_empty((n, d) if mx else shape, dtype=output_type)
-    sx = x.new_empty((roundup(n, 128), roundup(d // 32, 4)), dtype=torch.float8_e8m0fnu) if mx else None
+    norm = _empty(x, shape, dtype) if return_norm else None
+    q = _empty(x, (n, d) if mx and len(shape) != 2 else shape, output_type)
+    sx = None
+    if mx:
+        cols = (d // 32 + 3) // 4 * 4
+        sx = torch.empty_strided(((n + 127) // 128 * 128, cols), (cols, 1), dtype=torch.float8_e8m0fnu, device=device)
     if n:
         xf, rf = _rows_of(x, d), _rows_of(residual, d)
         _launch(device, "launch_add_rmsnorm_quantize_kernel", xf.data_ptr(), rf.data_ptr(), 0 if weight is None else weight.data_ptr(),
@@ -702,7 +714,17 @@ def add_rmsnorm_quantize_fp8(
     return (q, h, norm) if return_norm else (q, h)
 
 
-_Strides, _Pairs = ctypes.c_int64 * 17, ctypes.c_int32 * 8
+_Strides, _Pairs = ctypes.c_int64 * 11, ctypes.c_int32 * 8
+
+
+@functools.lru_cache(maxsize=256)
+def _axes(axes_dim: tuple):
+    """The C array of pairs per axis (read only), the elements that turn, the number of axes."""
+    if not 1 <= len(axes_dim) <= 8 or any(int(a) != a or a <= 0 or a % 2 for a in axes_dim):
+        raise ValueError
+    return _Pairs(*[int(a) // 2 for a in axes_dim]), int(sum(axes_dim)), len(axes_dim)
+
+
 _POSITION_CODES = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
 
 
@@ -721,8 +743,11 @@ def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim,
         heads_k = k_shape[heads_dim]
         if xk.dtype != dtype or k_shape[0] != b or k_shape[tokens_dim] != n or k_shape[3] != d:
             raise ValueError(f"{what}: q and k must agree in dtype and all dimensions but the heads")
-    turned, count = sum(axes_dim), len(axes_dim)
-    if not 1 <= count <= 8 or turned > d or d % 2 or any(a <= 0 or a % 2 for a in axes_dim):
+    try:
+        pairs, turned, count = _axes(tuple(axes_dim))
+    except ValueError:
+        turned = d + 1
+    if turned > d or d % 2:
         raise ValueError(f"{what}: axes_dim {list(axes_dim)} must be 1 to 8 positive even sizes that add up to at most the (even) head dim {d}")
     if freqs.dtype != torch.float64 or freqs.shape != (turned // 2,):
         raise ValueError(f"{what}: freqs must be float64 [{turned // 2}], one per pair")
@@ -736,8 +761,8 @@ def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim,
         raise ValueError(f"{what}: positions must be float32, float64, int32 or int64")
     _no_grad(what, xq, xk, positions, freqs)
     _same_device(what, device, xk, positions, freqs)
-    oq = xq.new_empty(q_shape)
-    ok = None if xk is None else xk.new_empty(k_shape)
+    oq = _empty(xq, q_shape, dtype)
+    ok = None if xk is None else _empty(xk, k_shape, dtype)
     if b == 0 or n == 0 or d == 0 or heads_q == 0 or (xk is not None and heads_k == 0):
         if oq.numel():
             oq, _ = _rope_axes(what, xq, None, positions, freqs, axes_dim, split_half, tokens_dim, inverse)
@@ -748,13 +773,11 @@ def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim,
         freqs = freqs.contiguous()
     sq, sp = xq.stride(), positions.stride()
     sk = sq if xk is None else xk.stride()
-    # contiguous outputs: [B, H, N, D] or [B, N, H, D]
-    (to, ho), (tk, hk) = ((d, n * d), (d, n * d)) if tokens_dim == 2 else ((heads_q * d, d), (heads_k * d, d))
-    strides = _Strides(sq[0], sq[tokens_dim], sq[heads_dim], sq[3], sk[0], sk[tokens_dim], sk[heads_dim], sk[3], heads_q * n * d, to, ho,
-                       heads_k * n * d, tk, hk, 0 if p_shape[0] == 1 else sp[0], sp[-2], sp[-1])
+    strides = _Strides(sq[0], sq[tokens_dim], sq[heads_dim], sq[3], sk[0], sk[tokens_dim], sk[heads_dim], sk[3],
+                       0 if p_shape[0] == 1 else sp[0], sp[-2], sp[-1])
     _launch(device, "launch_apply_rope_axes_kernel", xq.data_ptr(), 0 if xk is None else xk.data_ptr(), positions.data_ptr(), freqs.data_ptr(),
-            oq.data_ptr(), 0 if xk is None else ok.data_ptr(), strides, b, n, heads_q, heads_k, d, _Pairs(*[a // 2 for a in axes_dim]), count,
-            _code(dtype, what), code, split_half, inverse)
+            oq.data_ptr(), 0 if xk is None else ok.data_ptr(), strides, b, n, heads_q, heads_k, d, pairs, count,
+            _code(dtype, what), code, tokens_dim == 1, split_half, inverse)
     return oq, ok
 
 
@@ -817,32 +840,39 @@ def lora_add(
     _no_grad(what, y, x, a, b, scales)
     _same_device(what, device, y, a, b, adapter_ids, scales, out)
     if out is None:
-        out = y.new_empty(y_shape)
+        out = _empty(y, y_shape, dtype)
     elif out.shape != y_shape or out.dtype != dtype:
         raise ValueError(f"{what}: out must have y's shape and dtype")
     rows = x.numel() // k
     if rows == 0:
         return out
-
-    def aligned(t):   # the kernels move 16 bytes at a time
-        return t.data_ptr() % 16 == 0 and (t.is_contiguous() or t.shape[0] == 1 or t.stride(0) % 8 == 0)
-
+    # the kernels move 16 bytes at a time
     xf, yf, of = _rows_of(x, k), _rows_of(y, n), _rows_of(out, n)
-    if of.data_ptr() != out.data_ptr() or not aligned(of):
+    x_stride, y_stride, o_stride = _row_stride(xf, k), _row_stride(yf, n), _row_stride(of, n)
+    px, py, po, pa, pb = xf.data_ptr(), yf.data_ptr(), of.data_ptr(), a.data_ptr(), b.data_ptr()
+    if po != out.data_ptr() or po % 16 or o_stride % 8:
         raise ValueError(f"{what}: out must have unit column stride, rows of one stride and 16-byte alignment")
-    xf = xf if aligned(xf) else xf.clone(memory_format=torch.contiguous_format)
-    yf = yf if aligned(yf) else yf.clone(memory_format=torch.contiguous_format)
-    a = a if a.is_contiguous() and a.data_ptr() % 16 == 0 else a.clone(memory_format=torch.contiguous_format)
-    b = b if b.is_contiguous() and b.data_ptr() % 16 == 0 else b.clone(memory_format=torch.contiguous_format)
+    if px % 16 or x_stride % 8:
+        xf = xf.clone(memory_format=torch.contiguous_format)
+        px, x_stride = xf.data_ptr(), k
+    if py % 16 or y_stride % 8:
+        yf = yf.clone(memory_format=torch.contiguous_format)
+        py, y_stride = yf.data_ptr(), n
+    if pa % 16 or not a.is_contiguous():
+        a = a.clone(memory_format=torch.contiguous_format)
+        pa = a.data_ptr()
+    if pb % 16 or not b.is_contiguous():
+        b = b.clone(memory_format=torch.contiguous_format)
+        pb = b.data_ptr()
     ids = adapter_ids if adapter_ids.is_contiguous() else adapter_ids.contiguous()
     if scales is not None and not scales.is_contiguous():
         scales = scales.contiguous()
-    # fp32 partial sums of the first product; the allocator's, so that streams and captured graphs keep theirs apart
-    need = _native.load().ck_lora_workspace_bytes(rows, k, rank, adapters)
-    work = x.new_empty(need, dtype=torch.uint8) if need else None
-    _launch(device, "launch_lora_add_kernel", yf.data_ptr(), xf.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
-            0 if scales is None else scales.data_ptr(), of.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, _row_stride(yf, n), _row_stride(xf, k),
-            _row_stride(of, n), rows // ids.numel(), _code(dtype, what), ids_dtype == torch.int64)
+    # scratch of the tiled kernels; the allocator's, so that streams and captured graphs keep theirs apart
+    need = _native.load().ck_lora_workspace_bytes(rows, k, rank, adapters) if rows > 1 else 0
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch(device, "launch_lora_add_kernel", py, px, pa, pb, ids.data_ptr(), 0 if scales is None else scales.data_ptr(), po,
+            0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, y_stride, x_stride, o_stride, rows // ids.numel(),
+            _code(dtype, what), ids_dtype == torch.int64)
     return out
 
 
@@ -864,8 +894,6 @@ def build_constraints() -> dict:
     rope2 = fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                xk=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),)))
-    positions, radians = frozenset(_POSITION_CODES), ParamConstraint(dtypes=frozenset({torch.float64}), shape_rules=(ExactDims(1),))
-    halves = ParamConstraint(dtypes=frozenset({torch.bfloat16, torch.float16}))
     norm = dict(x=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=floats), shift=ParamConstraint(dtypes=floats))
     return {
         "quantize_per_tensor_fp8": fc(x=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=frozenset({torch.float32})),
@@ -899,15 +927,12 @@ def build_constraints() -> dict:
         "stochastic_rounding_fp8": fc(x=ParamConstraint(dtypes=floats), rng=ParamConstraint(dtypes=frozenset({torch.uint8}))),
         "qk_norm_rope": fc(qkv=ParamConstraint(dtypes=frozenset({torch.bfloat16, torch.float16})),
                            freqs_cis=ParamConstraint(dtypes=frozenset({torch.float32}))),
-        "add_rmsnorm_quantize_mxfp8": fc(x=ParamConstraint(dtypes=floats), residual=ParamConstraint(dtypes=floats),
-                                         weight=ParamConstraint(dtypes=floats)),
-        "add_rmsnorm_quantize_fp8": fc(x=ParamConstraint(dtypes=floats), residual=ParamConstraint(dtypes=floats),
-                                       weight=ParamConstraint(dtypes=floats), scale=ParamConstraint(dtypes=frozenset({torch.float32})),
-                                       output_type=ParamConstraint(dtypes=fp8)),
-        "apply_rope_axes": fc(xq=rope2.params["xq"], xk=rope2.params["xk"], positions=ParamConstraint(dtypes=positions), freqs=radians),
-        "apply_rope_axes1": fc(x=rope.params["x"], positions=ParamConstraint(dtypes=positions), freqs=radians),
-        "lora_add": fc(y=halves, x=halves, a=halves, b=halves, adapter_ids=ParamConstraint(dtypes=frozenset({torch.int32, torch.int64})),
-                       scales=ParamConstraint(dtypes=frozenset({torch.float32}))),
+        # (these check the rest of their arguments themselves, with messages that name the shapes)
+        "add_rmsnorm_quantize_mxfp8": fc(x=ParamConstraint(dtypes=floats), weight=ParamConstraint(dtypes=floats)),
+        "add_rmsnorm_quantize_fp8": fc(x=ParamConstraint(dtypes=floats), weight=ParamConstraint(dtypes=floats),
+                                       scale=ParamConstraint(dtypes=frozenset({torch.float32}))),
+        "apply_rope_axes": fc(xq=ParamConstraint(dtypes=floats)), "apply_rope_axes1": fc(x=ParamConstraint(dtypes=floats)),
+        "lora_add": fc(x=ParamConstraint(dtypes=frozenset({torch.bfloat16, torch.float16}))),
         "quantize_nvfp4_gather": fc(per_tensor_scale=ParamConstraint(dtypes=frozenset({torch.float32}))),
     }
 

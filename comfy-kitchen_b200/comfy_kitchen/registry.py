@@ -122,8 +122,16 @@ class BackendRegistry:
         return True
 
     def get_capable_backend(self, func_name: str, kwargs: Mapping[str, Any] | None = None) -> str:
-        failures: dict[str, str] = {}
         override = getattr(self._tls, "backend_override", None)
+        if override is None:   # the usual call: the first backend of the list that takes it, without keeping a record of why others do not
+            for name in self._priority:
+                if name in self._backends and name not in self._disabled and func_name in self._capabilities.get(name, ()):
+                    cons = self._constraints.get((name, func_name))
+                    if not kwargs or cons is None or validate_function_call(cons, kwargs, self._compute_capability).success:
+                        if logger.isEnabledFor(logging.DEBUG):
+                            logger.debug("Backend %s selected for %s", name, func_name)
+                        return name
+        failures: dict[str, str] = {}
         candidates = ([override] if override else []) + [n for n in self._priority if n != override]
         for name in candidates:
             if name != override and (not self.is_available(name) or func_name not in self._capabilities.get(name, ())):

@@ -194,7 +194,7 @@ int launch(RopeAxesParams p, bool split, bool vec, cudaStream_t stream) {
 extern "C" int launch_apply_rope_axes_kernel(const void* xq, const void* xk, const void* positions, const double* freqs,
                                              void* xq_out, void* xk_out, const int64_t* strides, int64_t batch, int64_t tokens,
                                              int64_t heads_q, int64_t heads_k, int64_t head_dim, const int32_t* axis_pairs,
-                                             int n_axes, int dtype_code, int positions_code, bool split_half, bool inverse,
+                                             int n_axes, int dtype_code, int positions_code, bool tokens_first, bool split_half, bool inverse,
                                              cudaStream_t stream) {
     using namespace ck;
     if (!xq || !positions || !freqs || !xq_out || !strides || !axis_pairs) CK_FAIL(CK_ERR_NULL, "apply_rope_axes: null pointer");
@@ -216,9 +216,15 @@ extern "C" int launch_apply_rope_axes_kernel(const void* xq, const void* xk, con
     }
     p.x[0] = xq; p.x[1] = xk; p.o[0] = xq_out; p.o[1] = xk_out;
     p.pos = positions; p.freqs = freqs;
-    // strides: q (batch, token, head, element), k (the same), q_out (batch, token, head), k_out, positions (batch, token, axis)
+    // strides: q (batch, token, head, element), k (the same), positions (batch, token, axis)
     for (int i = 0; i < 4; ++i) { p.sx[0][i] = strides[i]; p.sx[1][i] = strides[4 + i]; }
-    for (int i = 0; i < 3; ++i) { p.so[0][i] = strides[8 + i]; p.so[1][i] = strides[11 + i]; p.sp[i] = strides[14 + i]; }
+    for (int i = 0; i < 3; ++i) p.sp[i] = strides[8 + i];
+    const int64_t heads[2] = {heads_q, heads_k};
+    for (int w = 0; w < 2; ++w) {
+        p.so[w][0] = heads[w] * tokens * head_dim;
+        p.so[w][1] = tokens_first ? heads[w] * head_dim : head_dim;
+        p.so[w][2] = tokens_first ? head_dim : tokens * head_dim;
+    }
     p.batch = batch; p.tokens = tokens; p.heads[0] = (int)heads_q; p.heads[1] = (int)heads_k;
     p.D = (int)head_dim; p.P = (int)pairs; p.n_axes = n_axes; p.pos_type = positions_code;
     p.sign = inverse ? -1.0f : 1.0f;

@@ -171,14 +171,14 @@ int launch_apply_rope_kernel(const void* xq, const void* xk, const void* freqs, 
  * No counterpart in the reference (its apply_rope reads [.., head_dim/2, 2, 2] matrices; the formula is
  * backends/eager/rope.py:9-32 with F = [[cos, -sin], [sin, cos]]).  Pair p turns by position[axis(p)] * freqs[p] radians;
  * axis i owns the next axis_pairs[i] pairs (1 to 8 axes); elements behind the pairs are copied.  freqs: float64
- * [pairs].  positions_code: 0 float32, 1 float64, 2 int32, 3 int64.  strides (HOST array of 17, in elements): xq batch,
- * token, head, element; xk the same; xq_out batch, token, head; xk_out the same (outputs have unit element stride);
- * positions batch, token, axis.  xk / xk_out may both be NULL (heads_k = 0).  axis_pairs: HOST array.  inverse: rotate
- * back (the transpose, i.e. the gradient's rotation). */
+ * [pairs].  positions_code: 0 float32, 1 float64, 2 int32, 3 int64.  strides (HOST array of 11, in elements): xq batch,
+ * token, head, element; xk the same; positions batch, token, axis.  The outputs are contiguous: [batch, tokens, heads,
+ * head_dim] with tokens_first, else [batch, heads, tokens, head_dim].  xk / xk_out may both be NULL (heads_k = 0).
+ * axis_pairs: HOST array.  inverse: rotate back (the transpose, i.e. the gradient's rotation). */
 int launch_apply_rope_axes_kernel(const void* xq, const void* xk, const void* positions, const double* freqs, void* xq_out,
                                   void* xk_out, const int64_t* strides, int64_t batch, int64_t tokens, int64_t heads_q,
                                   int64_t heads_k, int64_t head_dim, const int32_t* axis_pairs, int n_axes, int dtype_code,
-                                  int positions_code, bool split_half, bool inverse, ck_stream_t stream);
+                                  int positions_code, bool tokens_first, bool split_half, bool inverse, ck_stream_t stream);
 
 /* Per-head RMSNorm of q and k + RoPE of both + relayout of q, k, v for attention, one pass.
  * No single counterpart in the reference: it composes apply_rope (backends/eager/rope.py:9-32)

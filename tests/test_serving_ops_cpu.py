@@ -135,11 +135,11 @@ def test_native_norm_refusals():
 
 
 def test_native_rope_refusals():
-    strides = (ctypes.c_int64 * 17)(*([8] * 17))
+    strides = (ctypes.c_int64 * 11)(*([8] * 11))
 
     def call(q=P, k=0, pos=P, f=P, oq=P, ok=0, st=strides, b=1, n=2, hq=1, hk=0, d=8, axes=(4,), count=None, t=2, pt=0):
         pairs = (ctypes.c_int32 * max(1, len(axes)))(*axes)
-        _refused("launch_apply_rope_axes_kernel", q, k, pos, f, oq, ok, st, b, n, hq, hk, d, pairs, len(axes) if count is None else count, t, pt, False, False, None)
+        _refused("launch_apply_rope_axes_kernel", q, k, pos, f, oq, ok, st, b, n, hq, hk, d, pairs, len(axes) if count is None else count, t, pt, False, False, False, None)
 
     for bad in (dict(q=0), dict(pos=0), dict(f=0), dict(oq=0), dict(k=P), dict(k=P, ok=P), dict(hk=1), dict(b=0), dict(n=0), dict(hq=0), dict(hq=70000), dict(d=7),
                 dict(axes=(5,)), dict(axes=(0,)), dict(axes=(2, 3)), dict(count=0), dict(axes=(1,) * 9, d=32), dict(t=5), dict(pt=4), dict(pt=-1), dict(b=1 << 20), dict(n=1 << 60, d=64)):
