@@ -7,8 +7,9 @@
 // Bound by HBM in either direction: x is read once, y read and out written once (2 K + 4 N bytes a row), each used adapter
 // once; the products' 2 R (K + N) flop a row stay below that up to a rank of about 128.  Two forms:
 //   few rows:   one CTA per row.
-//   many rows:  three kernels, the first and the last on the tensor cores (tcgen05):
-//               shrink:  low[t, :] = A x[t], equal shares of all tiles' K steps for every SM, partial sums in fp32;
+//   many rows:  four kernels, two of them on the tensor cores (tcgen05):
+//               count:   how many adapters each tile of rows asks for, by which the others share out their work;
+//               shrink:  low[t, :] = A x[t], equal shares of the tiles' K steps for every SM, partial sums in fp32;
 //               join:    the partial sums added in order (no atomics, the same bits every time) and laid out as the
 //                        next product's operand;
 //               expand:  out = y + scale * (B low), y tiles fetched and out tiles stored by TMA while the products run.
@@ -43,7 +44,11 @@ struct LoraArgs {
     void* out;
     uint8_t* image;         // many rows: per tile the low-rank vectors as the second product's operand (hi blocks, lo blocks)
     float* factor;          // [rows]: what a row's second product is multiplied by
-    float* partial;         // [parts, tiles of 256 rows, 256, R]
+    float* partial;         // [blocks, 256, R]: sums over a part of K for a tile of 256 rows
+    int* asked128;          // [tiles of 128 rows]: how many adapters a tile asks for
+    int* asked256;          // [tiles of 256 rows]
+    int* first_block;       // [tiles of 256 rows]: a tile's blocks in `partial`, first
+    int* last_block;        // and last
     int64_t rows, K, N, R, L;
     int64_t y_stride, x_stride, out_stride;
     int64_t rows_per_id;
@@ -165,7 +170,7 @@ __device__ __forceinline__ void tile_ids(const LoraArgs& p, int64_t row0, int la
 }
 
 // The different adapters among them, in the order of their first rows: calls each(place, id, first row, last row) with
-// every lane, leaves each row's place in `slot` (-1: none) and returns their number.  By a whole warp.
+// every lane, leaves each row's place in `slot` (-1: none; may be null) and returns their number.  By a whole warp.
 template <int kRows, typename Each>
 __device__ __forceinline__ int tile_adapters(const int (&id)[kRows / 32], int lane, int16_t* slot, Each each) {
     constexpr int kQ = kRows / 32;
@@ -193,9 +198,75 @@ __device__ __forceinline__ int tile_adapters(const int (&id)[kRows / 32], int la
         ++count;
     }
 #pragma unroll
-    for (int q = 0; q < kQ; ++q) slot[32 * q + lane] = (int16_t)place[q];
+    for (int q = 0; q < kQ; ++q)
+        if (slot) slot[32 * q + lane] = (int16_t)place[q];
     __syncwarp();
     return count;
+}
+
+// ---- shares: tiles ask for different numbers of adapters and cost accordingly, so a CTA's share is an equal run of weighted
+// steps, a tile's being `steps` steps of the weight that its number of adapters has (nought: the tile needs no work).
+
+struct Place { int tile, step, worked; };   // `worked`: how many tiles before have work
+
+// Where position `pos` of all tiles' weighted steps lies.  By a whole warp.
+template <typename Weight>
+__device__ __forceinline__ Place locate(const int* asked, int tiles, int steps, int64_t pos, int lane, Weight weight) {
+    int64_t before = 0;
+    int worked = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+        const int w = t0 + lane < tiles ? weight(__ldcg(asked + t0 + lane)) : 0;
+        int upto = w;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, w > 0 && pos < (before + upto) * steps);
+        const uint32_t work = __ballot_sync(0xffffffffu, w > 0);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const int wt = __shfl_sync(0xffffffffu, w, l);
+            const int64_t start = (before + __shfl_sync(0xffffffffu, upto, l) - wt) * steps;
+            return Place{t0 + l, (int)((pos - start) / wt), worked + __popc(work & ((1u << l) - 1))};
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+        worked += __popc(work);
+    }
+    return Place{tiles, 0, worked};   // (the end)
+}
+
+// All tiles' weight, and how many of them have work.  By a whole warp.
+template <typename Weight>
+__device__ __forceinline__ int64_t total_weight(const int* asked, int tiles, int lane, int& worked, Weight weight) {
+    int64_t sum = 0;
+    worked = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+        const int w = t0 + lane < tiles ? weight(__ldcg(asked + t0 + lane)) : 0;
+        worked += __popc(__ballot_sync(0xffffffffu, w > 0));
+        sum += w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+// One CTA per 256 rows: warps 0 and 1 count a half's adapters, warp 2 the whole tile's.
+__global__ void __launch_bounds__(96) lora_count_kernel(const LoraArgs p) {
+    tc::launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t tile = blockIdx.x;
+    int n;
+    if (warp < 2) {
+        int id[4];
+        tile_ids<128>(p, tile * 256 + warp * 128, lane, id);
+        n = tile_adapters<128>(id, lane, nullptr, [](int, int, int, int) {});
+    } else {
+        int id[8];
+        tile_ids<256>(p, tile * 256, lane, id);
+        n = tile_adapters<256>(id, lane, nullptr, [](int, int, int, int) {});
+    }
+    if (lane == 0) (warp < 2 ? p.asked128 + tile * 2 + warp : p.asked256 + tile)[0] = n;
 }
 
 template <typename T>
@@ -241,9 +312,7 @@ __device__ __forceinline__ void put_image(uint8_t* image, int blocks, int row, i
 struct ShrinkPlan {
     int k_tiles, halves;        // 64-element steps of K; 128-row tiles of A (2 for ranks over 128)
     int blocks;                 // 64-element blocks of R
-    int tiles, ctas;            // tiles of 256 rows; CTAs that share the tiles x k_tiles units,
-    int each, more;             // `each` units a CTA, and one more for the first `more` of them
-    int parts;                  // most CTAs that meet in one tile
+    int tiles, ctas;            // tiles of 256 rows; CTAs
     int x_stages, a_stages;     // rings of x and A tiles
     int smem;
 };
@@ -262,15 +331,13 @@ struct TileList {
     int count, unused;
 };
 
-// First unit (tile x K step) of a CTA's share, and the CTA whose share holds a unit.
-__device__ __forceinline__ int share(const ShrinkPlan& plan, int cta) { return plan.each * cta + min(cta, plan.more); }
-__device__ __forceinline__ int owner(const ShrinkPlan& plan, int unit) {
-    const int longer = plan.more * (plan.each + 1);
-    return unit < longer ? unit / (plan.each + 1) : plan.more + (unit - longer) / plan.each;
-}
+// A K step of a tile of c adapters takes about (3 + c) / 4 of the time of one of a single adapter's.  (The weight ends at 8,
+// twice the least one: with at least four steps a CTA on average, no share is then shorter than a step.)
+__device__ __forceinline__ int shrink_weight(int asked) { return asked == 0 ? 0 : 3 + min(asked, 5); }
 
-// low[t][:] = A_{ids[t]} x[t] as partial sums over parts of K: every CTA takes an equal run of (tile, K step) units, so that
-// all SMs are busy whatever the number of rows, and leaves one part for each tile that it meets.
+// low[t][:] = A_{ids[t]} x[t] as partial sums over parts of K: every CTA takes an equal run of the tiles' K steps, so that all
+// SMs are busy whatever the number of rows, and leaves a block of sums for each tile that it meets.  CTA c's block for
+// the n-th tile that has work is block c + n: of two neighbouring blocks either the CTA or the tile is another one.
 //
 // The product is taken as A x^T: an MMA of 128 rows costs 128 clocks whether it has 64 columns or 256, so the rank is its M
 // (what lies behind it in shared memory only fills accumulator rows that nobody reads) and 256 tokens its N; with the roles
@@ -299,13 +366,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* listed = drain + 1;                                             // [2] a tile's lists are there
     uint64_t* unlisted = listed + 2;                                          // [2] nobody needs them any more
     TileList* s_lists = reinterpret_cast<TileList*>(unlisted + 2);            // [2]
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_lists + 2);
+    Place* s_share = reinterpret_cast<Place*>(s_lists + 2);                   // this CTA's: from, to
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_share + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int unit0 = share(plan, blockIdx.x), unit1 = share(plan, blockIdx.x + 1);
-    const int tile0 = unit0 / plan.k_tiles, tile1 = (unit1 - 1) / plan.k_tiles;
-
     if (warp == 1) {
         tc::tmem_alloc(s_tmem, kShrinkColumns);
     } else if (threadIdx.x == 0) {
@@ -317,12 +382,24 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         for (int i = 0; i < 2; ++i) { tc::mbar_init(&listed[i], 1); tc::mbar_init(&unlisted[i], 10); }
         *s_abort = 0;
         tc::mbar_init_done();
+    } else if (warp == 2) {
+        tc::wait_for_dependency();      // the counts
+        int worked;
+        const int64_t all = total_weight(p.asked256, plan.tiles, lane, worked, shrink_weight) * plan.k_tiles;
+        const int sharing = min(plan.ctas, max(1, worked * plan.k_tiles / 4));   // (at least four steps a CTA)
+        const int cta = min((int)blockIdx.x, sharing);
+        const Place from = locate(p.asked256, plan.tiles, plan.k_tiles, all * cta / sharing, lane, shrink_weight);
+        const Place to = locate(p.asked256, plan.tiles, plan.k_tiles, all * min(cta + 1, sharing) / sharing, lane, shrink_weight);
+        if (lane == 0) { s_share[0] = from; s_share[1] = to; }
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     tc::launch_dependents();
     const uint32_t tmem = *s_tmem;
+    const Place from = s_share[0], to = s_share[1];
+    const bool idle = from.tile == to.tile && from.step == to.step;
+    const int tile0 = from.tile, tile1 = idle ? tile0 - 1 : to.step > 0 ? to.tile : to.tile - 1;   // (the last one that has steps of this share)
 
     if (warp == 10) {
         // lists, a tile ahead of the other warps
@@ -344,11 +421,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     }
     tc::Ring xr, ar;
     uint32_t xs = 0, as = 0, n = 0;     // tiles issued (warp 0); accumulator rounds
-    // x's first tiles are on their way before the ids are known (they are wanted unless nobody asks for an adapter)
+    // x's first tiles are on their way before the ids are listed
     int ahead = 0;
     if (warp == 0) {
-        const int k0 = unit0 - tile0 * plan.k_tiles, k1 = min(plan.k_tiles, unit1 - tile0 * plan.k_tiles);
-        for (; ahead < min(plan.x_stages, k1 - k0); ++ahead) {
+        const int k0 = from.step, k1 = tile0 == to.tile ? to.step : plan.k_tiles;
+        for (; ahead < min(plan.x_stages, k1 - k0) && tile0 <= tile1; ++ahead) {
             if (tc::elect_one()) {
                 tc::mbar_expect_tx(&x_full[ahead], kXBytes);
                 tc::tma_load_2d(s_x + ahead * kXBytes, &map_x, (k0 + ahead) * 64, tile0 * kShrinkRows, &x_full[ahead]);
@@ -357,9 +434,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         }
     }
     bool ok = true;
+    int block = (int)blockIdx.x + from.worked;
     for (int tile = tile0; tile <= tile1 && ok && warp < 10; ++tile) {
-        const int base = tile * plan.k_tiles, at = (tile - tile0) & 1;
-        const int k0 = max(0, unit0 - base), k1 = min(plan.k_tiles, unit1 - base);
+        const int at = (tile - tile0) & 1;
+        const int k0 = tile == tile0 ? from.step : 0, k1 = tile == to.tile ? to.step : plan.k_tiles;
         ok = tc::mbar_wait(&listed[at], (tile - tile0) >> 1 & 1, s_abort, &g_lora_status, kWaitList);
         const TileList& l = s_lists[at];
         const int count = ok ? l.count : 0;
@@ -399,14 +477,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     }
                 }
             }
-            // a first tile in which nobody asked for an adapter: its x tiles are taken out of the ring again
-            for (; ahead > 0 && ok; --ahead) {
-                ok = tc::mbar_wait(&x_full[xr.at], xr.round, s_abort, &g_lora_status, kWaitFull);
-                if (lane == 0) tc::mbar_arrive(&x_empty[xr.at]);
-                __syncwarp();
-                ++xs;
-                xr.next(plan.x_stages);
-            }
         } else if (warp == 1) {
             for (int first = 0, until; first < count && ok; first = until, ++n) {
                 until = batch_end(first);
@@ -437,12 +507,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                     }
                 }
             }
-            if (tile == tile0 && count == 0)   // (warp 0 takes the first tiles out)
-                for (int i = 0; i < min(plan.x_stages, k1 - k0); ++i) xr.next(plan.x_stages);
         } else {
             // a warp: 32 elements of the vector (its TMEM lanes) of every other 16 tokens
             const int quarter = warp & 3, half = (warp - 2) >> 2;
-            float* part = p.partial + ((int64_t)((int)blockIdx.x - owner(plan, base)) * plan.tiles + tile) * kShrinkRows * p.R;
+            float* part = p.partial + (int64_t)block * kShrinkRows * p.R;
+            if (threadIdx.x == 64 && count > 0) {
+                if (k0 == 0) p.first_block[tile] = block;
+                if (k1 == plan.k_tiles) p.last_block[tile] = block;
+            }
             const int R = (int)p.R;
             for (int first = 0, until; first < count && ok; first = until, ++n) {
                 until = batch_end(first);
@@ -481,6 +553,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 if (lane == 0) tc::mbar_arrive(acc_empty);
             }
         }
+        block += count > 0;
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&unlisted[at]);
     }
@@ -511,10 +584,9 @@ __global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs 
     const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 8) + (threadIdx.x >> 3);
     const int sub = threadIdx.x & 7;
     const int id = row < p.rows ? adapter_of(p, row) : -1;
-    const int base = (int)(row / kShrinkRows) * plan.k_tiles;
-    const int parts = owner(plan, base + plan.k_tiles - 1) - owner(plan, base) + 1;
     const float scale = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.0f;
     tc::wait_for_dependency();
+    const int tile = (int)(row / kShrinkRows), block0 = id >= 0 ? __ldcg(p.first_block + tile) : 0, block1 = id >= 0 ? __ldcg(p.last_block + tile) : -1;
     float v[kMaxRank / 64][8];
 #pragma unroll
     for (int u = 0; u < kMaxRank / 64; ++u) {
@@ -522,9 +594,9 @@ __global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
         if (id >= 0 && c < p.R) {
-            const float* src = p.partial + row * p.R + c;   // (row = tile * 256 + row in tile)
+            const float* src = p.partial + ((int64_t)block0 * kShrinkRows + row % kShrinkRows) * p.R + c;
 #pragma unroll 4
-            for (int k = 0; k < parts; ++k, src += (int64_t)plan.tiles * kShrinkRows * p.R) {
+            for (int k = block0; k <= block1; ++k, src += kShrinkRows * p.R) {
                 const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
                 v[u][0] += a.x; v[u][1] += a.y; v[u][2] += a.z; v[u][3] += a.w;
                 v[u][4] += b.x; v[u][5] += b.y; v[u][6] += b.z; v[u][7] += b.w;
@@ -552,7 +624,8 @@ __global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs 
 }
 
 struct ExpandPlan {
-    int64_t steps, items;       // column steps of a tile; tiles x steps
+    int steps, tiles;           // column steps of a tile; tiles of 128 rows
+    int k_steps;                // 16-element steps of R
     int blocks;                 // 64-element blocks of R
     int b_stages, y_stages;
     int smem;
@@ -589,11 +662,11 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     uint64_t* drain = low_done + 1;
     int* s_list = reinterpret_cast<int*>(drain + 1);                   // (warp 10's)
     int16_t* s_slots = reinterpret_cast<int16_t*>(s_list + kTile);
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slots + kExpandThreads / 32 * kTile);
+    Place* s_share = reinterpret_cast<Place*>(s_slots + kExpandThreads / 32 * kTile);   // this CTA's: from, to
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_share + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t first = plan.items * blockIdx.x / gridDim.x, last = plan.items * (blockIdx.x + 1) / gridDim.x;
     const bool in_place = p.out == p.y;
     int16_t* s_slot = s_slots + warp * kTile;                // a warp's own: the roles are at different tiles
 
@@ -608,14 +681,30 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::mbar_init_done();
     }
     if (warp == 1) tc::tmem_alloc(s_tmem, kExpandColumns);
+    if (warp == 3) {
+        // (The counts are there: this kernel can start only when every CTA of the two before it has, and the first of those
+        // waits for them.)  In units of 128 clocks: an item's share of HBM's time, its MMAs, what another adapter adds.
+        const int mmas = kU * plan.k_steps + 1;
+        auto weight = [&](int asked) { return asked == 0 ? (in_place ? 0 : 11 * kU) : max(11 * kU, asked * mmas) + 3 * min(asked - 1, 64); };
+        int worked;
+        const int64_t all = total_weight(p.asked128, plan.tiles, lane, worked, weight) * plan.steps;
+        const Place from = locate(p.asked128, plan.tiles, plan.steps, all * blockIdx.x / gridDim.x, lane, weight);
+        const Place to = locate(p.asked128, plan.tiles, plan.steps, all * (blockIdx.x + 1) / gridDim.x, lane, weight);
+        if (lane == 0) { s_share[0] = from; s_share[1] = to; }
+    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *s_tmem;
+    const Place from = s_share[0], to = s_share[1];
+    const bool idle = from.tile == to.tile && from.step == to.step;
+    const int tile1 = idle ? from.tile - 1 : to.step > 0 ? to.tile : to.tile - 1;   // the last tile that has steps of this share
+    auto begin_of = [&](int tile) { return tile == from.tile ? from.step : 0; };
+    auto end_of = [&](int tile) { return tile == to.tile ? to.step : plan.steps; };
 
     int id[kTile / 32];
-    auto tile_count = [&](int64_t tile) {
-        tile_ids<kTile>(p, tile * kTile, lane, id);
+    auto tile_count = [&](int tile) {
+        tile_ids<kTile>(p, (int64_t)tile * kTile, lane, id);
         return tile_adapters<kTile>(id, lane, s_slot, [](int, int, int, int) {});
     };
     // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles
@@ -623,16 +712,15 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::Ring yr;
         uint32_t issued = 0;
         bool ok = true;
-        for (int64_t item = first; item < last && ok;) {
-            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
-            item += end - begin;
+        for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
+            const int begin = begin_of(tile), end = end_of(tile);
             if (in_place && tile_count(tile) == 0) continue;
-            for (int unit = (int)begin * kU; unit < (int)end * kU; ++unit) {
+            for (int unit = begin * kU; unit < end * kU; ++unit) {
                 ok = tc::mbar_wait(&y_empty[yr.at], yr.round ^ 1u, s_abort, &g_lora_status, kWaitYFree);
                 if (!ok) break;
                 if (tc::elect_one()) {
                     tc::mbar_expect_tx(&y_full[yr.at], kTileBytes);
-                    tc::tma_load_2d(s_y + yr.at * kTileBytes, &map_y, unit * 64, (int)(tile * kTile), &y_full[yr.at]);
+                    tc::tma_load_2d(s_y + yr.at * kTileBytes, &map_y, unit * 64, tile * kTile, &y_full[yr.at]);
                 }
                 __syncwarp();
                 ++issued;
@@ -644,12 +732,11 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::Ring br;
         uint32_t issued = 0;
         bool ok = true;
-        for (int64_t item = first; item < last && ok;) {
-            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
-            item += end - begin;
-            tile_ids<kTile>(p, tile * kTile, lane, id);
+        for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
+            const int begin = begin_of(tile), end = end_of(tile);
+            tile_ids<kTile>(p, (int64_t)tile * kTile, lane, id);
             const int count = tile_adapters<kTile>(id, lane, s_slot, [&](int j, int which, int, int) { if (lane == 0) s_list[j] = which; });
-            for (int step = (int)begin; step < (int)end && ok; ++step)
+            for (int step = begin; step < end && ok; ++step)
                 for (int j = 0; j < count && ok; ++j) {
                     const int which = s_list[j];
                     for (int k = 0; k < plan.blocks; ++k) {
@@ -668,26 +755,25 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         if (!ok) tc::ring_drain(b_full, br, issued, plan.b_stages);
     } else if (warp == 1) {
         const uint32_t desc = tc::idesc(Elem<T>::code == CK_BF16, kStep);
-        const int k_steps = (int)ceil_div(p.R, 16);
+        const int k_steps = plan.k_steps;
         tc::Ring br;
         uint32_t n = 0, seg = 0;
         bool ok = true;
         tc::wait_for_dependency();      // the first kernel's image
-        for (int64_t item = first; item < last && ok;) {
-            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
-            item += end - begin;
+        for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
+            const int begin = begin_of(tile), end = end_of(tile);
             const int count = tile_count(tile);
             if (count == 0) continue;
             ok = tc::mbar_wait(low_done, (seg & 1) ^ 1, s_abort, &g_lora_status, kWaitAcc);   // nothing reads s_low any more
             if (!ok) break;
             if (tc::elect_one()) {
                 tc::mbar_expect_tx(low_full, low_bytes);
-                tc::bulk_load(s_low, p.image + tile * low_bytes, low_bytes, low_full);
+                tc::bulk_load(s_low, p.image + (int64_t)tile * low_bytes, low_bytes, low_full);
             }
             __syncwarp();
             ok = tc::mbar_wait(low_full, seg & 1, s_abort, &g_lora_status, kWaitLow);
             ++seg;
-            const int products = (int)(end - begin) * count;
+            const int products = (end - begin) * count;
             for (int i = 0; i < products && ok; ++i, ++n) {
                 const uint32_t buf = n & 1;
                 ok = tc::mbar_wait(&acc_empty[buf], (n >> 1 & 1) ^ 1, s_abort, &g_lora_status, kWaitAccFree);
@@ -726,15 +812,14 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::Ring yr;
         int before = -1;
         bool ok = true;
-        for (int64_t item = first; item < last && ok;) {
-            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
-            item += end - begin;
+        for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
+            const int begin = begin_of(tile), end = end_of(tile);
             if (in_place && tile_count(tile) == 0) continue;
-            for (int unit = (int)begin * kU; unit < (int)end * kU; ++unit, yr.next(plan.y_stages)) {
+            for (int unit = begin * kU; unit < end * kU; ++unit, yr.next(plan.y_stages)) {
                 ok = tc::mbar_wait(&y_done[yr.at], yr.round, s_abort, &g_lora_status, kWaitDone);
                 if (!ok) break;
                 if (lane == 0) {
-                    tc::tma_store_2d(&map_out, s_y + yr.at * kTileBytes, unit * 64, (int)(tile * kTile));
+                    tc::tma_store_2d(&map_out, s_y + yr.at * kTileBytes, unit * 64, tile * kTile);
                     tc::tma_store_commit();
                     tc::tma_store_wait_read<1>();
                     if (before >= 0) tc::mbar_arrive(&y_empty[before]);
@@ -754,14 +839,13 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         uint32_t odd = 0;               // the parity of the step's first unit: which group takes it
         bool ok = true;
         tc::wait_for_dependency();      // the first kernel's factors
-        for (int64_t item = first; item < last && ok;) {
-            const int64_t tile = item / plan.steps, begin = item - tile * plan.steps, end = min(plan.steps, begin + last - item);
-            item += end - begin;
+        for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
+            const int begin = begin_of(tile), end = end_of(tile);
             const int count = tile_count(tile);
             if (count == 0 && in_place) continue;
             const int mine = s_slot[r_in_tile];
-            const float factor = mine >= 0 ? __ldcg(p.factor + tile * kTile + r_in_tile) : 0.0f;
-            for (int step = (int)begin; step < (int)end && ok; ++step) {
+            const float factor = mine >= 0 ? __ldcg(p.factor + (int64_t)tile * kTile + r_in_tile) : 0.0f;
+            for (int step = begin; step < end && ok; ++step) {
                 for (int j = 0; j < count && ok; ++j, ++n) {
                     const uint32_t buf = n & 1;
                     ok = tc::mbar_wait(&acc_full[buf], n >> 1 & 1, s_abort, &g_lora_status, kWaitAcc);
@@ -856,13 +940,9 @@ ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R) {
     s.halves = R > kTile ? 2 : 1;
     s.blocks = (int)ceil_div(R, 64);
     s.tiles = (int)ceil_div(rows, kShrinkRows);
-    const int units = s.tiles * s.k_tiles, most = (int)ceil_div(units, 4);   // at least four steps of K for a CTA
-    s.ctas = most < sm_count() ? most : sm_count();
-    s.each = units / s.ctas;
-    s.more = units % s.ctas;
-    s.parts = (int)ceil_div(s.k_tiles - 1, s.each) + 1;      // a run of k_tiles units touches at most this many shares
-    if (s.parts > s.ctas) s.parts = s.ctas;
-    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + 2 * (int)sizeof(TileList) + 16;
+    const int64_t most = ceil_div((int64_t)s.tiles * s.k_tiles, 4);   // at least four steps of K for a CTA
+    s.ctas = (int)(most < sm_count() ? most : sm_count());
+    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + 2 * (int)(sizeof(TileList) + sizeof(Place)) + 16;
     s.x_stages = (kSmemMost - rest - a_bytes) / (kXBytes + a_bytes);
     s.a_stages = s.x_stages + 1;
     s.smem = rest + s.x_stages * kXBytes + s.a_stages * a_bytes;
@@ -871,13 +951,14 @@ ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R) {
 
 // Where the parts of the workspace lie.
 struct Workspace {
-    int64_t factor, partial, bytes;   // (the image is at 0)
+    int64_t factor, partial, tables, bytes;   // (the image is at 0)
 };
 Workspace workspace_of(const ShrinkPlan& s, int64_t rows, int64_t R) {
     Workspace w{};
     w.factor = (int64_t)s.tiles * (kShrinkRows / kTile) * 2 * s.blocks * kTileBytes;
     w.partial = w.factor + round_up(rows * 4, 128);
-    w.bytes = w.partial + (int64_t)s.parts * s.tiles * kShrinkRows * R * 4;
+    w.tables = w.partial + (int64_t)(s.ctas + s.tiles) * kShrinkRows * R * 4;
+    w.bytes = w.tables + (int64_t)s.tiles * 5 * 4;
     return w;
 }
 
@@ -907,10 +988,12 @@ template <typename T, int kU>
 int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     constexpr int kStep = kU * 64, b_bytes = kStep * 128;
     ExpandPlan e{};
-    e.steps = ceil_div(p.N, kStep);
-    e.items = e.steps * ceil_div(p.rows, kTile);
+    e.steps = (int)ceil_div(p.N, kStep);
+    e.tiles = (int)ceil_div(p.rows, kTile);
+    e.k_steps = (int)ceil_div(p.R, 16);
+    const int64_t items = (int64_t)e.steps * e.tiles;
     e.blocks = (int)ceil_div(p.R, 64);
-    const int rest = 1024 + 48 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 16;
+    const int rest = 1024 + 48 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 2 * (int)sizeof(Place) + 16;
     // The image, a stage of B and four units of y (their number is even, so that a stage always serves
     // the same group of epilogue warps; a group that waited for a stage whose last load it had not seen might mistake that
     // one's end for its own); then y and B in turn.
@@ -935,7 +1018,7 @@ int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     auto kernel = lora_expand_kernel<T, kU>;
     const int rc = opt_in(kernel, kU + (Elem<T>::code == CK_BF16 ? 0 : 4) - 1);
     if (rc != CK_OK) return rc;
-    Launch l((unsigned)(e.items < sm_count() ? e.items : sm_count()), kExpandThreads, e.smem, stream, true);
+    Launch l((unsigned)(items < sm_count() ? items : sm_count()), kExpandThreads, e.smem, stream, true);
     return launched(cudaLaunchKernelEx(&l.cfg, kernel, map_b, map_y, map_out, p, e), "expand");
 }
 
@@ -946,6 +1029,10 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
     p.image = workspace;
     p.factor = reinterpret_cast<float*>(workspace + w.factor);
     p.partial = reinterpret_cast<float*>(workspace + w.partial);
+    p.asked128 = reinterpret_cast<int*>(workspace + w.tables);
+    p.asked256 = p.asked128 + 2 * s.tiles;
+    p.first_block = p.asked256 + s.tiles;
+    p.last_block = p.first_block + s.tiles;
     CUtensorMap map_x, map_a;
     const int64_t xd[2] = {p.K, p.rows}, xs[1] = {p.x_stride * 2};
     const int64_t ad[3] = {p.K, p.R, p.L}, as[2] = {p.K * 2, p.R * p.K * 2};
@@ -953,7 +1040,10 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
         CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: a tensor map could not be encoded");
     int rc = opt_in(lora_shrink_kernel<T>, Elem<T>::code == CK_BF16);
     if (rc != CK_OK) return rc;
-    Launch shrink((unsigned)s.ctas, kShrinkThreads, s.smem, stream, false);
+    Launch count((unsigned)s.tiles, 96, 0, stream, false);
+    rc = launched(cudaLaunchKernelEx(&count.cfg, lora_count_kernel, p), "count");
+    if (rc != CK_OK) return rc;
+    Launch shrink((unsigned)s.ctas, kShrinkThreads, s.smem, stream, true);
     rc = launched(cudaLaunchKernelEx(&shrink.cfg, lora_shrink_kernel<T>, map_x, map_a, p, s), "shrink");
     if (rc != CK_OK) return rc;
     Launch join((unsigned)ceil_div(p.rows, kJoinThreads / 8), kJoinThreads, 0, stream, true);
@@ -1001,7 +1091,7 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
-    const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
+    const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
     if (few_rows(rows)) {
         const dim3 grid(kFewCluster, (unsigned)rows);
         if (dtype_code == CK_BF16) lora_few_kernel<__nv_bfloat16><<<grid, kFewThreads, 0, stream>>>(p);

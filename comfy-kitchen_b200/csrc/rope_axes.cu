@@ -17,6 +17,7 @@ namespace ck {
 namespace {
 
 constexpr int kMaxAxes = 8;
+constexpr int kThreads = 128;
 enum PosType { kPosF32 = 0, kPosF64 = 1, kPosI32 = 2, kPosI64 = 3 };
 
 struct RopeAxesParams {
@@ -73,7 +74,7 @@ __device__ __forceinline__ void head_at(const RopeAxesParams& p, int64_t b, int6
 
 // Vectors of 8 elements: unit stride, D (and, split-half, P) a multiple of 8, 16-byte aligned rows.
 template <typename T, bool kSplit>
-__global__ void __launch_bounds__(256) rope_axes_vec_kernel(const RopeAxesParams p) {
+__global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const RopeAxesParams p) {
     constexpr int kPairs = kSplit ? 8 : 4;
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t site = item / p.n_vec;
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(256) rope_axes_vec_kernel(const RopeAxesParams
 
 // Any strides, any even D: one pair per thread and head; a thread behind the pairs copies two elements.
 template <typename T>
-__global__ void __launch_bounds__(256) rope_axes_generic_kernel(const RopeAxesParams p, const bool split) {
+__global__ void __launch_bounds__(kThreads) rope_axes_generic_kernel(const RopeAxesParams p, const bool split) {
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t site = item / p.n_vec;
     const int pair = (int)(item - site * p.n_vec);
@@ -171,20 +172,23 @@ template <typename T>
 int launch(RopeAxesParams p, bool split, bool vec, cudaStream_t stream) {
     p.n_vec = vec ? (split ? p.P / 8 + (int)ceil_div(p.D - 2 * p.P, 16) : p.D / 8) : p.D / 2;
     const int heads = p.heads[0] + p.heads[1];
-    // Heads are split over threads until the machine is full (about 1024 threads an SM), but not below 4 a thread.
+    // A thread walks at most 16 heads: enough to make the sines cheap, few enough for the last CTAs to end together
+    // (25037 tokens x 80 heads: 159 us; 80 heads a thread 177, 10 heads 173), and fewer while an SM has less than 768
+    // threads (3 x 1377 x 25: 16.9 us with 5 heads a thread, 22.2 with all; one token: 4.1 us with one, 4.9 with four).
     const int64_t sites = p.batch * p.tokens * p.n_vec;
-    int64_t chunks = ceil_div(148LL * 1024, sites);
-    if (chunks > ceil_div(heads, 4)) chunks = ceil_div(heads, 4);
+    int64_t chunks = ceil_div(148LL * 768, sites);
+    if (chunks > heads) chunks = heads;
+    if (chunks < ceil_div(heads, 16)) chunks = ceil_div(heads, 16);
     if (chunks > 65535 / p.batch) chunks = 65535 / p.batch;   // (batch x chunks is a grid dimension)
     if (chunks < 1) chunks = 1;
     p.chunk = (int)ceil_div(heads, chunks);
     p.n_chunks = (int)ceil_div(heads, p.chunk);
-    const int64_t gx = ceil_div(p.tokens * p.n_vec, 256), gy = p.batch * p.n_chunks;
+    const int64_t gx = ceil_div(p.tokens * p.n_vec, kThreads), gy = p.batch * p.n_chunks;
     if (gx > 0x7fffffff) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: %lld tokens are more than a grid holds", (long long)p.tokens);
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (!vec) rope_axes_generic_kernel<T><<<grid, 256, 0, stream>>>(p, split);
-    else if (split) rope_axes_vec_kernel<T, true><<<grid, 256, 0, stream>>>(p);
-    else rope_axes_vec_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    if (!vec) rope_axes_generic_kernel<T><<<grid, kThreads, 0, stream>>>(p, split);
+    else if (split) rope_axes_vec_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
+    else rope_axes_vec_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
     return launch_status("apply_rope_axes");
 }
 
