@@ -359,11 +359,11 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     uint8_t* stage_base = smem;
     uint8_t* s_out = smem + kStages * kStageBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + kSmemOut);
-    uint64_t* full = bars;                    // [kStages]  this CTA's TMA copies landed -> its scale movers
-    uint64_t* empty = bars + kStages;         // [kStages]  movers have read the scales + the pair's MMAs of the k-tile are
+    uint64_t* full = bars;                    // [2 kStages] this CTA's TMA copies landed -> its scale movers (kCp: both CTAs' -> MMA issuers)
+    uint64_t* empty = bars + 2 * kStages;     // [kStages]  movers have read the scales + the pair's MMAs of the k-tile are
                                               //            done -> TMA producer (stage free), movers (scale buffer free)
-    uint64_t* sf_full = empty + kStages;      // [kSfBufs]  (leader's) both CTAs' scales in TMEM -> MMA issuer
-    uint64_t* tmem_full = sf_full + kSfBufs;  //            accumulator complete -> epilogue
+    uint64_t* sf_full = empty + kStages;      // [2 kSfBufs] (leader's) both CTAs' scales in TMEM -> MMA issuer
+    uint64_t* tmem_full = sf_full + 2 * kSfBufs;  //            accumulator complete -> epilogue
     uint64_t* tmem_empty = tmem_full + 1;     //            (leader's) both CTAs' accumulators copied out -> MMA issuer
     uint64_t* tile_open = tmem_empty + 1;     //            first MMA of a tile issued -> the second MMA issuer
     uint64_t* drain = tile_open + 1;          // [2]        an MMA issuer that gave up: its MMAs in flight are done
@@ -378,10 +378,16 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     constexpr int kSfTilesPerStage = kFp4 ? 4 : 1;        // 512-byte tiles per 128 rows per k-tile
     const int k_tiles = (p.K + kElemsPerTile - 1) / kElemsPerTile;
     const int num_tiles = p.tiles_m * p.tiles_n;
+    // The MMA issuers take every other k-tile each, so what they wait on has two barriers per stage (or scale buffer), used
+    // in turn: k-tile `it` signals barrier it % (2 n), and a barrier always has the same issuer.  With one barrier per stage
+    // and an odd number of stages an issuer saw only every other phase, of equal parity, and took the phase before, when
+    // that k-tile's copies landed late and out of order, for its own (one launch of 4608 x 9216 x 3072 in about 2000).
+    constexpr int kFulls = kCp ? 2 * kStages : kStages, kSfFulls = 2 * kSfBufs;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], kCp ? 2 : 1); mbar_init(&empty[s], kCp ? 1 : 5); }
-        for (int b = 0; b < kSfBufs; ++b) mbar_init(&sf_full[b], 8);
+        for (int s = 0; s < 2 * kStages; ++s) mbar_init(&full[s], kCp ? 2 : 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&empty[s], kCp ? 1 : 5);
+        for (int b = 0; b < 2 * kSfBufs; ++b) mbar_init(&sf_full[b], 8);
         mbar_init(tmem_full, 2);   // one commit per tile from each MMA issuer
         mbar_init(tile_open, 1);
         mbar_init(&drain[0], 1);
@@ -429,7 +435,7 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
                 if constexpr (kCp) {
                     // every box is transferred whole (zero-filled outside the tensor): a fixed byte count per stage
                     constexpr uint32_t kSfBox = kSfTilesPerStage * 512u;
-                    const uint32_t lead_full = cluster_addr(&full[s], 0);
+                    const uint32_t lead_full = cluster_addr(&full[it % kFulls], 0);
                     if (elect_one()) {
                         mbar_expect_tx_cluster(lead_full, kSmemA + kSmemB + 3u * kSfBox);
                         tma_load_2d_pair(st, &map_a, kt * 128, tm * 256 + (int)rank * BM, lead_full);
@@ -457,8 +463,7 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         if (kCp && !ok) __nanosleep(50000);
         const uint32_t first = it > (uint32_t)kStages ? it - kStages : 0;
         for (uint32_t j = (kCp && rank != 0) ? it : first; j < it; ++j) {
-            const int s = j % kStages;
-            (void)mbar_wait(&full[s], (j / kStages) & 1, s_abort, kTimeoutFull);
+            (void)mbar_wait(&full[j % kFulls], (j / kFulls) & 1, s_abort, kTimeoutFull);
         }
     } else if (kCp && warp >= kFirstMoverWarp && warp < kSecondMmaWarp) {
         // (these warps have no work in this variant)
@@ -516,16 +521,16 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(&sf_full[b], 0);   // the leader's barrier
+                if (lane == 0) mbar_arrive_cluster(&sf_full[it % kSfFulls], 0);   // the leader's barrier
             }
         }
     } else if (warp == 1 || warp == kSecondMmaWarp) {
         // ------------------------------------------------------------ MMA issuers (leader CTA only)
         // Issuing one block-scaled MMA keeps a thread ~100 clocks and the bookkeeping of a k-tile (barrier
         // look-ahead, commit) another ~150, while the tensor cores need 128 clocks per MMA: a single issuer
-        // cannot keep them fed.  Two warps therefore take the k-tiles in turn (warp 1 the even ones).  The
+        // cannot keep them fed.  Two warps therefore take the k-tiles in turn (of all tiles: warp 1 the even ones).  The
         // accumulation order does not matter except for the first MMA of a tile, which overwrites: the second
-        // issuer waits (tile_open) until the first has issued it.  A commit covers the committing thread's own
+        // issuer of a tile waits (tile_open) until the first has issued it.  A commit covers the committing thread's own
         // MMAs, so each issuer releases the stages it consumed and both commit to tmem_full.
         const uint32_t which = warp == 1 ? 0u : 1u;
         if (rank == 0) {
@@ -541,20 +546,21 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
             if (!ok) break;
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + kTmemAcc;
-            if (which == 1 && k_tiles > 1) {   // the overwriting MMA must be in the pipe before any of mine
+            const uint32_t opener = it & 1u;
+            if (which != opener && k_tiles > 1) {   // the overwriting MMA must be in the pipe before any of mine
                 ok = mbar_wait(tile_open, local_tile & 1, s_abort, kTimeoutTmemEmpty);
                 if (!ok) break;
             }
             for (int kt = 0; kt < k_tiles && ok; ++kt, ++it) {
-                if ((uint32_t)(kt & 1) != which) continue;
+                if ((it & 1u) != which) continue;
                 const int s = it % kStages;
                 const uint32_t sb = kCp ? (uint32_t)s : it % kSfBufs;
                 // The movers of both CTAs publish sf_full only after they saw their full[s], so this one wait
                 // covers the operands too.  `ready` is an early look taken while the previous k-tile was issued.
                 // (kCp: full[s] here in the leader collects the copies of both CTAs.)
                 if (!__all_sync(0xffffffffu, ready))
-                    ok = kCp ? mbar_wait(&full[s], (it / kStages) & 1, s_abort, kTimeoutFull)
-                             : mbar_wait(&sf_full[sb], (it / kSfBufs) & 1, s_abort, kTimeoutSfFull);
+                    ok = kCp ? mbar_wait(&full[it % kFulls], (it / kFulls) & 1, s_abort, kTimeoutFull)
+                             : mbar_wait(&sf_full[it % kSfFulls], (it / kSfFulls) & 1, s_abort, kTimeoutSfFull);
                 if (!ok) break;
                 tc_fence_after();
                 // every descriptor of this stage is "stage start >> 4" plus a constant (the same in both CTAs)
@@ -582,12 +588,12 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
                         if (kFp4) { sfa += 4 * kb; sfb += 8 * kb; }
                         else { idesc |= ((uint32_t)kb << 29) | ((uint32_t)kb << 4); }
                         tc_mma<kFp4>(d_tmem, a_lo + 2 * kb, b_lo + 2 * kb, idesc, (kt > 0 || kb > 0) ? 1u : 0u, sfa, sfb);
-                        if (kt == 0 && kb == 0 && lane == 0) mbar_arrive(tile_open);   // which == 0 here
+                        if (kt == 0 && kb == 0 && lane == 0) mbar_arrive(tile_open);   // which == opener here
                     }
                     // the pipe is busy with these for a while: look at my next k-tile's barrier now
                     if (kb == 1) ready = kt + 2 < k_tiles &&
-                                         (kCp ? mbar_test_wait(&full[(it + 2) % kStages], ((it + 2) / kStages) & 1)
-                                              : mbar_test_wait(&sf_full[(it + 2) % kSfBufs], ((it + 2) / kSfBufs) & 1));
+                                         (kCp ? mbar_test_wait(&full[(it + 2) % kFulls], ((it + 2) / kFulls) & 1)
+                                              : mbar_test_wait(&sf_full[(it + 2) % kSfFulls], ((it + 2) / kSfFulls) & 1));
                 }
                 tc_commit_pair(&empty[s]);                      // stage and scale buffer reusable once these MMAs are done
             }
