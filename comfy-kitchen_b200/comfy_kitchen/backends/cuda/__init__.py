@@ -846,6 +846,9 @@ def lora_add(
     rows = x.numel() // k
     if rows == 0:
         return out
+    if device.index is not None and device.index != torch.cuda.current_device():   # (the scratch's size goes by the device)
+        with torch.cuda.device(device):
+            return lora_add(y, x, a, b, adapter_ids, scales, out)
     # the kernels move 16 bytes at a time
     xf, yf, of = _rows_of(x, k), _rows_of(y, n), _rows_of(out, n)
     x_stride, y_stride, o_stride = _row_stride(xf, k), _row_stride(yf, n), _row_stride(of, n)
@@ -868,7 +871,7 @@ def lora_add(
     if scales is not None and not scales.is_contiguous():
         scales = scales.contiguous()
     # scratch of the tiled kernels; the allocator's, so that streams and captured graphs keep theirs apart
-    need = _native.load().ck_lora_workspace_bytes(rows, k, rank, adapters) if rows > 1 else 0
+    need = _native.load().ck_lora_workspace_bytes(rows, k, n, rank) if rows > 1 else 0
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch(device, "launch_lora_add_kernel", py, px, pa, pb, ids.data_ptr(), 0 if scales is None else scales.data_ptr(), po,
             0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, y_stride, x_stride, o_stride, rows // ids.numel(),

@@ -683,9 +683,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     if (warp == 1) tc::tmem_alloc(s_tmem, kExpandColumns);
     if (warp == 3) {
         // (The counts are there: this kernel can start only when every CTA of the two before it has, and the first of those
-        // waits for them.)  In units of 128 clocks: an item's share of HBM's time, its MMAs, what another adapter adds.
+        // waits for them.)  In units of 128 clocks: an item's share of HBM's time, half as much again for each further adapter
+        // (ranks 64 and 128), or the MMAs of a high rank.
         const int mmas = kU * plan.k_steps + 1;
-        auto weight = [&](int asked) { return asked == 0 ? (in_place ? 0 : 11 * kU) : max(11 * kU, asked * mmas) + 3 * min(asked - 1, 64); };
+        auto weight = [&](int asked) { return asked == 0 ? (in_place ? 0 : 11 * kU) : max(11 * kU * (asked + 1) / 2, asked * mmas); };
         int worked;
         const int64_t all = total_weight(p.asked128, plan.tiles, lane, worked, weight) * plan.steps;
         const Place from = locate(p.asked128, plan.tiles, plan.steps, all * blockIdx.x / gridDim.x, lane, weight);
@@ -917,10 +918,15 @@ int sm_count() {
     return cached[dev];
 }
 
-#ifndef CK_LORA_FEW
-#define CK_LORA_FEW 64
-#endif
-bool few_rows(int64_t rows) { return rows <= CK_LORA_FEW; }
+// Whether a call takes the kernel with a cluster per row.  Its time goes with rows x rank x (K + N), the adapters' elements
+// that it reads from L2 (32 us at 67 M elements), that of the tiled kernels with the number of adapters that meet in a tile,
+// which only the device knows: 64 rows of 16 adapters, rank 32, 4096 -> 14336: 17 us against 67 (one adapter: 22); 128
+// rows 32 against 80 (24); 512 rows, rank 16, 4096 -> 4096: 36 against 99 (26).
+bool few_rows(int64_t rows, int64_t K, int64_t N, int64_t R) { return rows <= 512 && rows * R * (K + N) <= 80000000; }
+
+// What keeps tile coordinates, grids and the number of K steps within 32 bits.
+constexpr int64_t kMostRows = 1 << 27, kMostColumns = 1 << 24;
+bool units_fit(int64_t rows, int64_t K) { return ceil_div(rows, kShrinkRows) * ceil_div(K, 64) <= 0x3fffffff; }
 
 template <typename K>
 int opt_in(K kernel, int which) {   // dynamic shared memory beyond 48 KB, once per kernel and device
@@ -1055,10 +1061,10 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
 }  // namespace
 }  // namespace ck
 
-extern "C" int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t rank, int64_t adapters) {
+extern "C" int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t rank) {
     using namespace ck;
-    if (rows <= 0 || rows > (1 << 27) || K <= 0 || K > (1 << 24) || rank <= 0 || adapters <= 0 || few_rows(rows)) return 0;
-    if (ceil_div(rows, kShrinkRows) * ceil_div(K, 64) > 0x3fffffff) return 0;   // (refused)
+    if (rows <= 0 || rows > kMostRows || K <= 0 || K > kMostColumns || N <= 0 || N > kMostColumns || rank <= 0 || rank > kMaxRank) return 0;   // (refused)
+    if (few_rows(rows, K, N, rank) || !units_fit(rows, K)) return 0;
     return workspace_of(shrink_plan(rows, K, rank), rows, rank).bytes;
 }
 
@@ -1081,18 +1087,17 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     using namespace ck;
     if (!y || !x || !a || !b || !ids || !out) CK_FAIL(CK_ERR_NULL, "lora_add: null pointer");
     if (dtype_code != CK_F16 && dtype_code != CK_BF16) CK_FAIL(CK_ERR_DTYPE, "lora_add: dtype code %d (bf16 or fp16)", dtype_code);
-    // (tiles are addressed with 32-bit coordinates; 2^27 rows keep the grid of the first product within its bounds)
-    if (rows <= 0 || rows > (1 << 27) || K <= 0 || K > (1 << 24) || N <= 0 || N > (1 << 24) || adapters <= 0 || adapters > 0x7fffffff ||
+    if (rows <= 0 || rows > kMostRows || K <= 0 || K > kMostColumns || N <= 0 || N > kMostColumns || adapters <= 0 || adapters > 0x7fffffff ||
         K % 8 != 0 || N % 8 != 0 || rows_per_id <= 0 || x_row_stride < K || y_row_stride < N || out_row_stride < N)
         CK_FAIL(CK_ERR_SHAPE, "lora_add: bad shape rows=%lld K=%lld N=%lld adapters=%lld (K and N multiples of 8)", (long long)rows,
                 (long long)K, (long long)N, (long long)adapters);
-    if (ceil_div(rows, kShrinkRows) * ceil_div(K, 64) > 0x3fffffff)
+    if (!units_fit(rows, K))
         CK_FAIL(CK_ERR_SHAPE, "lora_add: %lld rows of %lld are too many", (long long)rows, (long long)K);
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
     const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
-    if (few_rows(rows)) {
+    if (few_rows(rows, K, N, rank)) {
         const dim3 grid(kFewCluster, (unsigned)rows);
         if (dtype_code == CK_BF16) lora_few_kernel<__nv_bfloat16><<<grid, kFewThreads, 0, stream>>>(p);
         else lora_few_kernel<__half><<<grid, kFewThreads, 0, stream>>>(p);

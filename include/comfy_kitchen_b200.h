@@ -245,13 +245,13 @@ int ck_norm_device_status(void);
  * [0, adapters).  y: [rows, N], the shared projection's output; x: [rows, K]; a: [adapters, rank, K]; b: [adapters, N, rank];
  * all bf16 or all fp16, 16-byte aligned, row strides (elements) multiples of 8; ids: int32 or int64; scales: fp32
  * [adapters] or NULL (ones); out may be y.  K, N, rank multiples of 8, rank at most 256.  workspace: scratch of
- * ck_lora_workspace_bytes(), 16-byte aligned, used by this call only until it ends on the stream. */
+ * ck_lora_workspace_bytes(), 16-byte aligned, used by this call only until it ends on the stream (need not be set). */
 int launch_lora_add_kernel(const void* y, const void* x, const void* a, const void* b, const void* ids, const float* scales,
                            void* out, void* workspace, int64_t rows, int64_t K, int64_t N, int64_t rank, int64_t adapters,
                            int64_t y_row_stride, int64_t x_row_stride, int64_t out_row_stride, int64_t rows_per_id, int dtype_code,
                            bool ids_64bit, ck_stream_t stream);
 /* Bytes of device memory that a call of this shape needs as workspace (0: none; depends on the current device's SM count). */
-int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t rank, int64_t adapters);
+int64_t ck_lora_workspace_bytes(int64_t rows, int64_t K, int64_t N, int64_t rank);
 /* Synchronises the device, reads and clears the adapter kernels' status word: 0, or CK_ERR_DEVICE_TIMEOUT when a bounded
  * device-side wait ran out since the last call. */
 int ck_lora_device_status(void);

@@ -322,7 +322,8 @@ LORAS = [
     (31, 200, 136, 8, 2, "runs"), (33, 1024, 512, 64, 4, "mixed"), (64, 2048, 1032, 32, 20, "mixed"), (65, 264, 520, 128, 3, "runs"), (127, 320, 64, 16, 300, "mixed"),
     (128, 640, 256, 256, 2, "mixed"), (129, 1032, 392, 72, 7, "runs"), (300, 4096, 24, 64, 40, "mixed"), (511, 136, 2056, 16, 3, "runs"),
     (1000, 768, 776, 200, 6, "runs"), (2049, 256, 512, 64, 9, "runs"), (4100, 512, 1544, 32, 4, "runs"),
-    (9473, 200, 136, 72, 9, "mixed"), (9728, 1032, 264, 128, 5, "runs"), (19200, 520, 72, 16, 3, "runs"),
+    (513, 64, 64, 256, 2, "mixed"), (600, 264, 136, 24, 40, "mixed"), (777, 1032, 520, 200, 9, "mixed"), (1025, 8, 8, 8, 3, "mixed"), (2000, 72, 4104, 48, 300, "mixed"),
+    (400, 4096, 4096, 128, 3, "runs"), (40, 8192, 8192, 256, 5, "mixed"), (9473, 200, 136, 72, 9, "mixed"), (9728, 1032, 264, 128, 5, "runs"), (19200, 520, 72, 16, 3, "runs"),
 ]
 
 
@@ -339,7 +340,7 @@ def test_lora(ck, case, dtype):
     assert ck.lora_add(own, x, a, b, ids, scales, out=own) is own and torch.equal(own, got)
 
 
-@pytest.mark.parametrize("rows,n,rank", [(3, 96, 16), (40, 96, 16), (200, 96, 16), (300, 4104, 256), (16500, 520, 128), (20000, 264, 64)])
+@pytest.mark.parametrize("rows,n,rank", [(3, 96, 16), (40, 96, 16), (700, 96, 16), (600, 4104, 256), (16500, 520, 128), (20000, 264, 64)])
 def test_lora_nothing_to_add(ck, rows, n, rank):
     x, y, a, b, _, scales = _lora_case(rows, 512, n, rank, 4, BF16, 8, "one")
     for value in (-1, 4, -2 ** 31, 2 ** 31 - 1):
@@ -366,7 +367,7 @@ def test_lora_some_tiles_without_adapters(ck, rows, rank):
     assert cuda.lora_device_status() == 0
 
 
-@pytest.mark.parametrize("rows", [5, 70, 300])
+@pytest.mark.parametrize("rows", [5, 70, 900])
 def test_lora_keeps_infinities_in_their_rows(ck, rows):
     x, y, a, b, ids, scales = _lora_case(rows, 264, 136, 24, 4, BF16, 9, "mixed")
     clean = ck.lora_add(y, x, a, b, ids, scales)
@@ -387,7 +388,7 @@ def test_lora_keeps_infinities_in_their_rows(ck, rows):
 def test_lora_large_low_rank_values(ck):
     """A first product beyond fp16's range is no infinity, and a tiny one does not vanish."""
     g = _gen(10)
-    for scale, rows in ((300.0, 4), (300.0, 150), (2.0 ** -11, 4), (2.0 ** -11, 150)):
+    for scale, rows in ((300.0, 4), (300.0, 700), (2.0 ** -11, 4), (2.0 ** -11, 700)):
         x, a = _randn(g, rows, 512, dtype=FP16, scale=scale), _randn(g, 2, 16, 512, dtype=FP16, scale=min(scale, 20.0))
         b = _randn(g, 2, 64, 16, dtype=FP16, scale=2.0 ** -12 if scale > 1 else 30.0)
         y = _randn(g, rows, 64, dtype=FP16, scale=1.0 if scale > 1 else 2.0 ** -10)
@@ -396,7 +397,7 @@ def test_lora_large_low_rank_values(ck):
         _check_lora(ck.lora_add(y, x, a, b, ids), y, x, a, b, ids, None)
 
 
-@pytest.mark.parametrize("rows", [6, 48, 260])
+@pytest.mark.parametrize("rows", [6, 48, 800])
 def test_lora_strides_and_batches(ck, rows):
     g = _gen(11)
     k, n, rank = 256, 128, 16
@@ -453,7 +454,7 @@ def _front_case(ck, rows, seed):
             torch.arange(rows, device="cuda") % 4, 0.5 + torch.rand(3, generator=g, device="cuda"), pos, ck.rope_axes_freqs(axes), axes, heads, dim]
 
 
-@pytest.mark.parametrize("rows", [1, 50, 333])
+@pytest.mark.parametrize("rows", [1, 50, 700])
 def test_layer_front_end(ck, rows):
     args = _front_case(ck, rows, rows)
     x, res, nw, wq, ws, a, b, ids, scales, pos, freqs, axes, heads, dim = args
@@ -471,7 +472,7 @@ def test_layer_front_end(ck, rows):
     assert torch.equal(h, h2) and torch.equal(v, parts[2])
 
 
-@pytest.mark.parametrize("rows", [4, 333])
+@pytest.mark.parametrize("rows", [4, 700])
 def test_front_end_on_another_stream_and_in_graphs(ck, rows):
     args, other = _front_case(ck, rows, 20), _front_case(ck, rows, 21)
     want, want_other = _front_end(ck, *args), _front_end(ck, *other)

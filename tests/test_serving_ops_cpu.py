@@ -147,7 +147,7 @@ def test_native_rope_refusals():
 
 
 def test_native_lora_refusals():
-    def call(y=P, x=P, a=P, b=P, ids=P, out=P, ws=P, rows=400, k=24, n=16, r=8, count=2, ys=16, xs=24, os=16, per=1, t=2):
+    def call(y=P, x=P, a=P, b=P, ids=P, out=P, ws=P, rows=4000, k=24, n=16, r=8, count=2, ys=16, xs=24, os=16, per=1, t=2):
         _refused("launch_lora_add_kernel", y, x, a, b, ids, 0, out, ws, rows, k, n, r, count, ys, xs, os, per, t, False, None)
 
     for bad in (dict(y=0), dict(x=0), dict(a=0), dict(b=0), dict(ids=0), dict(out=0), dict(rows=0), dict(rows=1 << 40), dict(k=0), dict(k=20), dict(n=12), dict(r=0), dict(r=4),
