@@ -10,6 +10,9 @@ Addition: tensor parallelism.  With ``parallel="column"`` or ``"row"`` and (rank
 its shard of the checkpoint's weight, cut out of the packed codes and the tiled scale buffer without
 re-quantizing (comfy_kitchen/sharding.py); ``in_features`` / ``out_features`` stay those of the full layer.
 A row-parallel module returns this rank's partial sum (bias on rank 0 only); the caller sums over the ranks.
+
+Addition: adapters.  ``set_adapters`` gives a layer the low-rank adapters of many requests, unmerged beside its one
+quantized weight; ``forward(x, adapter_ids)`` then adds each row's own (``comfy_kitchen.lora_add``).
 """
 from __future__ import annotations
 
@@ -18,13 +21,43 @@ import logging
 import torch
 import torch.nn as nn
 
+import comfy_kitchen
 from comfy_kitchen.sharding import shard_linear_state
 from comfy_kitchen.tensor import QuantizedTensor, TensorCoreNVFP4Layout
 
 logger = logging.getLogger(__name__)
 
 
-class NVFP4Linear(nn.Module):
+class _WithAdapters(nn.Module):
+    """Low-rank adapters beside a layer's weight: held outside the state dict, moved with the module."""
+
+    def _no_adapters(self) -> None:
+        for name in ("adapter_a", "adapter_b", "adapter_scales"):
+            self.register_buffer(name, None, persistent=False)
+
+    def set_adapters(self, a: torch.Tensor | None, b: torch.Tensor | None = None, scales: torch.Tensor | None = None) -> None:
+        """a: [L, R, in_features], b: [L, out_features, R] (a tensor-parallel layer's shard of them), scales: float32 [L] or
+        None for ones; ``set_adapters(None)`` takes them off."""
+        if a is None:
+            self.adapter_a = self.adapter_b = self.adapter_scales = None
+            return
+        if b is None or a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.dtype != b.dtype:
+            raise ValueError("adapters are a [L, R, in_features] and b [L, out_features, R] of one dtype")
+        if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (a.shape[0],)):
+            raise ValueError(f"scales must be float32 [{a.shape[0]}]")
+        self.adapter_a, self.adapter_b, self.adapter_scales = a.detach().contiguous(), b.detach().contiguous(), scales
+
+    def _add_adapters(self, y: torch.Tensor, x: torch.Tensor, adapter_ids: torch.Tensor | None) -> torch.Tensor:
+        if adapter_ids is None:
+            return y
+        if self.adapter_a is None:
+            raise ValueError("adapter_ids given to a layer without adapters: call set_adapters first")
+        if isinstance(x, QuantizedTensor):
+            raise ValueError("the adapters read the layer's input unquantized: pass a plain tensor")
+        return comfy_kitchen.lora_add(y, x, self.adapter_a, self.adapter_b, adapter_ids, self.adapter_scales)
+
+
+class NVFP4Linear(_WithAdapters):
     """Linear layer whose weight lives only as NVFP4 codes + block scales (no full-precision copy)."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None,
@@ -37,6 +70,7 @@ class NVFP4Linear(nn.Module):
         self.parallel, self.rank, self.world = (parallel if world > 1 else None), rank, world
         self.weight = None   # set while loading a state dict
         self.input_scale = None
+        self._no_adapters()
         local_out = out_features // world if self.parallel == "column" else out_features
         keeps_bias = bias and not (self.parallel == "row" and rank != 0)
         if keeps_bias:
@@ -89,13 +123,12 @@ class NVFP4Linear(nn.Module):
         sd.update(self.weight.state_dict(prefix + "weight"))
         return sd
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if not isinstance(x, QuantizedTensor):
-            x = QuantizedTensor.from_float(x, "TensorCoreNVFP4Layout", scale=self.input_scale)
-        return torch.nn.functional.linear(x, self.weight, self.bias)
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        qx = x if isinstance(x, QuantizedTensor) else QuantizedTensor.from_float(x, "TensorCoreNVFP4Layout", scale=self.input_scale)
+        return self._add_adapters(torch.nn.functional.linear(qx, self.weight, self.bias), x, adapter_ids)
 
 
-class MXFP8Linear(nn.Module):
+class MXFP8Linear(_WithAdapters):
     """Linear layer with an MXFP8 weight (32-element E4M3 blocks, E8M0 scales)."""
 
     def __init__(self, in_features: int, out_features: int, bias: nn.Parameter | None = None,
@@ -104,6 +137,7 @@ class MXFP8Linear(nn.Module):
         self.in_features, self.out_features, self.compute_dtype = in_features, out_features, compute_dtype
         self.weight = nn.Parameter(weight_qt, requires_grad=False) if weight_qt is not None else None
         self.bias = bias
+        self._no_adapters()
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, device: str = "cuda") -> "MXFP8Linear":
@@ -117,7 +151,10 @@ class MXFP8Linear(nn.Module):
                    weight.dtype)
 
     @torch.no_grad()
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        return self._add_adapters(self._linear(x), x, adapter_ids)
+
+    def _linear(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         if not isinstance(x, QuantizedTensor):
             if x.ndim == 3:

@@ -430,6 +430,36 @@ def test_lora_of_nothing(ck):
     assert ck.lora_add(torch.empty(0, 32, device="cuda", dtype=BF16), e, a, b, torch.empty(0, device="cuda", dtype=torch.int32)).shape == (0, 32)
 
 
+def test_layers_with_adapters(ck):
+    """The linear layers on quantized weights call it beside their projection."""
+    from comfy_kitchen.linear import MXFP8Linear, NVFP4Linear
+
+    g = _gen(12)
+    k, n, rows = 256, 384, 70
+    a, b, scales = _randn(g, 3, 16, k, dtype=BF16, scale=0.06), _randn(g, 3, n, 16, dtype=BF16, scale=0.1), 0.5 + torch.rand(3, device="cuda")
+    w = _randn(g, n, k, dtype=BF16, scale=0.06)
+    mx = MXFP8Linear.from_linear(torch.nn.Linear(k, n, bias=False, device="cuda", dtype=BF16).requires_grad_(False))
+    ts = w.float().abs().max().reshape(1) / (6 * 448)
+    q, sf = ck.quantize_nvfp4(w, ts)
+    nv = NVFP4Linear(k, n, bias=False, device="cuda")
+    nv.load_state_dict({"weight": q, "weight_scale": sf.view(torch.uint8), "weight_scale_2": ts}, strict=False)
+    x = _randn(g, rows, k, dtype=BF16)
+    ids = torch.arange(rows, device="cuda") % 4
+    for layer in (mx, nv):
+        base = layer(x)
+        layer.set_adapters(a, b, scales)
+        assert torch.equal(layer(x), base)
+        got = layer(x, ids)
+        assert torch.equal(got, ck.lora_add(base, x, a, b, ids, scales))
+        _check_lora(got, base, x, a, b, ids, scales)
+        layer.set_adapters(None)
+        with pytest.raises(ValueError):
+            layer(x, ids)
+    mx.set_adapters(a, b)
+    three = mx(x.view(2, rows // 2, k), torch.tensor([1, 2], device="cuda"))
+    assert torch.equal(three.view(rows, n), ck.lora_add(mx(x), x, a, b, torch.tensor([1, 2], device="cuda").repeat_interleave(rows // 2)))
+
+
 # ------------------------------------------------------------------ together, on other streams, in graphs
 
 

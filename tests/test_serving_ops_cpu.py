@@ -110,6 +110,23 @@ def test_cpu_tensors_find_no_backend():
         ck.apply_rope_axes1(torch.zeros(1, 1, 2, 8), torch.zeros(2, 1), torch.zeros(4, dtype=torch.float64), (8,))
 
 
+def test_adapters_of_a_layer():
+    from comfy_kitchen.linear import MXFP8Linear, NVFP4Linear
+
+    for layer in (NVFP4Linear(24, 16, bias=False), MXFP8Linear(24, 16)):
+        a, b = torch.zeros(2, 8, 24, dtype=BF16), torch.zeros(2, 16, 8, dtype=BF16)
+        layer.set_adapters(a, b, torch.ones(2))
+        assert layer.adapter_a.shape == a.shape and not any("adapter" in k for k in torch.nn.Module.state_dict(layer))
+        for bad in ((a, None), (a, b[:1]), (a, b.transpose(1, 2)), (a, b.float()), (a, b, torch.ones(3)), (a, b, torch.ones(2).double())):
+            with pytest.raises(ValueError):
+                layer.set_adapters(*bad)
+        layer.set_adapters(None)
+        with pytest.raises(ValueError, match="set_adapters"):
+            layer._add_adapters(torch.zeros(1, 16, dtype=BF16), torch.zeros(1, 24, dtype=BF16), torch.zeros(1, dtype=torch.int32))
+        y = torch.zeros(1, 16)
+        assert layer._add_adapters(y, None, None) is y
+
+
 def test_frequency_table():
     f = ck.rope_axes_freqs((4, 8), 100.0, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 100.0 ** -0.5, 1.0, 100.0 ** -0.25, 100.0 ** -0.5, 100.0 ** -0.75], dtype=torch.float64))
