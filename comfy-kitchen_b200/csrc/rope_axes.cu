@@ -72,7 +72,17 @@ __device__ __forceinline__ void head_at(const RopeAxesParams& p, int64_t b, int6
     dst = static_cast<T*>(p.o[which]) + b * p.so[which][0] + n * p.so[which][1] + h * p.so[which][2];
 }
 
-// Vectors of 8 elements: unit stride, D (and, split-half, P) a multiple of 8, 16-byte aligned rows.
+// Two pairs at a time with sm_100's packed fp32 instructions: (a0, a1) cos - (b0, b1) sin and (a0, a1) sin + (b0, b1) cos.
+__device__ __forceinline__ void rotate2(float2 c, float2 s, float2& a, float2& b) {
+    const float2 oa = __ffma2_rn(b, make_float2(-s.x, -s.y), __fmul2_rn(a, c));
+    b = __ffma2_rn(b, c, __fmul2_rn(a, s));
+    a = oa;
+}
+
+// Vectors of 8 elements: unit stride, D (and, split-half, P) a multiple of 8, 16-byte aligned rows.  The loop over heads is
+// kept to a few instructions an element (pointers that step by the head's stride, packed arithmetic): with 64-bit
+// offsets worked out for every head it took 140 instructions a vector, 80 % of the issue slots at full clock, and was
+// no longer bound by HBM where the clock is lower.
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const RopeAxesParams p) {
     constexpr int kPairs = kSplit ? 8 : 4;
@@ -89,50 +99,75 @@ __global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const RopeAxesP
     const int turning = kSplit ? p.P / 8 : (2 * p.P + 7) / 8;
     const bool rotates = v < turning;
     const int lo = kSplit && !rotates ? 2 * p.P + (v - turning) * 16 : v * 8;
-    const int hi = kSplit ? (rotates ? lo + p.P : lo + 8) : lo;
-    const bool second = kSplit && hi < p.D;
-    float2 t[kPairs];
+    const int apart = kSplit ? (rotates ? p.P : 8) : 0;
+    const bool second = kSplit && lo + apart < p.D;
+    const bool whole = kSplit || (v + 1) * 4 <= p.P;   // (interleaved: all four pairs turn)
+    float2 c[kPairs / 2], s[kPairs / 2];               // of pairs 2 i and 2 i + 1
     if (rotates) {
         const int64_t off = b * p.sp[0] + site * p.sp[1];
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-            const int pair = v * kPairs + i;
-            t[i] = pair < p.P ? pair_turn(p, off, pair) : make_float2(1.0f, 0.0f);
+        for (int i = 0; i < kPairs / 2; ++i) {
+            const int pair = v * kPairs + 2 * i;
+            const float2 t0 = pair < p.P ? pair_turn(p, off, pair) : make_float2(1.0f, 0.0f);
+            const float2 t1 = pair + 1 < p.P ? pair_turn(p, off, pair + 1) : make_float2(1.0f, 0.0f);
+            c[i] = make_float2(t0.x, t1.x);
+            s[i] = make_float2(t0.y, t1.y);
         }
     }
     constexpr int kBatch = kSplit ? 2 : 4;
-    for (int h = h0; h < h1; h += kBatch) {
-        Raw8<T> ra[kBatch], rb[kBatch];
-        const T* src[kBatch];
-        T* dst[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (h + i >= h1) break;
-            head_at<T>(p, b, site, h + i, src[i], dst[i]);
-            ra[i] = load_raw8<T>(src[i] + lo);
-            if (second) rb[i] = load_raw8<T>(src[i] + hi);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (h + i >= h1) break;
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {          // q's heads of the chunk, then k's
+        const int first = which ? p.heads[0] : 0;
+        const int from = max(h0, first) - first, n = min(h1, first + p.heads[which]) - first - from;
+        const int64_t step_in = p.sx[which][2], step_out = p.so[which][2];
+        const T* src = static_cast<const T*>(p.x[which]) + b * p.sx[which][0] + site * p.sx[which][1] + from * step_in + lo;
+        T* dst = static_cast<T*>(p.o[which]) + b * p.so[which][0] + site * p.so[which][1] + from * step_out + lo;
+        auto turn = [&](Raw8<T>& ra, Raw8<T>& rb, T* out) {
             float x[8], y[8];
-            unpack8(ra[i], x);
+            unpack8(ra, x);
             if (kSplit) {
-                if (second) unpack8(rb[i], y);
+                if (second) unpack8(rb, y);
                 if (rotates) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) rotate(t[j], x[j], y[j], x[j], y[j]);
+                    for (int i = 0; i < 4; ++i) {
+                        float2 e = make_float2(x[2 * i], x[2 * i + 1]), f = make_float2(y[2 * i], y[2 * i + 1]);
+                        rotate2(c[i], s[i], e, f);
+                        x[2 * i] = e.x; x[2 * i + 1] = e.y;
+                        y[2 * i] = f.x; y[2 * i + 1] = f.y;
+                    }
                 }
-                store8<T>(dst[i] + lo, x);
-                if (second) store8<T>(dst[i] + hi, y);
+                store8<T>(out, x);
+                if (second) store8<T>(out + apart, y);
             } else {
                 if (rotates) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (v * 4 + j < p.P) rotate(t[j], x[2 * j], x[2 * j + 1], x[2 * j], x[2 * j + 1]);
+                    for (int i = 0; i < 2; ++i) {
+                        float2 e = make_float2(x[4 * i], x[4 * i + 2]), f = make_float2(x[4 * i + 1], x[4 * i + 3]);
+                        rotate2(c[i], s[i], e, f);
+                        if (whole || v * 4 + 2 * i < p.P) { x[4 * i] = e.x; x[4 * i + 1] = f.x; }
+                        if (whole || v * 4 + 2 * i + 1 < p.P) { x[4 * i + 2] = e.y; x[4 * i + 3] = f.y; }
+                    }
                 }
-                store8<T>(dst[i] + lo, x);
+                store8<T>(out, x);
             }
+        };
+        int h = 0;
+#pragma unroll 1
+        for (; h + kBatch <= n; h += kBatch, src += kBatch * step_in, dst += kBatch * step_out) {
+            Raw8<T> ra[kBatch], rb[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                ra[i] = load_raw8<T>(src + i * step_in);
+                if (second) rb[i] = load_raw8<T>(src + i * step_in + apart);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) turn(ra[i], rb[i], dst + i * step_out);
+        }
+#pragma unroll 1
+        for (; h < n; ++h, src += step_in, dst += step_out) {
+            Raw8<T> ra = load_raw8<T>(src), rb = ra;
+            if (second) rb = load_raw8<T>(src + apart);
+            turn(ra, rb, dst);
         }
     }
 }
