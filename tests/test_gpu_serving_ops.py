@@ -80,6 +80,30 @@ def test_norm_mxfp8_against_the_oracle(ck):
     assert torch.equal(_bytes(q).cpu(), _bytes(rq)) and torch.equal(_bytes(s).cpu(), _bytes(rs))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_norm_mxfp8_scales_over_the_whole_range(ck, dtype):
+    """Blocks from the smallest numbers of the type to the largest, with amax at, just below and just above 448 x 2^k, zeros, infinities and NaN:
+    the codes and scales are those of the quantizer for the norm as stored."""
+    low, high = {BF16: (-133, 127), FP32: (-149, 127), FP16: (-24, 15)}[dtype]
+    mags = []
+    for k in range(low, high + 1):
+        for m in (1.0, 1.75, 1.75 * (1 - torch.finfo(dtype).eps), 1.75 * (1 + torch.finfo(dtype).eps)):
+            mags.append(m * 2.0 ** k)
+    mags = mags + [0.0, float("inf"), float("nan")]
+    g = _gen(5)
+    # x is +-1 and eps 0, so the norm is the weight with a sign: the weight is what is quantized
+    width = 32 * len(mags)
+    sign = torch.where(torch.rand(5, width, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    part = torch.rand(len(mags), 32, generator=g, device="cuda", dtype=torch.float64)
+    part[torch.arange(len(mags)), torch.randint(0, 32, (len(mags),), generator=g, device="cuda")] = 1.0
+    weight = (part * torch.tensor(mags, dtype=torch.float64, device="cuda")[:, None]).reshape(-1).to(dtype)
+    q, s, h, y = ck.add_rmsnorm_quantize_mxfp8(sign.to(dtype), torch.zeros_like(sign).to(dtype), weight, 0.0, return_norm=True)
+    expect_q, expect_s = ck.quantize_mxfp8(y, pad_32x=True)
+    assert torch.equal(_bytes(q), _bytes(expect_q[:5])) and torch.equal(_bytes(s), _bytes(expect_s))
+    finite = torch.isfinite(weight.float())
+    assert torch.equal(y[:, finite].abs().double(), weight[finite].abs().double().expand(5, -1))
+
+
 @pytest.mark.parametrize("width", [1, 7, 16, 100, 1315, 4096, 8192, 33000])
 @pytest.mark.parametrize("dtype,stream,out", [(BF16, BF16, torch.float8_e4m3fn), (FP16, FP32, torch.float8_e5m2), (FP32, FP32, torch.float8_e4m3fn)])
 def test_norm_fp8(ck, width, dtype, stream, out):
