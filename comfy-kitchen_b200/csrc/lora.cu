@@ -331,9 +331,10 @@ struct TileList {
     int count, unused;
 };
 
-// A K step of a tile of c adapters takes about (3 + c) / 4 of the time of one of a single adapter's.  (The weight ends at 8,
-// twice the least one: with at least four steps a CTA on average, no share is then shorter than a step.)
-__device__ __forceinline__ int shrink_weight(int asked) { return asked == 0 ? 0 : 3 + min(asked, 5); }
+// A K step of a tile of two adapters takes about 5/4 of the time of one of a single adapter's, of three 7/4 (fewer steps of x
+// fit ahead of the A tiles' ring), and so on.  (The weight ends at 16, four times the least one: with at least four steps a CTA on
+// average, no share is then shorter than a step.)
+__device__ __forceinline__ int shrink_weight(int asked) { return asked == 0 ? 0 : asked < 3 ? 3 + asked : min(2 * asked + 1, 16); }
 
 // low[t][:] = A_{ids[t]} x[t] as partial sums over parts of K: every CTA takes an equal run of the tiles' K steps, so that all
 // SMs are busy whatever the number of rows, and leaves a block of sums for each tile that it meets.  CTA c's block for
@@ -683,10 +684,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     if (warp == 1) tc::tmem_alloc(s_tmem, kExpandColumns);
     if (warp == 3) {
         // (The counts are there: this kernel can start only when every CTA of the two before it has, and the first of those
-        // waits for them.)  In units of 128 clocks: an item's share of HBM's time, half as much again for each further adapter
-        // (ranks 64 and 128), or the MMAs of a high rank.
+        // waits for them.)  In units of 128 clocks: an item's share of HBM's time, three quarters as much again for each further
+        // adapter (ranks 64 and 128) and a third less without one, or the MMAs of a high rank.
         const int mmas = kU * plan.k_steps + 1;
-        auto weight = [&](int asked) { return asked == 0 ? (in_place ? 0 : 11 * kU) : max(11 * kU * (asked + 1) / 2, asked * mmas); };
+        auto weight = [&](int asked) { return asked == 0 ? (in_place ? 0 : 7 * kU) : max(11 * kU * (3 * asked + 1) / 4, asked * mmas); };
         int worked;
         const int64_t all = total_weight(p.asked128, plan.tiles, lane, worked, weight) * plan.steps;
         const Place from = locate(p.asked128, plan.tiles, plan.steps, all * blockIdx.x / gridDim.x, lane, weight);
@@ -760,10 +761,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         tc::Ring br;
         uint32_t n = 0, seg = 0;
         bool ok = true;
-        tc::wait_for_dependency();      // the first kernel's image
         for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
             const int begin = begin_of(tile), end = end_of(tile);
             const int count = tile_count(tile);
+            if (tile == from.tile) tc::wait_for_dependency();   // the first kernel's image
             if (count == 0) continue;
             ok = tc::mbar_wait(low_done, (seg & 1) ^ 1, s_abort, &g_lora_status, kWaitAcc);   // nothing reads s_low any more
             if (!ok) break;
@@ -839,10 +840,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         uint32_t n = 0;                 // accumulators so far
         uint32_t odd = 0;               // the parity of the step's first unit: which group takes it
         bool ok = true;
-        tc::wait_for_dependency();      // the first kernel's factors
         for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
             const int begin = begin_of(tile), end = end_of(tile);
             const int count = tile_count(tile);
+            if (tile == from.tile) tc::wait_for_dependency();   // the first kernel's factors
             if (count == 0 && in_place) continue;
             const int mine = s_slot[r_in_tile];
             const float factor = mine >= 0 ? __ldcg(p.factor + (int64_t)tile * kTile + r_in_tile) : 0.0f;
