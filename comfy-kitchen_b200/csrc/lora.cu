@@ -8,7 +8,7 @@
 // once; the products' 2 R (K + N) flop a row stay below that up to a rank of about 128.  Two forms:
 //   few rows:   one CTA per row.
 //   many rows:  four kernels, two of them on the tensor cores (tcgen05):
-//               count:   how many adapters each tile of rows asks for, by which the others share out their work;
+//               count:   which adapters each tile of rows asks for; by their number the others share out their work;
 //               shrink:  low[t, :] = A x[t], equal shares of the tiles' K steps for every SM, partial sums in fp32;
 //               join:    the partial sums added in order (no atomics, the same bits every time) and laid out as the
 //                        next product's operand;
@@ -34,6 +34,17 @@ constexpr int kSmemMost = 232448;
 __device__ int g_lora_status = 0;
 enum : int { kWaitFull = 1, kWaitEmpty = 2, kWaitAcc = 3, kWaitAccFree = 4, kWaitLow = 5, kWaitY = 6, kWaitYFree = 7, kWaitList = 8, kWaitDone = 9 };
 
+constexpr int kShrinkRows = 256;    // rows of x in a tile of the first product (its MMA's N)
+
+// What the rows of such a tile ask for.
+struct alignas(16) TileList {
+    int16_t slot[kShrinkRows];      // [token]: which adapter (-1: none)
+    int id[kShrinkRows];            // [adapter]: its id,
+    int16_t from[kShrinkRows];      // the first token (a multiple of 8)
+    int16_t wide[kShrinkRows];      // and the number of tokens (of 16) that its product is taken for
+    int count;
+};
+
 struct LoraArgs {
     const void* y;
     const void* x;
@@ -47,6 +58,9 @@ struct LoraArgs {
     float* partial;         // [blocks, 256, R]: sums over a part of K for a tile of 256 rows
     int* asked128;          // [tiles of 128 rows]: how many adapters a tile asks for
     int* asked256;          // [tiles of 256 rows]
+    int* list128;           // [tiles of 128 rows][128]: their ids
+    int16_t* slot128;       // [tiles of 128 rows][128]: which of them a row asks for (-1: none)
+    TileList* list256;      // [tiles of 256 rows]
     int* first_block;       // [tiles of 256 rows]: a tile's blocks in `partial`, first
     int* last_block;        // and last
     int64_t rows, K, N, R, L;
@@ -170,7 +184,7 @@ __device__ __forceinline__ void tile_ids(const LoraArgs& p, int64_t row0, int la
 }
 
 // The different adapters among them, in the order of their first rows: calls each(place, id, first row, last row) with
-// every lane, leaves each row's place in `slot` (-1: none; may be null) and returns their number.  By a whole warp.
+// every lane, leaves each row's place in `slot` (-1: none) and returns their number.  By a whole warp.
 template <int kRows, typename Each>
 __device__ __forceinline__ int tile_adapters(const int (&id)[kRows / 32], int lane, int16_t* slot, Each each) {
     constexpr int kQ = kRows / 32;
@@ -199,8 +213,7 @@ __device__ __forceinline__ int tile_adapters(const int (&id)[kRows / 32], int la
     }
 #pragma unroll
     for (int q = 0; q < kQ; ++q)
-        if (slot) slot[32 * q + lane] = (int16_t)place[q];
-    __syncwarp();
+        slot[32 * q + lane] = (int16_t)place[q];
     return count;
 }
 
@@ -251,22 +264,28 @@ __device__ __forceinline__ int64_t total_weight(const int* asked, int tiles, int
     return sum;
 }
 
-// One CTA per 256 rows: warps 0 and 1 count a half's adapters, warp 2 the whole tile's.
+// One CTA per 256 rows: warps 0 and 1 list a half's adapters, warp 2 the whole tile's.  (The kernels behind read the lists; working
+// them out again there, with code that no cache holds yet, took 4 us before the first product.)
 __global__ void __launch_bounds__(96) lora_count_kernel(const LoraArgs p) {
     tc::launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tile = blockIdx.x;
-    int n;
     if (warp < 2) {
+        const int64_t half = tile * 2 + warp;
         int id[4];
-        tile_ids<128>(p, tile * 256 + warp * 128, lane, id);
-        n = tile_adapters<128>(id, lane, nullptr, [](int, int, int, int) {});
+        tile_ids<kTile>(p, half * kTile, lane, id);
+        const int n = tile_adapters<kTile>(id, lane, p.slot128 + half * kTile, [&](int j, int which, int, int) { if (lane == 0) p.list128[half * kTile + j] = which; });
+        if (lane == 0) p.asked128[half] = n;
     } else {
+        TileList& l = p.list256[tile];
         int id[8];
-        tile_ids<256>(p, tile * 256, lane, id);
-        n = tile_adapters<256>(id, lane, nullptr, [](int, int, int, int) {});
+        tile_ids<kShrinkRows>(p, tile * kShrinkRows, lane, id);
+        const int n = tile_adapters<kShrinkRows>(id, lane, l.slot, [&](int j, int which, int lo, int hi) {
+            const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
+            if (lane == 0) { l.id[j] = which; l.wide[j] = (int16_t)wide; l.from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
+        });
+        if (lane == 0) { l.count = n; p.asked256[tile] = n; }
     }
-    if (lane == 0) (warp < 2 ? p.asked128 + tile * 2 + warp : p.asked256 + tile)[0] = n;
 }
 
 template <typename T>
@@ -317,19 +336,9 @@ struct ShrinkPlan {
     int smem;
 };
 
-constexpr int kShrinkRows = 256;           // rows of x in a tile (the MMA's N)
 constexpr int kShrinkThreads = 352;        // warp 0: TMA, warp 1: MMA, warps 2-9: epilogue, warp 10: the tiles' lists
 constexpr int kXBytes = kShrinkRows * 128;
 constexpr int kShrinkColumns = 512;        // all of TMEM
-
-// What the rows of a tile ask for.
-struct TileList {
-    int id[kShrinkRows];            // [adapter]: its id,
-    int16_t from[kShrinkRows];      // the first token (a multiple of 8)
-    int16_t wide[kShrinkRows];      // and the number of tokens (of 16) that its product is taken for
-    int16_t slot[kShrinkRows];      // [token]: which adapter (-1: none)
-    int count, unused;
-};
 
 // A K step of a tile of two adapters takes about 5/4 of the time of one of a single adapter's, of three 7/4 (fewer steps of x
 // fit ahead of the A tiles' ring), and so on.  (The weight ends at 16, four times the least one: with at least four steps a CTA on
@@ -366,7 +375,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     uint64_t* drain = acc_empty + 1;
     uint64_t* listed = drain + 1;                                             // [2] a tile's lists are there
     uint64_t* unlisted = listed + 2;                                          // [2] nobody needs them any more
-    TileList* s_lists = reinterpret_cast<TileList*>(unlisted + 2);            // [2]
+    TileList* s_lists = reinterpret_cast<TileList*>((reinterpret_cast<uintptr_t>(unlisted + 2) + 15) & ~uintptr_t(15));   // [2]
     Place* s_share = reinterpret_cast<Place*>(s_lists + 2);                   // this CTA's: from, to
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_share + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
@@ -408,15 +417,27 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         for (int tile = tile0; tile <= tile1 && ok; ++tile) {
             const int at = (tile - tile0) & 1;
             TileList& l = s_lists[at];
-            int id[kShrinkRows / 32];
-            tile_ids<kShrinkRows>(p, (int64_t)tile * kShrinkRows, lane, id);
+            const TileList& from_count = p.list256[tile];
+            // (a lane's share of the slots, of the first 32 adapters and the count at once)
+            const uint4 slots = __ldcg(reinterpret_cast<const uint4*>(from_count.slot) + lane);
+            const int found = __ldcg(&from_count.count);
+            int id = __ldcg(from_count.id + lane);
+            int16_t first = __ldcg(from_count.from + lane), wide = __ldcg(from_count.wide + lane);
             ok = tc::mbar_wait(&unlisted[at], ((tile - tile0) >> 1 & 1) ^ 1, s_abort, &g_lora_status, kWaitList);
             if (!ok) break;
-            const int found = tile_adapters<kShrinkRows>(id, lane, l.slot, [&](int j, int which, int lo, int hi) {
-                const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
-                if (lane == 0) { l.id[j] = which; l.wide[j] = (int16_t)wide; l.from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
-            });
-            if (lane == 0) { l.count = found; tc::mbar_arrive(&listed[at]); }
+            reinterpret_cast<uint4*>(l.slot)[lane] = slots;
+            for (int j = lane;;) {
+                l.id[j] = id;
+                l.from[j] = first;
+                l.wide[j] = wide;
+                if ((j += 32) >= found) break;
+                id = __ldcg(from_count.id + j);
+                first = __ldcg(from_count.from + j);
+                wide = __ldcg(from_count.wide + j);
+            }
+            if (lane == 0) l.count = found;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&listed[at]);
             __syncwarp();
         }
     }
@@ -662,14 +683,12 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     uint64_t* low_done = low_full + 1;                                 // a tile's last MMA is complete
     uint64_t* drain = low_done + 1;
     int* s_list = reinterpret_cast<int*>(drain + 1);                   // (warp 10's)
-    int16_t* s_slots = reinterpret_cast<int16_t*>(s_list + kTile);
-    Place* s_share = reinterpret_cast<Place*>(s_slots + kExpandThreads / 32 * kTile);   // this CTA's: from, to
+    Place* s_share = reinterpret_cast<Place*>(s_list + kTile);         // this CTA's: from, to
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_share + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool in_place = p.out == p.y;
-    int16_t* s_slot = s_slots + warp * kTile;                // a warp's own: the roles are at different tiles
 
     if (threadIdx.x == 64) {
         for (int s = 0; s < plan.b_stages; ++s) { tc::mbar_init(&b_full[s], 1); tc::mbar_init(&b_empty[s], 1); }
@@ -704,11 +723,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     auto begin_of = [&](int tile) { return tile == from.tile ? from.step : 0; };
     auto end_of = [&](int tile) { return tile == to.tile ? to.step : plan.steps; };
 
-    int id[kTile / 32];
-    auto tile_count = [&](int tile) {
-        tile_ids<kTile>(p, (int64_t)tile * kTile, lane, id);
-        return tile_adapters<kTile>(id, lane, s_slot, [](int, int, int, int) {});
-    };
+    auto tile_count = [&](int tile) { return __ldcg(p.asked128 + tile); };
     // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles
     if (warp == 0) {
         tc::Ring yr;
@@ -736,8 +751,9 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         bool ok = true;
         for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
             const int begin = begin_of(tile), end = end_of(tile);
-            tile_ids<kTile>(p, (int64_t)tile * kTile, lane, id);
-            const int count = tile_adapters<kTile>(id, lane, s_slot, [&](int j, int which, int, int) { if (lane == 0) s_list[j] = which; });
+            const int count = tile_count(tile);
+            for (int j = lane; j < count; j += 32) s_list[j] = __ldcg(p.list128 + (int64_t)tile * kTile + j);
+            __syncwarp();
             for (int step = begin; step < end && ok; ++step)
                 for (int j = 0; j < count && ok; ++j) {
                     const int which = s_list[j];
@@ -843,9 +859,9 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         for (int tile = from.tile; tile <= tile1 && ok; ++tile) {
             const int begin = begin_of(tile), end = end_of(tile);
             const int count = tile_count(tile);
+            const int mine = __ldcg(p.slot128 + (int64_t)tile * kTile + r_in_tile);
             if (tile == from.tile) tc::wait_for_dependency();   // the first kernel's factors
             if (count == 0 && in_place) continue;
-            const int mine = s_slot[r_in_tile];
             const float factor = mine >= 0 ? __ldcg(p.factor + (int64_t)tile * kTile + r_in_tile) : 0.0f;
             for (int step = begin; step < end && ok; ++step) {
                 for (int j = 0; j < count && ok; ++j, ++n) {
@@ -949,7 +965,7 @@ ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R) {
     s.tiles = (int)ceil_div(rows, kShrinkRows);
     const int64_t most = ceil_div((int64_t)s.tiles * s.k_tiles, 4);   // at least four steps of K for a CTA
     s.ctas = (int)(most < sm_count() ? most : sm_count());
-    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + 2 * (int)(sizeof(TileList) + sizeof(Place)) + 16;
+    const int a_bytes = s.halves * kTileBytes, rest = 1024 + 32 * 8 + 16 + 2 * (int)(sizeof(TileList) + sizeof(Place)) + 16;
     s.x_stages = (kSmemMost - rest - a_bytes) / (kXBytes + a_bytes);
     s.a_stages = s.x_stages + 1;
     s.smem = rest + s.x_stages * kXBytes + s.a_stages * a_bytes;
@@ -958,14 +974,15 @@ ShrinkPlan shrink_plan(int64_t rows, int64_t K, int64_t R) {
 
 // Where the parts of the workspace lie.
 struct Workspace {
-    int64_t factor, partial, tables, bytes;   // (the image is at 0)
+    int64_t factor, partial, lists, tables, bytes;   // (the image is at 0)
 };
 Workspace workspace_of(const ShrinkPlan& s, int64_t rows, int64_t R) {
     Workspace w{};
     w.factor = (int64_t)s.tiles * (kShrinkRows / kTile) * 2 * s.blocks * kTileBytes;
     w.partial = w.factor + round_up(rows * 4, 128);
-    w.tables = w.partial + (int64_t)(s.ctas + s.tiles) * kShrinkRows * R * 4;
-    w.bytes = w.tables + (int64_t)s.tiles * 5 * 4;
+    w.lists = w.partial + (int64_t)(s.ctas + s.tiles) * kShrinkRows * R * 4;
+    w.tables = w.lists + (int64_t)s.tiles * (int64_t)sizeof(TileList);
+    w.bytes = w.tables + (int64_t)s.tiles * (5 * 4 + kShrinkRows * (4 + 2));
     return w;
 }
 
@@ -1000,21 +1017,19 @@ int launch_expand(const LoraArgs& p, cudaStream_t stream) {
     e.k_steps = (int)ceil_div(p.R, 16);
     const int64_t items = (int64_t)e.steps * e.tiles;
     e.blocks = (int)ceil_div(p.R, 64);
-    const int rest = 1024 + 48 * 8 + kTile * 4 + kExpandThreads / 32 * kTile * 2 + 2 * (int)sizeof(Place) + 16;
+    const int rest = 1024 + 64 * 8 + kTile * 4 + 2 * (int)sizeof(Place) + 16;
     // The image, a stage of B and four units of y (their number is even, so that a stage always serves
     // the same group of epilogue warps; a group that waited for a stage whose last load it had not seen might mistake that
-    // one's end for its own); then y and B in turn.
+    // one's end for its own); then, as far as there is room, six units of y, B for two steps, eight units of y.
+    // (16384 x 8192, rank 128: six units with B for one step, 1 1/2 and 2: 227, 210 and 204 us; four units and two steps 214.)
     e.b_stages = 1;
     e.y_stages = 4;
     int room = kSmemMost - rest - 2 * e.blocks * kTileBytes - b_bytes - e.y_stages * kTileBytes;
     if (room < 0) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld does not fit", (long long)p.R);
-    while (e.y_stages < 8 || e.b_stages < 4) {
-        const bool y = e.y_stages < 8 && room >= 2 * kTileBytes;
-        if (y) { e.y_stages += 2; room -= 2 * kTileBytes; }
-        const bool b = e.b_stages < 4 && room >= b_bytes;
-        if (b) { ++e.b_stages; room -= b_bytes; }
-        if (!b && !y) break;
-    }
+    auto more_y = [&](int most) { while (e.y_stages < most && room >= 2 * kTileBytes) { e.y_stages += 2; room -= 2 * kTileBytes; } };
+    more_y(6);
+    while (e.b_stages < 2 * e.blocks + 1 && room >= b_bytes) { ++e.b_stages; room -= b_bytes; }
+    more_y(8);
     e.smem = kSmemMost - room;
     CUtensorMap map_b, map_y, map_out;
     const int64_t bd[3] = {p.R, p.N, p.L}, bs[2] = {p.R * 2, p.N * p.R * 2};
@@ -1040,6 +1055,9 @@ int launch_many(LoraArgs p, uint8_t* workspace, cudaStream_t stream) {
     p.asked256 = p.asked128 + 2 * s.tiles;
     p.first_block = p.asked256 + s.tiles;
     p.last_block = p.first_block + s.tiles;
+    p.list128 = p.last_block + s.tiles;
+    p.slot128 = reinterpret_cast<int16_t*>(p.list128 + (int64_t)s.tiles * kShrinkRows);
+    p.list256 = reinterpret_cast<TileList*>(workspace + w.lists);
     CUtensorMap map_x, map_a;
     const int64_t xd[2] = {p.K, p.rows}, xs[1] = {p.x_stride * 2};
     const int64_t ad[3] = {p.K, p.R, p.L}, as[2] = {p.K * 2, p.R * p.K * 2};
@@ -1097,7 +1115,7 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
-    const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
+    const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
     if (few_rows(rows, K, N, rank)) {
         const dim3 grid(kFewCluster, (unsigned)rows);
         if (dtype_code == CK_BF16) lora_few_kernel<__nv_bfloat16><<<grid, kFewThreads, 0, stream>>>(p);
