@@ -665,7 +665,7 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
             raise ValueError(f"{what}: weight must be [{d}], got {list(weight.shape)}")
         if weight.dtype != dtype or not weight.is_contiguous():
             weight = weight.to(dtype).contiguous()
-    _no_grad(what, x, residual, weight)
+    _no_grad(what, x, residual, weight, sum_out)
     _same_device(what, device, residual, weight, sum_out)
     if sum_out is None:
         sum_out = _empty(residual, shape, stream_dtype)
@@ -837,7 +837,7 @@ def lora_add(
         raise ValueError(f"{what}: adapter_ids {list(ids_shape)} must have the shape of x's leading dimensions {list(x_shape[:-1])} or of the first of them")
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,)):
         raise ValueError(f"{what}: scales must be float32 [{adapters}]")
-    _no_grad(what, y, x, a, b, scales)
+    _no_grad(what, y, x, a, b, scales, out)
     _same_device(what, device, y, a, b, adapter_ids, scales, out)
     if out is None:
         out = _empty(y, y_shape, dtype)
@@ -871,7 +871,7 @@ def lora_add(
     if scales is not None and not scales.is_contiguous():
         scales = scales.contiguous()
     # scratch of the tiled kernels; the allocator's, so that streams and captured graphs keep theirs apart
-    need = _native.load().ck_lora_workspace_bytes(rows, k, n, rank) if rows > 1 else 0
+    need = _native.load().ck_lora_workspace_bytes(rows, k, n, rank)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch(device, "launch_lora_add_kernel", py, px, pa, pb, ids.data_ptr(), 0 if scales is None else scales.data_ptr(), po,
             0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, y_stride, x_stride, o_stride, rows // ids.numel(),

@@ -37,7 +37,8 @@ class _WithAdapters(nn.Module):
 
     def set_adapters(self, a: torch.Tensor | None, b: torch.Tensor | None = None, scales: torch.Tensor | None = None) -> None:
         """a: [L, R, in_features], b: [L, out_features, R] (a tensor-parallel layer's shard of them), scales: float32 [L] or
-        None for ones; ``set_adapters(None)`` takes them off."""
+        None for ones; ``set_adapters(None)`` takes them off.  They move with the module; a cast of the module to another
+        dtype takes the scales along, so set them again behind one."""
         if a is None:
             self.adapter_a = self.adapter_b = self.adapter_scales = None
             return

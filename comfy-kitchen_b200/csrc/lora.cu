@@ -17,6 +17,10 @@
 // rows and keeps a row's own (a row of another request never enters a sum, whatever it holds).  Requests that lie behind
 // one another cost nothing extra; a tile of 128 different adapters reads 128 adapters, as it must.
 //
+// Measured, back to back: 16384 rows, 8192 -> 8192, rank 128, 8 requests: 204 us (64 % of the copy rate; 193 us in a short burst, of
+// which count 5, shrink 65, join 9, expand 100); 4608 rows, 4096 -> 12288, rank 64, 7 requests: 76 us (54 %), of which about 20 are
+// the four kernels' beginnings and ends; one row 4.2 us, 64 rows of 16 adapters 16.7 us on the device.
+//
 // Rounding: sums in fp32.  The low-rank vector is the second product's 16-bit operand: it goes in as two parts, the
 // rounded value and what the rounding left (for fp16 scaled by a power of two per row, which keeps large and small vectors
 // in range), so that about 16 bits (fp16: 22) of it are used and the output's rounding is the only one that shows.
@@ -605,7 +609,9 @@ __global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs 
     tc::launch_dependents();
     const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 8) + (threadIdx.x >> 3);
     const int sub = threadIdx.x & 7;
-    const int id = row < p.rows ? adapter_of(p, row) : -1;
+    // (the lists, as all others use them, not the ids: a tile that nobody asked anything of then has no sums)
+    const int place = row < p.rows ? __ldcg(p.slot128 + row) : -1;
+    const int id = place >= 0 ? __ldcg(p.list128 + row / kTile * kTile + place) : -1;
     const float scale = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.0f;
     tc::wait_for_dependency();
     const int tile = (int)(row / kShrinkRows), block0 = id >= 0 ? __ldcg(p.first_block + tile) : 0, block1 = id >= 0 ? __ldcg(p.last_block + tile) : -1;
@@ -658,8 +664,9 @@ constexpr int kExpandThreads = 128 + kEpiGroups * 128;  // warp 0: y's tiles, 1:
 
 // Persistent CTAs take equal runs of (tile, column step) items; a step is kU units of 64 columns.  The MMA of 128 rows
 // costs 128 clocks however few columns it has, and reads its 128 rows of the image from shared memory each time, so steps
-// have two units (16384 x 8192, rank 128: 150 us; one unit 229 us, four units, whose tiles leave no room to fetch y ahead, 195)
-// unless that leaves SMs without an item.
+// have two units unless that leaves SMs without an item (the whole call for 16384 x 8192, rank 128: 204 us, with one unit
+// 235; 4608 x 12288, rank 64: 76 and 80).  Three or four units leave no room to fetch y ahead.  With the vectors in tensor
+// memory instead, put there by the epilogue warps, there is room, but a tile begins later: 207 and 81 us.
 template <typename T, int kU>
 __global__ void __launch_bounds__(kExpandThreads, 1)
 lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y,
@@ -937,8 +944,8 @@ int sm_count() {
 
 // Whether a call takes the kernel with a cluster per row.  Its time goes with rows x rank x (K + N), the adapters' elements
 // that it reads from L2 (32 us at 67 M elements), that of the tiled kernels with the number of adapters that meet in a tile,
-// which only the device knows: 64 rows of 16 adapters, rank 32, 4096 -> 14336: 17 us against 67 (one adapter: 22); 128
-// rows 32 against 80 (24); 512 rows, rank 16, 4096 -> 4096: 36 against 99 (26).
+// which only the device knows: 64 rows of 16 adapters, rank 32, 4096 -> 14336: 17 us against 64 (one adapter: 20); 128
+// rows 32 against 74 (21); 512 rows, rank 16, 4096 -> 4096: 37 against 91 (21).
 bool few_rows(int64_t rows, int64_t K, int64_t N, int64_t R) { return rows <= 512 && rows * R * (K + N) <= 80000000; }
 
 // What keeps tile coordinates, grids and the number of K steps within 32 bits.

@@ -448,6 +448,13 @@ def test_lora_strides_and_batches(ck, rows):
     _check_lora(ck.lora_add(y3, shared, a, b, each).reshape(rows, n), y3.reshape(rows, n), shared.reshape(rows, k), a, b, flat, None)
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 312576), (1, 312576, 64), (2, 64, 160000)])
+def test_lora_few_rows_of_many_columns(ck, rows, k, n):
+    """So many columns that the tiled kernels take a single row."""
+    x, y, a, b, ids, scales = _lora_case(rows, k, n, 256, 2, BF16, 77, "one")
+    _check_lora(ck.lora_add(y, x, a, b, ids, scales), y, x, a, b, ids, scales)
+
+
 def test_lora_of_nothing(ck):
     e = torch.empty(0, 64, device="cuda", dtype=BF16)
     a, b = torch.zeros(1, 8, 64, device="cuda", dtype=BF16), torch.zeros(1, 32, 8, device="cuda", dtype=BF16)

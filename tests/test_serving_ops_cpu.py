@@ -96,6 +96,10 @@ def test_no_gradient_is_dropped_in_silence():
         backend.add_rmsnorm_quantize_mxfp8(leaf(2, 64), torch.zeros(2, 64, dtype=BF16))
     with pytest.raises(RuntimeError, match="no backward"):
         backend.apply_rope_axes1(leaf(1, 1, 2, 8), torch.zeros(2, 1), torch.zeros(4, dtype=torch.float64), (8,))
+    with pytest.raises(RuntimeError, match="no backward"):     # (nor is a leaf written to)
+        backend.lora_add(**_lora(out=leaf(3, 16)))
+    with pytest.raises(RuntimeError, match="no backward"):
+        backend.add_rmsnorm_quantize_mxfp8(torch.zeros(2, 64, dtype=BF16), torch.zeros(2, 64, dtype=BF16), sum_out=leaf(2, 64))
 
 
 def test_cpu_tensors_find_no_backend():
@@ -159,7 +163,7 @@ def test_native_rope_refusals():
         _refused("launch_apply_rope_axes_kernel", q, k, pos, f, oq, ok, st, b, n, hq, hk, d, pairs, len(axes) if count is None else count, t, pt, False, False, False, None)
 
     for bad in (dict(q=0), dict(pos=0), dict(f=0), dict(oq=0), dict(k=P), dict(k=P, ok=P), dict(hk=1), dict(b=0), dict(n=0), dict(hq=0), dict(hq=70000), dict(d=7),
-                dict(axes=(5,)), dict(axes=(0,)), dict(axes=(2, 3)), dict(count=0), dict(axes=(1,) * 9, d=32), dict(t=5), dict(pt=4), dict(pt=-1), dict(b=1 << 20), dict(n=1 << 60, d=64)):
+                dict(axes=(5,)), dict(axes=(0,)), dict(axes=(2, 3)), dict(count=0), dict(axes=(1,) * 9, d=32), dict(t=5), dict(pt=4), dict(pt=-1), dict(b=1 << 20), dict(n=1 << 60, d=64), dict(b=512, n=1 << 40, d=65536)):
         call(**bad)
 
 
