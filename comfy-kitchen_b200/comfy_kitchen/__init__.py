@@ -55,7 +55,8 @@ class _Ops:
         if torch._C._len_torch_function_stack() > 0:
             return False
         for a in args:
-            if isinstance(a, torch.Tensor) and type(a) is not torch.Tensor and type(a) is not torch.nn.Parameter:
+            kind = type(a)
+            if kind is not torch.Tensor and kind is not torch.nn.Parameter and isinstance(a, torch.Tensor):
                 return False
         return True
 

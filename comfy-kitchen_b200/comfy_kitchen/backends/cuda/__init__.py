@@ -617,34 +617,33 @@ def _same_device(what: str, device, *tensors) -> None:
 def _launch(device, name: str, *args) -> None:
     """_native.call with ``device`` current, on its current stream (appended as the last argument)."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():   # (torch.cuda.current_device without its look at whether CUDA is up)
         _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
             _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
-    """t as [rows, width] with unit column stride, rows apart by at least their width; a copy where it has no such view."""
+def _rows(t: torch.Tensor, width: int):
+    """t as rows of `width` elements with unit column stride -> (the tensor that holds them, elements from row to row); a copy
+    where it has no such view.  Of a contiguous tensor only the address matters."""
+    if t.is_contiguous():
+        return t, width
     if t.dim() != 2:
         try:
             t = t.view(-1, width)
         except RuntimeError:
-            return t.reshape(-1, width).contiguous()
-    if not t.is_contiguous() and (t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width)):
-        t = t.contiguous()
-    return t
-
-
-def _row_stride(t: torch.Tensor, width: int) -> int:
-    return t.stride(0) if t.shape[0] > 1 else width
+            return t.reshape(-1, width).contiguous(), width
+    rows, (apart, step) = t.shape[0], t.stride()
+    if step != 1 or (rows > 1 and apart < width):
+        return t.contiguous(), width
+    return t, apart if rows > 1 else width
 
 
 def _empty(like: torch.Tensor, shape, dtype) -> torch.Tensor:
     """A contiguous tensor on ``like``'s device; torch.empty_like is the cheapest way to one where it fits (1.4 against 2.6 us)."""
-    if shape is like.shape or shape == like.shape:
-        if like.is_contiguous():
-            return torch.empty_like(like) if dtype == like.dtype else torch.empty_like(like, dtype=dtype)
+    if shape == like.shape and like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
     return like.new_empty(shape, dtype=dtype)
 
 
@@ -678,10 +677,10 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
         cols = (d // 32 + 3) // 4 * 4
         sx = torch.empty_strided(((n + 127) // 128 * 128, cols), (cols, 1), dtype=torch.float8_e8m0fnu, device=device)
     if n:
-        xf, rf = _rows_of(x, d), _rows_of(residual, d)
+        (xf, x_stride), (rf, r_stride) = _rows(x, d), _rows(residual, d)
         _launch(device, "launch_add_rmsnorm_quantize_kernel", xf.data_ptr(), rf.data_ptr(), 0 if weight is None else weight.data_ptr(),
                 0 if mx else scale.data_ptr(), sum_out.data_ptr(), norm.data_ptr() if return_norm else 0, q.data_ptr(),
-                sx.data_ptr() if mx else 0, n, d, _row_stride(xf, d), _row_stride(rf, d), eps, _code(dtype, what),
+                sx.data_ptr() if mx else 0, n, d, x_stride, r_stride, eps, _code(dtype, what),
                 _code(stream_dtype, what), DTYPE_TO_CODE[output_type])
     return q, sx, sum_out, norm
 
@@ -846,12 +845,11 @@ def lora_add(
     rows = x.numel() // k
     if rows == 0:
         return out
-    if device.index is not None and device.index != torch.cuda.current_device():   # (the scratch's size goes by the device)
+    if device.index is not None and device.index != torch._C._cuda_getDevice():   # (the scratch's size goes by the device)
         with torch.cuda.device(device):
             return lora_add(y, x, a, b, adapter_ids, scales, out)
     # the kernels move 16 bytes at a time
-    xf, yf, of = _rows_of(x, k), _rows_of(y, n), _rows_of(out, n)
-    x_stride, y_stride, o_stride = _row_stride(xf, k), _row_stride(yf, n), _row_stride(of, n)
+    (xf, x_stride), (yf, y_stride), (of, o_stride) = _rows(x, k), _rows(y, n), _rows(out, n)
     px, py, po, pa, pb = xf.data_ptr(), yf.data_ptr(), of.data_ptr(), a.data_ptr(), b.data_ptr()
     if po != out.data_ptr() or po % 16 or o_stride % 8:
         raise ValueError(f"{what}: out must have unit column stride, rows of one stride and 16-byte alignment")

@@ -117,7 +117,7 @@ _OK = ValidationResult.ok()
 
 def validate_param(name: str, value, constraint: ParamConstraint, default_devices: frozenset) -> ValidationResult:
     if value is None:
-        return ValidationResult.ok()
+        return _OK
     if type(value) is torch.Tensor and constraint.devices is None and (
             constraint.dtypes is None or value.dtype in constraint.dtypes) and value.device.type in default_devices:
         for rule in constraint.shape_rules:
@@ -152,4 +152,4 @@ def validate_function_call(constraints: FunctionConstraints, kwargs: Mapping,
         res = validate_param(pname, kwargs.get(pname), pc, constraints.default_devices)
         if not res.success:
             return res
-    return ValidationResult.ok()
+    return _OK
