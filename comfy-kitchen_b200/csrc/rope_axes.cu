@@ -74,10 +74,19 @@ __device__ __forceinline__ void head_at(const RopeAxesParams& p, int64_t b, int6
     dst = static_cast<T*>(p.o[which]) + b * p.so[which][0] + n * p.so[which][1] + h * p.so[which][2];
 }
 
-// Two pairs at a time with sm_100's packed fp32 instructions: (a0, a1) cos - (b0, b1) sin and (a0, a1) sin + (b0, b1) cos.
+// Two pairs: (a0, a1) cos - (b0, b1) sin and (a0, a1) sin + (b0, b1) cos; 16-bit types with sm_100's packed fp32 instructions.
+// (fp32 has half as many elements a byte and instructions to spare; packed it took 20.2 us for 3 x 1377 x 25 heads of 80, not 17.3.)
+template <typename T>
 __device__ __forceinline__ void rotate2(float2 c, float2 s, float2& a, float2& b) {
-    const float2 oa = __ffma2_rn(b, make_float2(-s.x, -s.y), __fmul2_rn(a, c));
-    b = __ffma2_rn(b, c, __fmul2_rn(a, s));
+    float2 oa;
+    if (sizeof(T) == 4) {
+        const float2 ia = a, ib = b;
+        rotate(make_float2(c.x, s.x), ia.x, ib.x, oa.x, b.x);
+        rotate(make_float2(c.y, s.y), ia.y, ib.y, oa.y, b.y);
+    } else {
+        oa = __ffma2_rn(b, make_float2(-s.x, -s.y), __fmul2_rn(a, c));
+        b = __ffma2_rn(b, c, __fmul2_rn(a, s));
+    }
     a = oa;
 }
 
@@ -133,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const RopeAxesP
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float2 e = make_float2(x[2 * i], x[2 * i + 1]), f = make_float2(y[2 * i], y[2 * i + 1]);
-                        rotate2(c[i], s[i], e, f);
+                        rotate2<T>(c[i], s[i], e, f);
                         x[2 * i] = e.x; x[2 * i + 1] = e.y;
                         y[2 * i] = f.x; y[2 * i + 1] = f.y;
                     }
@@ -145,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const RopeAxesP
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float2 e = make_float2(x[4 * i], x[4 * i + 2]), f = make_float2(x[4 * i + 1], x[4 * i + 3]);
-                        rotate2(c[i], s[i], e, f);
+                        rotate2<T>(c[i], s[i], e, f);
                         if (whole || v * 4 + 2 * i < p.P) { x[4 * i] = e.x; x[4 * i + 1] = f.x; }
                         if (whole || v * 4 + 2 * i + 1 < p.P) { x[4 * i + 2] = e.y; x[4 * i + 3] = f.y; }
                     }
@@ -211,7 +220,7 @@ int launch(RopeAxesParams p, bool split, bool vec, cudaStream_t stream) {
     const int heads = p.heads[0] + p.heads[1];
     // A thread walks at most 16 heads: enough to make the sines cheap, few enough for the last CTAs to end together
     // (25037 tokens x 80 heads: 159 us; 80 heads a thread 177, 10 heads 173), and fewer while an SM has less than 768
-    // threads (3 x 1377 x 25: 16.9 us with 5 heads a thread, 22.2 with all; one token: 4.1 us with one, 4.9 with four).
+    // threads (3 x 1377 x 25: 17 us with 5 heads a thread, 22.2 with all; one token: 4.1 us with one, 4.9 with four).
     const int64_t gx = ceil_div(p.tokens * p.n_vec, kThreads);
     if (gx > 0x7fffffff) CK_FAIL(CK_ERR_SHAPE, "apply_rope_axes: %lld tokens are more than a grid holds", (long long)p.tokens);
     const int64_t sites = p.batch * p.tokens * p.n_vec;
