@@ -118,13 +118,6 @@ _OK = ValidationResult.ok()
 def validate_param(name: str, value, constraint: ParamConstraint, default_devices: frozenset) -> ValidationResult:
     if value is None:
         return _OK
-    if type(value) is torch.Tensor and constraint.devices is None and (
-            constraint.dtypes is None or value.dtype in constraint.dtypes) and value.device.type in default_devices:
-        for rule in constraint.shape_rules:
-            if not rule.check(value):
-                break
-        else:
-            return _OK   # the common case in one look
     if not constraint.check_dtype(value):
         shown = value.dtype if isinstance(value, torch.Tensor) else value
         return ValidationResult.fail(name, f"dtype {shown} not in {set(constraint.dtypes)}")
@@ -148,8 +141,18 @@ def validate_function_call(constraints: FunctionConstraints, kwargs: Mapping,
         if tuple(compute_capability) < tuple(need):
             have = ".".join(map(str, compute_capability))
             return ValidationResult.fail("__hardware__", f"compute capability {have} < required {need[0]}.{need[1]}")
+    devices = constraints.default_devices
     for pname, pc in constraints.params.items():
-        res = validate_param(pname, kwargs.get(pname), pc, constraints.default_devices)
+        value = kwargs.get(pname)
+        if value is None:
+            continue
+        if type(value) is torch.Tensor and pc.devices is None and (pc.dtypes is None or value.dtype in pc.dtypes) and value.device.type in devices:
+            for rule in pc.shape_rules:
+                if not rule.check(value):
+                    break
+            else:
+                continue   # the common case in one look
+        res = validate_param(pname, value, pc, devices)
         if not res.success:
             return res
     return _OK

@@ -27,6 +27,10 @@ logger = logging.getLogger("comfy_kitchen.dispatch")
 KNOWN_BACKENDS = ("cuda", "triton", "eager")  # names the reference reports in list_backends()
 
 
+class _PerThread(threading.local):
+    backend_override = None
+
+
 class BackendRegistry:
     def __init__(self):
         self._backends: dict[str, Any] = {}
@@ -36,7 +40,7 @@ class BackendRegistry:
         self._disabled: set[str] = set()
         self._unavailable: dict[str, str] = {}
         self._lock = threading.Lock()
-        self._tls = threading.local()
+        self._tls = _PerThread()
         self._cc: tuple[int, int] | None | bool = False  # False = not looked up yet
 
     # ------------------------------------------------------------------ hardware
@@ -122,7 +126,7 @@ class BackendRegistry:
         return True
 
     def get_capable_backend(self, func_name: str, kwargs: Mapping[str, Any] | None = None) -> str:
-        override = getattr(self._tls, "backend_override", None)
+        override = self._tls.backend_override
         if override is None:   # the usual call: the first backend of the list that takes it, without keeping a record of why others do not
             for name in self._priority:
                 if name in self._backends and name not in self._disabled and func_name in self._capabilities.get(name, ()):
@@ -163,7 +167,7 @@ class BackendRegistry:
             if backend_name in self._unavailable:
                 raise BackendNotFoundError(backend_name, self._unavailable[backend_name])
             raise BackendNotFoundError(backend_name, "disabled" if backend_name in self._disabled else "not registered")
-        previous = getattr(self._tls, "backend_override", None)
+        previous = self._tls.backend_override
         self._tls.backend_override = backend_name
         try:
             yield
