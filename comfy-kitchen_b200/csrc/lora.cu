@@ -17,8 +17,8 @@
 // rows and keeps a row's own (a row of another request never enters a sum, whatever it holds).  Requests that lie behind
 // one another cost nothing extra; a tile of 128 different adapters reads 128 adapters, as it must.
 //
-// Measured, back to back: 16384 rows, 8192 -> 8192, rank 128, 8 requests: 204 us (64 % of the copy rate; 193 us in a short burst, of
-// which count 5, shrink 65, join 9, expand 100); 4608 rows, 4096 -> 12288, rank 64, 7 requests: 76 us (54 %), of which about 20 are
+// Measured, back to back: 16384 rows, 8192 -> 8192, rank 128, 8 requests: 204 us (64 % of the copy rate; 186 in a short burst:
+// the first product at 8, x done at 71, the sums joined at 81, the first output at 87); 4608 rows, 4096 -> 12288, rank 64, 7 requests: 76 us (54 %), of which about 20 are
 // the four kernels' beginnings and ends; one row 4.2 us, 64 rows of 16 adapters 16.7 us on the device.
 //
 // Rounding: sums in fp32.  The low-rank vector is the second product's 16-bit operand: it goes in as two parts, the
