@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from comfy_kitchen import _native
 from comfy_kitchen.backends._modulation import adaln_prep_modulation
@@ -601,11 +602,16 @@ def rmsnorm_quantize_nvfp4(
 
 
 def _no_grad(what: str, *tensors) -> None:
-    """These entry points record no gradient; a call that would drop one is refused."""
+    """These entry points record no gradient; a call that would drop one is refused.  Asked of the tensors as the caller gave
+    them: a parameter that _plain() has seen wants none any more."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:   # inside forward_ad.dual_level(), where torch.no_grad() does not apply
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: call it with forward_ad.unpack_dual(t).primal")
 
 
 def _same_device(what: str, device, *tensors) -> None:
@@ -648,6 +654,7 @@ def _empty(like: torch.Tensor, shape, dtype) -> torch.Tensor:
 
 
 def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm, sum_out):
+    _no_grad(what, x, residual, weight, sum_out)
     x, residual = _plain(x), _plain(residual)
     shape, dtype, device, stream_dtype = x.shape, x.dtype, x.device, residual.dtype
     if shape != residual.shape or not shape:
@@ -664,7 +671,6 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
             raise ValueError(f"{what}: weight must be [{d}], got {list(weight.shape)}")
         if weight.dtype != dtype or not weight.is_contiguous():
             weight = weight.to(dtype).contiguous()
-    _no_grad(what, x, residual, weight, sum_out)
     _same_device(what, device, residual, weight, sum_out)
     if sum_out is None:
         sum_out = _empty(residual, shape, stream_dtype)
@@ -706,6 +712,8 @@ def add_rmsnorm_quantize_fp8(
     """The same with quantize_per_tensor_fp8(normalised h, scale, output_type): -> (data in x's shape, h[, normalised h])."""
     if output_type not in (torch.float8_e4m3fn, torch.float8_e5m2):
         raise ValueError(f"Unsupported output_type: {output_type}. Expected torch.float8_e4m3fn or torch.float8_e5m2")
+    if isinstance(scale, torch.Tensor):
+        _no_grad("add_rmsnorm_quantize_fp8", scale)
     scale = _scalar_on(scale, x.device)
     if scale.numel() != 1:
         raise ValueError("add_rmsnorm_quantize_fp8: scale must be a scalar tensor")
@@ -728,6 +736,7 @@ _POSITION_CODES = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int
 
 
 def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim, inverse):
+    _no_grad(what, xq, xk, positions, freqs)
     xq = _plain(xq)
     if tokens_dim != 1 and tokens_dim != 2:
         raise ValueError(f"{what}: tokens_dim is 2 for [B, H, N, D] or 1 for [B, N, H, D], got {tokens_dim}")
@@ -758,7 +767,6 @@ def _rope_axes(what, xq, xk, positions, freqs, axes_dim, split_half, tokens_dim,
     code = _POSITION_CODES.get(positions.dtype)
     if code is None:
         raise ValueError(f"{what}: positions must be float32, float64, int32 or int64")
-    _no_grad(what, xq, xk, positions, freqs)
     _same_device(what, device, xk, positions, freqs)
     oq = _empty(xq, q_shape, dtype)
     ok = None if xk is None else _empty(xk, k_shape, dtype)
@@ -814,6 +822,7 @@ def lora_add(
     ``out``: where to write, in y's shape; may be y itself.  K, N and R are multiples of 8, R at most 256.
     """
     what = "lora_add"
+    _no_grad(what, y, x, a, b, scales, out)
     y, x, a, b = _plain(y), _plain(x), _plain(a), _plain(b)
     x_shape, y_shape, a_shape, b_shape, dtype, device = x.shape, y.shape, a.shape, b.shape, x.dtype, x.device
     if len(a_shape) != 3 or len(b_shape) != 3 or not x_shape:
@@ -836,7 +845,6 @@ def lora_add(
         raise ValueError(f"{what}: adapter_ids {list(ids_shape)} must have the shape of x's leading dimensions {list(x_shape[:-1])} or of the first of them")
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,)):
         raise ValueError(f"{what}: scales must be float32 [{adapters}]")
-    _no_grad(what, y, x, a, b, scales, out)
     _same_device(what, device, y, a, b, adapter_ids, scales, out)
     if out is None:
         out = _empty(y, y_shape, dtype)
