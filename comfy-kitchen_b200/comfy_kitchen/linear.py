@@ -20,12 +20,25 @@ import logging
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 import comfy_kitchen
 from comfy_kitchen.sharding import shard_linear_state
 from comfy_kitchen.tensor import QuantizedTensor, TensorCoreNVFP4Layout
 
 logger = logging.getLogger(__name__)
+
+
+class _Onto(torch.autograd.Function):
+    """``out`` = y + what carries no gradient: its gradient is y's."""
+
+    @staticmethod
+    def forward(ctx, y, out):
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad, None
 
 
 class _WithAdapters(nn.Module):
@@ -55,7 +68,10 @@ class _WithAdapters(nn.Module):
             raise ValueError("adapter_ids given to a layer without adapters: call set_adapters first")
         if isinstance(x, QuantizedTensor):
             raise ValueError("the adapters read the layer's input unquantized: pass a plain tensor")
-        return comfy_kitchen.lora_add(y, x, self.adapter_a, self.adapter_b, adapter_ids, self.adapter_scales)
+        # the projection wants a gradient where the bias does; adapters leave that one as it is, and x's is refused
+        passed_on = torch.is_grad_enabled() and y.requires_grad and forward_ad._current_level < 0
+        out = comfy_kitchen.lora_add(y.detach() if passed_on else y, x, self.adapter_a, self.adapter_b, adapter_ids, self.adapter_scales)
+        return _Onto.apply(y, out) if passed_on else out
 
 
 class NVFP4Linear(_WithAdapters):

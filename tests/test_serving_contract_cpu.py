@@ -3,6 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import comfy_kitchen as ck
 from comfy_kitchen.backends import cuda as backend
 
 BF16 = torch.bfloat16
@@ -55,3 +56,49 @@ def test_dual_level_takes_what_has_no_tangent():
         with pytest.raises(Exception) as e:
             entry(**args)
     assert "forward-mode" not in str(e.value) and "backward" not in str(e.value)
+
+
+# ---- a layer with adapters
+
+
+def _plain_lora(y, x, a, b, adapter_ids, scales=None):
+    """lora_add on the CPU, with its question about gradients."""
+    backend._no_grad("lora_add", y, x, a, b, scales)
+    f = torch.ones(a.shape[0]) if scales is None else scales
+    more = [f[i] * (x[t].double() @ a[i].double().T) @ b[i].double().T for t, i in enumerate(adapter_ids.tolist())]
+    return (y.double() + torch.stack(more)).to(y.dtype)
+
+
+@pytest.fixture
+def layer(monkeypatch):
+    """An NVFP4Linear as it is built by default, with a plain weight in the quantized one's place and its adapters."""
+    from comfy_kitchen.linear import NVFP4Linear, QuantizedTensor
+
+    monkeypatch.setattr(QuantizedTensor, "from_float", staticmethod(lambda x, *args, **kwargs: x))
+    monkeypatch.setattr(ck, "lora_add", _plain_lora)
+    g = torch.Generator().manual_seed(1)
+    layer = NVFP4Linear(24, 16)
+    layer.weight = torch.nn.Parameter(torch.randn(16, 24, generator=g).to(BF16), requires_grad=False)
+    layer.bias.data.normal_(generator=g)
+    layer.set_adapters(torch.randn(2, 8, 24, generator=g).to(BF16), torch.randn(2, 16, 8, generator=g).to(BF16))
+    return layer
+
+
+def test_layer_with_its_default_bias_takes_adapters(layer):
+    """The bias wants a gradient, so the projection does: it passes through the adapters' sum as it is."""
+    g = torch.Generator().manual_seed(2)
+    x, ids, grad = torch.randn(3, 24, generator=g).to(BF16), torch.tensor([1, 0, 1]), torch.randn(3, 16, generator=g).to(BF16)
+    base = layer(x)
+    assert base.requires_grad
+    got = layer(x, ids)
+    assert torch.equal(got, _plain_lora(base.detach(), x, layer.adapter_a, layer.adapter_b, ids))
+    want, = torch.autograd.grad(base, layer.bias, grad)
+    have, = torch.autograd.grad(got, layer.bias, grad)
+    assert torch.equal(have, want)
+    with torch.no_grad():
+        assert torch.equal(layer(x, ids), got) and not layer(x, ids).requires_grad
+
+
+def test_layer_does_not_drop_the_input_gradient(layer):
+    with pytest.raises(RuntimeError, match="no backward"):
+        layer(torch.zeros(1, 24, dtype=BF16, requires_grad=True), torch.tensor([1]))
