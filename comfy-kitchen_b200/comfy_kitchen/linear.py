@@ -50,8 +50,9 @@ class _WithAdapters(nn.Module):
 
     def set_adapters(self, a: torch.Tensor | None, b: torch.Tensor | None = None, scales: torch.Tensor | None = None) -> None:
         """a: [L, R, in_features], b: [L, out_features, R] (a tensor-parallel layer's shard of them), scales: float32 [L] or
-        None for ones; ``set_adapters(None)`` takes them off.  They move with the module; a cast of the module to another
-        dtype takes the scales along, so set them again behind one."""
+        None for ones; ``set_adapters(None)`` takes them off.  They are kept
+        detached and move with the module; a cast of the module to another dtype takes the scales along, so set them again
+        behind one."""
         if a is None:
             self.adapter_a = self.adapter_b = self.adapter_scales = None
             return
@@ -59,7 +60,8 @@ class _WithAdapters(nn.Module):
             raise ValueError("adapters are a [L, R, in_features] and b [L, out_features, R] of one dtype")
         if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (a.shape[0],)):
             raise ValueError(f"scales must be float32 [{a.shape[0]}]")
-        self.adapter_a, self.adapter_b, self.adapter_scales = a.detach().contiguous(), b.detach().contiguous(), scales
+        self.adapter_a, self.adapter_b = a.detach().contiguous(), b.detach().contiguous()
+        self.adapter_scales = None if scales is None else scales.detach()
 
     def _add_adapters(self, y: torch.Tensor, x: torch.Tensor, adapter_ids: torch.Tensor | None) -> torch.Tensor:
         if adapter_ids is None:

@@ -102,3 +102,14 @@ def test_layer_with_its_default_bias_takes_adapters(layer):
 def test_layer_does_not_drop_the_input_gradient(layer):
     with pytest.raises(RuntimeError, match="no backward"):
         layer(torch.zeros(1, 24, dtype=BF16, requires_grad=True), torch.tensor([1]))
+
+
+def test_adapters_given_as_parameters_stay_out_of_the_state(layer):
+    """Scales as well as a and b: buffers that no state dict or optimizer sees."""
+    layer.set_adapters(torch.nn.Parameter(_zeros(2, 8, 24)), torch.nn.Parameter(_zeros(2, 16, 8)), torch.nn.Parameter(torch.ones(2)))
+    assert sorted(n for n, _ in layer.named_parameters()) == ["bias", "weight"]
+    assert not any("adapter" in k for k in torch.nn.Module.state_dict(layer))
+    assert not any(t.requires_grad for t in (layer.adapter_a, layer.adapter_b, layer.adapter_scales))
+    assert layer(_zeros(1, 24), torch.tensor([1])).shape == (1, 16)
+    layer.set_adapters(None)
+    assert layer.adapter_scales is None
