@@ -170,16 +170,13 @@ __device__ __forceinline__ void encode_chunk(const AddNormArgs& a, int64_t row, 
         word |= __shfl_xor_sync(0xffffffffu, word, 4);
         if ((lane & 7) == 0 && (chunk >> 1) < a.sf_cpad) *reinterpret_cast<uint32_t*>(a.sf + sf_row + (chunk >> 3) * 512) = word;
     } else {
-        const float most = a.e5m2 ? 57344.0f : 448.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) {   // (the conversions saturate; NaN stays NaN)
             float t[4];
             const float2 f = y.get(2 * j), g = y.get(2 * j + 1);
             t[0] = __fmul_rn(f.x, inv); t[1] = __fmul_rn(f.y, inv); t[2] = __fmul_rn(g.x, inv); t[3] = __fmul_rn(g.y, inv);
             Elem<T>::round2(t[0], t[1]);
             Elem<T>::round2(t[2], t[3]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) t[k] = fminf(fmaxf(t[k], -most), most);
             w[j] = a.e5m2 ? cvt_e5m2x2(t[1], t[0]) | (cvt_e5m2x2(t[3], t[2]) << 16) : cvt_e4m3x2(t[1], t[0]) | (cvt_e4m3x2(t[3], t[2]) << 16);
         }
     }

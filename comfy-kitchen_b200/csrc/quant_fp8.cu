@@ -2,7 +2,8 @@
 //
 // quantize (comfy_kitchen/backends/eager/quantization.py:43-57):
 //   inv = (1/scale) rounded to x's dtype;  t = x*inv rounded to x's dtype;
-//   out = fp8_rne(clamp(t, +-max))           (max 448 for E4M3, 57344 for E5M2)
+//   out = fp8_rne(clamp(t, +-max))           (max 448 for E4M3, 57344 for E5M2; a NaN stays one)
+// The conversion saturates by itself and keeps NaN; a clamp by fminf / fmaxf before it would turn NaN into -max.
 // The product of two bf16 (or two fp16) values is exact in fp32, so rounding the
 // fp32 product once to the narrow type reproduces the reference's 16-bit
 // multiply bit for bit.  (A true x/scale in fp32 does not: about 3 % of codes
@@ -27,14 +28,11 @@ __device__ __forceinline__ uint32_t to_fp8x2(float hi, float lo) {
 
 template <typename T, bool kE4M3>
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inv) {
-    constexpr float kMax = kE4M3 ? 448.0f : 57344.0f;
     uint32_t w[2] = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float a = Elem<T>::round(__fmul_rn(v[2 * i], inv));
-        float b = Elem<T>::round(__fmul_rn(v[2 * i + 1], inv));
-        a = fminf(fmaxf(a, -kMax), kMax);
-        b = fminf(fmaxf(b, -kMax), kMax);
+        const float a = Elem<T>::round(__fmul_rn(v[2 * i], inv));
+        const float b = Elem<T>::round(__fmul_rn(v[2 * i + 1], inv));
         w[i >> 1] |= to_fp8x2<kE4M3>(b, a) << (16 * (i & 1));
     }
     return make_uint2(w[0], w[1]);
@@ -44,7 +42,6 @@ template <typename T, bool kE4M3>
 __global__ void __launch_bounds__(kThreads)
 quantize_fp8_kernel(const T* __restrict__ x, const float* __restrict__ scale, uint8_t* __restrict__ out, int64_t numel,
                     bool vec_ok) {
-    constexpr float kMax = kE4M3 ? 448.0f : 57344.0f;
     const float inv = Elem<T>::round(__fdiv_rn(1.0f, __ldg(scale)));
     const int64_t full = vec_ok ? (numel / kChunk) * kChunk : 0;
     for (int64_t base = (int64_t)blockIdx.x * kChunk; base < full; base += (int64_t)gridDim.x * kChunk) {
@@ -57,8 +54,7 @@ quantize_fp8_kernel(const T* __restrict__ x, const float* __restrict__ scale, ui
     }
     // tail (and the whole tensor when the pointers are not 16-byte aligned)
     for (int64_t i = full + (int64_t)blockIdx.x * kThreads + threadIdx.x; i < numel; i += (int64_t)gridDim.x * kThreads) {
-        float t = Elem<T>::round(__fmul_rn(Elem<T>::to_f32(x[i]), inv));
-        t = fminf(fmaxf(t, -kMax), kMax);
+        const float t = Elem<T>::round(__fmul_rn(Elem<T>::to_f32(x[i]), inv));
         out[i] = (uint8_t)(to_fp8x2<kE4M3>(0.0f, t) & 0xffu);
     }
 }

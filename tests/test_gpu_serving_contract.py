@@ -58,3 +58,45 @@ def test_layers_with_a_bias_take_adapters(ck):
             assert torch.equal(have, want)
         with torch.no_grad():
             assert torch.equal(layer(x, ids), got.detach())
+
+
+# ------------------------------------------------------------------ per-tensor FP8: infinities and NaN
+
+
+def _fp8_ref(x, scale, out):
+    """The definition on the CPU: a product rounded to x's type, clamped (NaN stays), rounded to 8 bits."""
+    x, most = x.cpu(), torch.finfo(out).max
+    inverse = (1.0 / scale.cpu()).to(x.dtype)
+    return (x.float() * inverse.float()).to(x.dtype).float().clamp(-most, most).to(out)
+
+
+def _same_codes(got, want):
+    got, want = got.cpu(), want.cpu()
+    nan = want.float().isnan()
+    assert torch.equal(got.float().isnan(), nan)
+    assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("scale", [1.0, 0.37, 1e-30, float("nan"), float("inf"), 0.0])
+def test_fp8_quantizer_on_every_number_of_a_type(ck, dtype, out, scale):
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype).cuda()
+    scale = torch.tensor([scale], device="cuda")
+    _same_codes(ck.quantize_per_tensor_fp8(x, scale, out), _fp8_ref(x, scale, out))
+    odd = x[1:4099]                                                        # not aligned, no whole chunks
+    _same_codes(ck.quantize_per_tensor_fp8(odd, scale, out), _fp8_ref(odd, scale, out))
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("dtype,stream,width", [(BF16, BF16, 4096), (FP16, FP32, 96), (FP32, FP32, 33), (BF16, FP32, 20000)])
+def test_norm_fp8_keeps_infinities_and_nan(ck, dtype, stream, width, out):
+    g = _gen(width)
+    x, res, w = _randn(g, 6, width, dtype=dtype), _randn(g, 6, width, dtype=stream), _randn(g, width, dtype=dtype)
+    x[1, 3], x[2], x[4, 0], x[4, 1] = float("nan"), float("inf"), float("inf"), -float("inf")
+    for scale in (0.013, 1e-4):                                            # (the second one saturates)
+        scale = torch.tensor([scale], device="cuda")
+        q, h, y = ck.add_rmsnorm_quantize_fp8(x, res, w, scale, 1e-6, out, return_norm=True)
+        assert bool(y[1].isnan().all()) and bool(q[1].float().isnan().all())
+        _same_codes(q, _fp8_ref(y, scale, out))
+        _same_codes(q, ck.quantize_per_tensor_fp8(y, scale, out))
