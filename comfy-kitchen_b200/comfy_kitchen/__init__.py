@@ -102,7 +102,8 @@ def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: 
                                return_norm: bool = False, sum_out: torch.Tensor | None = None):
     """h = x + residual; ``quantize_mxfp8(rmsnorm(h, weight, eps).reshape(-1, D))`` in one pass.
     -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``residual`` and h
-    have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to, e.g. ``residual`` itself."""
+    have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to; ``residual`` itself (or x, where it has h's dtype),
+    or memory that no input lies in."""
     if sum_out is None and not _Ops._plain((x, residual, weight)):
         got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
         return got if return_norm else got[:-1]
@@ -127,7 +128,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
              scales: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y + scales[i] * (x @ a[i].T) @ b[i].T with i the row's adapter id: the low-rank adapters of many requests beside
     a shared projection y [..., N] of x [..., K].  a: [L, R, K]; b: [L, N, R]; adapter_ids: int32 or int64, one per row
-    or per leading index (outside [0, L): no adapter); ``out`` may be y."""
+    or per leading index (outside [0, L): no adapter); ``out``: y itself, or memory that no input lies in."""
     if out is None and not _Ops._plain((y, x, a, b, adapter_ids, scales)):
         return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
     impl = registry.get_implementation("lora_add", kwargs={"y": y, "x": x, "a": a, "b": b, "adapter_ids": adapter_ids, "scales": scales})

@@ -357,11 +357,22 @@ extern "C" int launch_add_rmsnorm_quantize_kernel(const void* x, const void* res
         CK_FAIL(CK_ERR_SHAPE, "add_rmsnorm_quantize: a residual updated in place is contiguous");
     if (mx && (reinterpret_cast<uintptr_t>(block_scales) & 3)) CK_FAIL(CK_ERR_ALIGN, "add_rmsnorm_quantize: block scales must be 4-byte aligned");
     const int64_t es = dtype_code == CK_F32 ? 4 : 2, rs = residual_dtype_code == CK_F32 ? 4 : 2;
+    // An element is read and written by the same thread, so an output may have x's or the residual's place, but no other.
+    const int64_t wide = mx ? round_up(D / 32, 4) : 0;
+    const Memory in[4] = {{x, N, x_row_stride * es, D * es}, {residual, N, residual_row_stride * rs, D * rs}, memory_of(weight, D * es), memory_of(scale, 4)};
+    const Memory out[4] = {{sum_out, N, D * rs, D * rs}, {norm_out, N, D * es, D * es}, memory_of(output, N * D), memory_of(block_scales, round_up(N, 128) * wide)};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 4; ++j)
+            if (overlap(out[i], in[j]) && !(j < 2 && same_place(out[i], in[j])))
+                CK_FAIL(CK_ERR_UNSUPPORTED, "add_rmsnorm_quantize: an output overlaps an input and has not its place");
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j])) CK_FAIL(CK_ERR_UNSUPPORTED, "add_rmsnorm_quantize: two outputs overlap");
+    }
     const bool vec = D % 16 == 0 && aligned32(x) && aligned32(residual) && aligned32(sum_out) && (!norm_out || aligned32(norm_out)) &&
                      (!weight || aligned32(weight)) && aligned16(output) && (x_row_stride * es) % 32 == 0 &&
                      (residual_row_stride * rs) % 32 == 0;
     AddNormArgs a{x, residual, weight, static_cast<const float*>(scale), sum_out, norm_out, static_cast<uint8_t*>(output),
-                  static_cast<uint8_t*>(block_scales), N, D, x_row_stride, residual_row_stride, mx ? round_up(D / 32, 4) : 0, eps,
+                  static_cast<uint8_t*>(block_scales), N, D, x_row_stride, residual_row_stride, wide, eps,
                   output_dtype_code == CK_E5M2};
     if (dtype_code == CK_F32) return launch_fmt<float, float>(a, mx, vec, stream);
     if (dtype_code == CK_F16)

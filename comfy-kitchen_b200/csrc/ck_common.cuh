@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <numeric>
+
 // dtype codes that cross the C ABI (same numbering as the reference:
 // comfy_kitchen/backends/eager/quantization.py:33-41).
 #define CK_F32 0
@@ -46,6 +48,29 @@ __host__ __device__ inline int64_t ceil_div(int64_t x, int64_t m) { return (x + 
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
+// `rows` runs of `bytes`, `stride` bytes from one to the next (of a single run any stride).
+struct Memory {
+    const void* at;
+    int64_t rows, stride, bytes;
+};
+inline Memory memory_of(const void* at, int64_t bytes) { return Memory{at, 1, 0, bytes}; }
+inline bool same_place(const Memory& a, const Memory& b) {
+    return a.at == b.at && a.rows == b.rows && a.bytes == b.bytes && (a.rows == 1 || a.stride == b.stride);
+}
+// Whether two of them share a byte.  Runs of one buffer that lie between one another (columns of it, every second row) do not;
+// where the spans meet, the runs are compared modulo the strides' common divisor (exact but for runs that would meet only
+// behind an end).
+inline bool overlap(const Memory& a, const Memory& b) {
+    if (!a.at || !b.at) return false;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.at), b0 = reinterpret_cast<uintptr_t>(b.at);
+    const uintptr_t a1 = a0 + (uintptr_t)((a.rows - 1) * a.stride + a.bytes), b1 = b0 + (uintptr_t)((b.rows - 1) * b.stride + b.bytes);
+    if (a1 <= b0 || b1 <= a0) return false;
+    const int64_t apart = std::gcd(a.rows > 1 ? a.stride : 0, b.rows > 1 ? b.stride : 0);
+    if (apart == 0) return true;
+    const int64_t from = b0 >= a0 ? (int64_t)((b0 - a0) % (uintptr_t)apart) : (apart - (int64_t)((a0 - b0) % (uintptr_t)apart)) % apart;
+    return from < a.bytes || from + b.bytes > apart;
+}
 
 // ---------------------------------------------------------------- element types
 

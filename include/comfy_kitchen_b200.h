@@ -174,7 +174,7 @@ int launch_apply_rope_kernel(const void* xq, const void* xk, const void* freqs, 
  * [pairs].  positions_code: 0 float32, 1 float64, 2 int32, 3 int64.  strides (HOST array of 11, in elements): xq batch,
  * token, head, element; xk the same; positions batch, token, axis.  The outputs are contiguous: [batch, tokens, heads,
  * head_dim] with tokens_first, else [batch, heads, tokens, head_dim].  xk / xk_out may both be NULL (heads_k = 0).
- * axis_pairs: HOST array.  inverse: rotate back (the transpose, i.e. the gradient's rotation). */
+ * axis_pairs: HOST array.  The outputs overlap no input.  inverse: rotate back (the transpose, i.e. the gradient's rotation). */
 int launch_apply_rope_axes_kernel(const void* xq, const void* xk, const void* positions, const double* freqs, void* xq_out,
                                   void* xk_out, const int64_t* strides, int64_t batch, int64_t tokens, int64_t heads_q,
                                   int64_t heads_k, int64_t head_dim, const int32_t* axis_pairs, int n_axes, int dtype_code,
@@ -229,7 +229,8 @@ int launch_adaln_quantize_mxfp8_kernel(const void* x, const void* scale, const v
  * output: block_scales given: the bytes of launch_quantize_mxfp8_kernel on y (E4M3, tiled E8M0 scales, padding
  * written; D a multiple of 32), else those of launch_quantize_fp8_kernel on y with the device scalar scale (any D).
  * x [N, D] and residual [N, D] have unit column stride and the given row strides; sum_out, norm_out, output are
- * contiguous; sum_out may be the residual itself if that is contiguous.  residual_dtype_code: x's or fp32; weight [D] in x's
+ * contiguous; an output may have the place of x or of the residual (same address, dtype and strides), any other overlap is
+ * refused (CK_ERR_UNSUPPORTED).  residual_dtype_code: x's or fp32; weight [D] in x's
  * type or NULL. */
 int launch_add_rmsnorm_quantize_kernel(const void* x, const void* residual, const void* weight, const void* scale,
                                        void* sum_out, void* norm_out, void* output, void* block_scales, int64_t N, int64_t D,
@@ -244,7 +245,8 @@ int ck_norm_device_status(void);
  * out[t] = y[t] + scales[a] * B_a (A_a x[t]) for every row, a = ids[t / rows_per_id]; out[t] = y[t] where a lies outside
  * [0, adapters).  y: [rows, N], the shared projection's output; x: [rows, K]; a: [adapters, rank, K]; b: [adapters, N, rank];
  * all bf16 or all fp16, 16-byte aligned, row strides (elements) multiples of 8; ids: int32 or int64; scales: fp32
- * [adapters] or NULL (ones); out may be y.  K, N, rank multiples of 8, rank at most 256.  workspace: scratch of
+ * [adapters] or NULL (ones); out may be y (same address and stride), any other overlap of it with an input is refused
+ * (CK_ERR_UNSUPPORTED).  K, N, rank multiples of 8, rank at most 256.  workspace: scratch of
  * ck_lora_workspace_bytes(), 16-byte aligned, used by this call only until it ends on the stream (need not be set). */
 int launch_lora_add_kernel(const void* y, const void* x, const void* a, const void* b, const void* ids, const float* scales,
                            void* out, void* workspace, int64_t rows, int64_t K, int64_t N, int64_t rank, int64_t adapters,

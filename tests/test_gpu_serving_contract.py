@@ -100,3 +100,56 @@ def test_norm_fp8_keeps_infinities_and_nan(ck, dtype, stream, width, out):
         assert bool(y[1].isnan().all()) and bool(q[1].float().isnan().all())
         _same_codes(q, _fp8_ref(y, scale, out))
         _same_codes(q, ck.quantize_per_tensor_fp8(y, scale, out))
+
+
+# ------------------------------------------------------------------ outputs beside and over inputs
+
+
+@pytest.mark.parametrize("rows", [3, 64, 700])
+def test_lora_out_beside_its_inputs(ck, rows):
+    g = _gen(rows)
+    n = k = 128
+    a, b, ids = _randn(g, 3, 16, k, scale=0.06), _randn(g, 3, n, 16, scale=0.1), torch.arange(rows, device="cuda") % 4
+    buf = _randn(g, rows, 3 * n)
+    y, x, kept = buf[:, :n], buf[:, n:2 * n], buf.clone()
+    want = ck.lora_add(y.clone(), x.clone(), a, b, ids)
+    ck.lora_add(y, x, a, b, ids, out=buf[:, 2 * n:])                       # a third column block of one buffer
+    assert torch.equal(buf[:, 2 * n:], want) and torch.equal(buf[:, :2 * n], kept[:, :2 * n])
+    ck.lora_add(y, x, a, b, ids, out=y)                                    # y's own
+    assert torch.equal(y, want) and torch.equal(x, kept[:, n:2 * n])
+    every = _randn(g, 3 * rows, n)
+    every[0::3], every[1::3] = kept[:, :n], kept[:, n:2 * n]
+    ck.lora_add(every[0::3], every[1::3], a, b, ids, out=every[2::3])      # every third row
+    assert torch.equal(every[2::3], want) and torch.equal(every[0::3], kept[:, :n])
+    rest = _randn(g, rows + 1, n)
+    for yy, xx, out in ((rest[:-1], x, rest[1:]), (rest[1:], x, rest[:-1]), (kept[:, :n], rest[:-1], rest[:-1]), (kept[:, :n], rest[1:], rest[:-1]),
+                        (buf[:, :n], x, buf[:, 64:n + 64])):
+        before = out.clone()
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ck.lora_add(yy, xx, a, b, ids, out=out)
+        assert torch.equal(out, before)
+
+
+@pytest.mark.parametrize("width,dtype,stream", [(4096, BF16, BF16), (96, FP16, FP16), (32, FP32, FP32), (20000, FP32, FP32), (40000, BF16, BF16)])
+def test_norm_sum_over_its_inputs(ck, width, dtype, stream):
+    g = _gen(width)
+    x, res, w = _randn(g, 5, width, dtype=dtype), _randn(g, 5, width, dtype=stream), _randn(g, width, dtype=dtype)
+    want = ck.add_rmsnorm_quantize_mxfp8(x, res, w, return_norm=True)
+    for which in range(2):
+        args = [x.clone(), res.clone()]
+        got = ck.add_rmsnorm_quantize_mxfp8(*args, w, return_norm=True, sum_out=args[which])
+        assert got[2] is args[which] and torch.equal(args[1 - which], (x, res)[1 - which])
+        for u, v in zip(got, want):
+            assert torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+    both = x.to(stream)
+    twice = ck.add_rmsnorm_quantize_mxfp8(both.to(dtype), both, w)[2]
+    same = both.to(dtype)
+    assert torch.equal(ck.add_rmsnorm_quantize_mxfp8(same, same, w, sum_out=same)[2], twice)   # (x, residual and h in one place)
+    long = _randn(g, 6, width, dtype=stream)
+    before = long.clone()
+    for r, s in ((long[:5], long[1:]), (long[1:], long[:5])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ck.add_rmsnorm_quantize_mxfp8(x, r, w, sum_out=s)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ck.add_rmsnorm_quantize_fp8(r, x.to(stream), w, torch.ones(1, device="cuda"), sum_out=s)
+    assert torch.equal(long, before)

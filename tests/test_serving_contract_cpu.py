@@ -4,6 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 import comfy_kitchen as ck
+from comfy_kitchen import _native
 from comfy_kitchen.backends import cuda as backend
 
 BF16 = torch.bfloat16
@@ -113,3 +114,61 @@ def test_adapters_given_as_parameters_stay_out_of_the_state(layer):
     assert layer(_zeros(1, 24), torch.tensor([1])).shape == (1, 16)
     layer.set_adapters(None)
     assert layer.adapter_scales is None
+
+
+# ---- outputs that overlap inputs: asked of the C entry points, where addresses and strides are known (nothing is launched
+# for a refusal, and no pointer is read)
+
+P = 1 << 24
+FAR = 1 << 40    # where the arguments lie that are not in question, each FAR from the next
+
+
+def _status(name, *args):
+    lib = _native.load()
+    return getattr(lib, name)(*args), lib.ck_last_error().decode()
+
+
+def _lora_status(rows=4, y=1, x=2, out=7, ys=16, xs=24, os=16, per=1, **at):
+    """4 rows, 24 -> 16, rank 8, two adapters; a number below 100 stands for a place of its own."""
+    a, b, ids, scales = (at.get(n, i * FAR) for n, i in (("a", 3), ("b", 4), ("ids", 5), ("scales", 6)))
+    place = lambda v: v * FAR if v < 100 else v  # noqa: E731
+    return _status("launch_lora_add_kernel", place(y), place(x), a, b, ids, scales, place(out), 0, rows, 24, 16, 8, 2, ys, xs, os, per, 2, False, None)
+
+
+OVERLAPS = [
+    dict(y=P, out=P + 32),                          # a row on
+    dict(y=P + 32, out=P),
+    dict(y=P, out=P + 16),                          # half a row on
+    dict(y=P, out=P, os=24),                        # the same address, rows further apart
+    dict(y=P, ys=48, out=P + 16, os=48),            # columns that meet, of one buffer
+    dict(x=P, out=P),                               # x is read by CTAs that do not write these columns
+    dict(x=P, out=P + 48),
+    dict(x=P, xs=40, out=P + 32, os=40),
+    dict(a=P, out=P + 2 * 8 * 24 * 2 - 16),         # the end of the adapters
+    dict(b=P, out=P - 16),
+    dict(ids=P + 112, out=P),                       # the last of four rows
+    dict(scales=P + 4, out=P),
+    dict(y=P, ys=64, out=P + 16, os=32),            # rows of two spacings
+]
+
+
+@pytest.mark.parametrize("change", OVERLAPS)
+def test_lora_output_over_an_input_is_refused(change):
+    code, why = _lora_status(**change)
+    assert code == -5 and "overlap" in why, (code, why)
+
+
+def _norm_status(d=64, n=4, xs=64, rs=64, t=2, rt=2, mx=True, x=1, res=2, w=3, scale=4, s=5, y=6, q=7, sf=8):
+    place = lambda v: v * FAR if v < 100 else v  # noqa: E731
+    return _status("launch_add_rmsnorm_quantize_kernel", place(x), place(res), place(w), 0 if mx else place(scale), place(s), place(y), place(q),
+                   place(sf) if mx else 0, n, d, xs, rs, 1e-6, t, rt, 5, None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(s=P + 128, res=P), dict(s=P, res=P + 128), dict(s=P, res=P, rs=128), dict(s=P, x=P, rt=0), dict(s=P, x=P + 32), dict(s=P, x=P, xs=128),
+    dict(s=P, w=P + 64), dict(mx=False, s=P, scale=P + 4), dict(s=P, y=P), dict(s=P, q=P + 384), dict(q=P, sf=P + 64), dict(y=P, x=P + 128), dict(q=P, x=P),
+    dict(s=P, sf=P + 256),
+])
+def test_norm_output_over_an_input_is_refused(change):
+    code, why = _norm_status(**change)
+    assert code in (-2, -5) and ("overlap" in why or "in place" in why), (code, why)
