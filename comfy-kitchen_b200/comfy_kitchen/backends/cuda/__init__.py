@@ -672,7 +672,8 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
         if weight.dtype != dtype or not weight.is_contiguous():
             weight = weight.to(dtype).contiguous()
     _same_device(what, device, residual, weight, sum_out)
-    if sum_out is None:
+    given = sum_out
+    if given is None:
         sum_out = _empty(residual, shape, stream_dtype)
     elif sum_out.shape != shape or sum_out.dtype != stream_dtype or not sum_out.is_contiguous():
         raise ValueError(f"{what}: sum_out must be contiguous with the residual's shape and dtype")
@@ -688,6 +689,8 @@ def _add_rmsnorm(what, x, residual, weight, eps, scale, output_type, return_norm
                 0 if mx else scale.data_ptr(), sum_out.data_ptr(), norm.data_ptr() if return_norm else 0, q.data_ptr(),
                 sx.data_ptr() if mx else 0, n, d, x_stride, r_stride, eps, _code(dtype, what),
                 _code(stream_dtype, what), DTYPE_TO_CODE[output_type])
+        if given is not None:
+            torch.autograd.graph.increment_version(given)   # (autograd is told, as by torch's in-place operators)
     return q, sx, sum_out, norm
 
 
@@ -847,7 +850,8 @@ def lora_add(
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,)):
         raise ValueError(f"{what}: scales must be float32 [{adapters}]")
     _same_device(what, device, y, a, b, adapter_ids, scales, out)
-    if out is None:
+    given = out
+    if given is None:
         out = _empty(y, y_shape, dtype)
     elif out.shape != y_shape or out.dtype != dtype:
         raise ValueError(f"{what}: out must have y's shape and dtype")
@@ -856,7 +860,7 @@ def lora_add(
         return out
     if device.index is not None and device.index != torch._C._cuda_getDevice():   # (the scratch's size goes by the device)
         with torch.cuda.device(device):
-            return lora_add(y, x, a, b, adapter_ids, scales, out)
+            return lora_add(y, x, a, b, adapter_ids, scales, given)
     # the kernels move 16 bytes at a time
     (xf, x_stride), (yf, y_stride), (of, o_stride) = _rows(x, k), _rows(y, n), _rows(out, n)
     px, py, po, pa, pb = xf.data_ptr(), yf.data_ptr(), of.data_ptr(), a.data_ptr(), b.data_ptr()
@@ -883,6 +887,8 @@ def lora_add(
     _launch(device, "launch_lora_add_kernel", py, px, pa, pb, ids.data_ptr(), 0 if scales is None else scales.data_ptr(), po,
             0 if work is None else work.data_ptr(), rows, k, n, rank, adapters, y_stride, x_stride, o_stride, rows // ids.numel(),
             _code(dtype, what), ids_dtype == torch.int64)
+    if given is not None:
+        torch.autograd.graph.increment_version(given)
     return out
 
 

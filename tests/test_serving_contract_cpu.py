@@ -172,3 +172,33 @@ def _norm_status(d=64, n=4, xs=64, rs=64, t=2, rt=2, mx=True, x=1, res=2, w=3, s
 def test_norm_output_over_an_input_is_refused(change):
     code, why = _norm_status(**change)
     assert code in (-2, -5) and ("overlap" in why or "in place" in why), (code, why)
+
+
+# ---- outputs that the caller gives
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    monkeypatch.setattr(backend, "_launch", lambda *args: None)
+
+
+def _given(name):
+    """An entry point called with an output of the caller's, and that output: one of its inputs' place, as in place."""
+    entry, args = _calls()[name]
+    out = args["y" if name == "lora_add" else "residual"]
+    return lambda: entry(**args, **{"out" if name == "lora_add" else "sum_out": out}), out
+
+
+@pytest.mark.parametrize("name", ["lora_add", "mxfp8", "fp8"])
+def test_autograd_sees_what_is_written(no_launch, name):
+    """A tensor that a backward pass needs and that is overwritten makes that pass fail, as for torch's own operators."""
+    call, out = _given(name)
+    factor = torch.ones_like(out, requires_grad=True)
+    product = (out * factor).sum()
+    with torch.no_grad():
+        call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():        # (no versions there)
+        call, out = _given(name)
+        call()
