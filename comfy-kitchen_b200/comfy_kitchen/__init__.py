@@ -104,8 +104,12 @@ def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: 
     -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``residual`` and h
     have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to; ``residual`` itself (or x, where it has h's dtype),
     or memory that no input lies in."""
-    if sum_out is None and not _Ops._plain((x, residual, weight)):
-        got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
+    if not _Ops._plain((x, residual, weight, sum_out)):
+        if sum_out is None:
+            got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
+        else:
+            data, scales, norm = _ops_ns.add_rmsnorm_quantize_mxfp8_out(x, residual, weight, eps, return_norm, sum_out)
+            got = data, scales.view(torch.float8_e8m0fnu), sum_out, norm
         return got if return_norm else got[:-1]
     impl = registry.get_implementation("add_rmsnorm_quantize_mxfp8", kwargs={"x": x, "residual": residual, "weight": weight})
     return impl(x, residual, weight, eps, return_norm, sum_out)
@@ -116,8 +120,13 @@ def add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: to
                              sum_out: torch.Tensor | None = None):
     """h = x + residual; ``quantize_per_tensor_fp8(rmsnorm(h, weight, eps), scale, output_type)`` in one pass.
     -> (data, h), and the normalised h behind them with ``return_norm``; see ``add_rmsnorm_quantize_mxfp8``."""
-    if sum_out is None and not _Ops._plain((x, residual, weight, scale)):
-        got = _ops_ns.add_rmsnorm_quantize_fp8(x, residual, weight, scale, eps, DTYPE_TO_CODE[output_type], return_norm)
+    if not _Ops._plain((x, residual, weight, scale, sum_out)):
+        code = DTYPE_TO_CODE[output_type]
+        if sum_out is None:
+            got = _ops_ns.add_rmsnorm_quantize_fp8(x, residual, weight, scale, eps, code, return_norm)
+        else:
+            data, norm = _ops_ns.add_rmsnorm_quantize_fp8_out(x, residual, weight, scale, eps, code, return_norm, sum_out)
+            got = data, sum_out, norm
         return got if return_norm else got[:-1]
     impl = registry.get_implementation("add_rmsnorm_quantize_fp8", kwargs={"x": x, "residual": residual, "weight": weight, "scale": scale,
                                                                            "output_type": output_type})
@@ -129,8 +138,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """y + scales[i] * (x @ a[i].T) @ b[i].T with i the row's adapter id: the low-rank adapters of many requests beside
     a shared projection y [..., N] of x [..., K].  a: [L, R, K]; b: [L, N, R]; adapter_ids: int32 or int64, one per row
     or per leading index (outside [0, L): no adapter); ``out``: y itself, or memory that no input lies in."""
-    if out is None and not _Ops._plain((y, x, a, b, adapter_ids, scales)):
-        return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
+    if not _Ops._plain((y, x, a, b, adapter_ids, scales, out)):
+        if out is None:
+            return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
+        _ops_ns.lora_add_out(y, x, a, b, adapter_ids, scales, out)
+        return out
     impl = registry.get_implementation("lora_add", kwargs={"y": y, "x": x, "a": a, "b": b, "adapter_ids": adapter_ids, "scales": scales})
     return impl(y, x, a, b, adapter_ids, scales, out)
 

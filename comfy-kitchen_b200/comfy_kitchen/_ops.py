@@ -296,3 +296,49 @@ def _op_lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
 @_op_lora_add.register_fake
 def _(y, x, a, b, adapter_ids, scales):
     return torch.empty(y.shape, dtype=y.dtype, device=y.device)
+
+
+# The same with an output of the caller's, which may be an input (``residual``, ``y``) itself: an op returns no argument of its
+# own, so it returns only what is new.
+
+
+@torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_mxfp8_out", mutates_args=("sum_out",))
+def _op_add_rmsnorm_quantize_mxfp8_out(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float, return_norm: bool,
+                                       sum_out: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    # (the scales' bytes: torch's compiler does not take apart an op that writes to an argument and returns float8_e8m0fnu)
+    got = _dispatch("add_rmsnorm_quantize_mxfp8", x=x, residual=residual, weight=weight, eps=eps, return_norm=return_norm, sum_out=sum_out)
+    return got[0], got[1].view(torch.uint8), got[3] if return_norm else x.new_empty(0)
+
+
+@_op_add_rmsnorm_quantize_mxfp8_out.register_fake
+def _(x, residual, weight, eps, return_norm, sum_out):
+    d = x.shape[-1]
+    n = x.numel() // d
+    return (torch.empty((n, d), dtype=torch.float8_e4m3fn, device=x.device),
+            torch.empty((roundup(n, 128), roundup(d // 32, 4)), dtype=torch.uint8, device=x.device),
+            torch.empty(x.shape if return_norm else (0,), dtype=x.dtype, device=x.device))
+
+
+@torch.library.custom_op("comfy_kitchen::add_rmsnorm_quantize_fp8_out", mutates_args=("sum_out",))
+def _op_add_rmsnorm_quantize_fp8_out(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, scale: torch.Tensor, eps: float,
+                                     output_dtype_code: int, return_norm: bool, sum_out: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    got = _dispatch("add_rmsnorm_quantize_fp8", x=x, residual=residual, weight=weight, scale=scale, eps=eps,
+                    output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code], return_norm=return_norm, sum_out=sum_out)
+    return got[0], got[2] if return_norm else x.new_empty(0)
+
+
+@_op_add_rmsnorm_quantize_fp8_out.register_fake
+def _(x, residual, weight, scale, eps, output_dtype_code, return_norm, sum_out):
+    return (torch.empty(x.shape, dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code], device=x.device),
+            torch.empty(x.shape if return_norm else (0,), dtype=x.dtype, device=x.device))
+
+
+@torch.library.custom_op("comfy_kitchen::lora_add_out", mutates_args=("out",))
+def _op_lora_add_out(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+                     scales: torch.Tensor | None, out: torch.Tensor) -> None:
+    _dispatch("lora_add", y=y, x=x, a=a, b=b, adapter_ids=adapter_ids, scales=scales, out=out)
+
+
+@_op_lora_add_out.register_fake
+def _(y, x, a, b, adapter_ids, scales, out):
+    return None

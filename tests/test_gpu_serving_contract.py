@@ -153,3 +153,44 @@ def test_norm_sum_over_its_inputs(ck, width, dtype, stream):
         with pytest.raises(RuntimeError, match="overlaps"):
             ck.add_rmsnorm_quantize_fp8(r, x.to(stream), w, torch.ones(1, device="cuda"), sum_out=s)
     assert torch.equal(long, before)
+
+
+# ------------------------------------------------------------------ compiled, in place
+
+
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_in_place_forms_compiled(ck, backend):
+    g = _gen(5)
+    rows, width, n = 50, 256, 384
+    x, res, w, scale = _randn(g, rows, width), _randn(g, rows, width, dtype=FP32), _randn(g, width), torch.tensor([0.02], device="cuda")
+    a, b, ids = _randn(g, 3, 16, width, scale=0.06), _randn(g, 3, n, 16, scale=0.1), torch.arange(rows, device="cuda") % 4
+    y = _randn(g, rows, n)
+
+    def step(x, res, y, into):
+        q, s, h, norm = ck.add_rmsnorm_quantize_mxfp8(x, res, w, return_norm=True, sum_out=res)     # the stream's own place
+        q2, h2, norm2 = ck.add_rmsnorm_quantize_fp8(x, h, w, scale, return_norm=True, sum_out=into)
+        ck.lora_add(y, norm, a, b, ids, out=y)                                                       # the projection's
+        z = ck.lora_add(y, norm2, a, b, ids, out=torch.empty_like(y))
+        return [q, s, q2, h + 1, h2 * 2, norm, norm2, z]
+
+    def given():
+        return [x.clone(), res.clone(), y.clone(), torch.zeros_like(res)]
+
+    ours, theirs = given(), given()
+    with torch.no_grad():
+        want = step(*ours)
+        got = torch.compile(step, fullgraph=True, backend=backend)(*theirs)
+    for u, v in zip(want + ours, got + theirs):
+        assert u.dtype == v.dtype and torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+
+
+def test_in_place_ops(ck):
+    g = _gen(6)
+    x, res, w = _randn(g, 9, 64), _randn(g, 9, 64), _randn(g, 64)
+    a, b, ids, scale = _randn(g, 3, 16, 64), _randn(g, 3, 96, 16), torch.arange(9, device="cuda") % 4, torch.ones(1, device="cuda")
+    y = _randn(g, 9, 96)
+    ops, which = torch.ops.comfy_kitchen, ("test_schema", "test_faketensor")
+    torch.library.opcheck(ops.lora_add_out, (y, x, a, b, ids, None, torch.empty_like(y)), test_utils=which)
+    for keep in (True, False):
+        torch.library.opcheck(ops.add_rmsnorm_quantize_mxfp8_out, (x, res, w, 1e-6, keep, torch.empty_like(res)), test_utils=which)
+        torch.library.opcheck(ops.add_rmsnorm_quantize_fp8_out, (x, res, w, scale, 1e-6, 5, keep, torch.empty_like(res)), test_utils=which)

@@ -202,3 +202,20 @@ def test_autograd_sees_what_is_written(no_launch, name):
     with torch.inference_mode():        # (no versions there)
         call, out = _given(name)
         call()
+
+
+@pytest.mark.parametrize("same", [True, False])
+def test_given_outputs_under_a_fake_mode(same):
+    """The in-place forms are traceable, like those that return new tensors."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        (_, lora), (_, norm) = _calls()["lora_add"], _calls()["mxfp8"]
+        out = lora["y"] if same else torch.empty_like(lora["y"])
+        assert ck.lora_add(**lora, out=out) is out
+        sum_out = norm["residual"] if same else torch.empty_like(norm["residual"])
+        for keep in (False, True):
+            q, s, h, *y = ck.add_rmsnorm_quantize_mxfp8(**norm, return_norm=keep, sum_out=sum_out)
+            assert q.shape == (2, 64) and s.shape == (128, 4) and h is sum_out and [t.shape for t in y] == [norm["x"].shape] * keep
+            q, h, *y = ck.add_rmsnorm_quantize_fp8(**norm, scale=torch.ones(1), return_norm=keep, sum_out=sum_out)
+            assert q.shape == (2, 64) and q.dtype == torch.float8_e4m3fn and h is sum_out and [t.shape for t in y] == [norm["x"].shape] * keep
