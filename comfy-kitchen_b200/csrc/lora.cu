@@ -834,6 +834,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         }
     } else if (warp == 11) {
         // stores in the units' order; a stage is handed back one store later, when its own has read it
+        tc::wait_for_dependency();   // (a CTA without a share waits here, too: this grid ends behind those that it hangs on, whose tables are in a
+                                     // workspace that the next kernel may have been given)
         tc::Ring yr;
         int before = -1;
         bool ok = true;

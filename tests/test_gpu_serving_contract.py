@@ -194,3 +194,35 @@ def test_in_place_ops(ck):
     for keep in (True, False):
         torch.library.opcheck(ops.add_rmsnorm_quantize_mxfp8_out, (x, res, w, 1e-6, keep, torch.empty_like(res)), test_utils=which)
         torch.library.opcheck(ops.add_rmsnorm_quantize_fp8_out, (x, res, w, scale, 1e-6, 5, keep, torch.empty_like(res)), test_utils=which)
+
+
+# ------------------------------------------------------------------ adapters: workspaces
+
+
+@pytest.mark.parametrize("rows", [700, 5000])
+def test_lora_nothing_to_add_in_place_then_another(ck, rows):
+    """In place and with no adapter asked for no CTA of the last kernel has work; what follows, in the same memory, must find the kernels
+    before it done.  (A padded step of a captured graph.)"""
+    g = _gen(rows)
+    k, n, rank = 512, 1032, 64
+    a, b = _randn(g, 4, rank, k, scale=0.05), _randn(g, 4, n, rank, scale=0.1)
+    x, y = _randn(g, rows, k), _randn(g, rows, n)
+    none, some = torch.full((rows,), -1, device="cuda"), torch.arange(rows, device="cuda") // 100 % 5
+    want = ck.lora_add(y, x, a, b, some)
+    own = y.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for _ in range(4):
+            ck.lora_add(own, x, a, b, none, out=own)
+            garbage = torch.full((1 << 22,), 0x7F7F7F7F, dtype=torch.int32, device="cuda")    # into the workspace that was given back
+            del garbage
+            got = ck.lora_add(own, x, a, b, some)
+    for _ in range(50):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(own, y) and torch.equal(got, want)
+    from comfy_kitchen.backends import cuda
+
+    assert cuda.lora_device_status() == 0
