@@ -731,7 +731,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     auto end_of = [&](int tile) { return tile == to.tile ? to.step : plan.steps; };
 
     auto tile_count = [&](int tile) { return __ldcg(p.asked128 + tile); };
-    // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles
+    // y's and B's tiles come from two warps: what frees a y tile needs products, and what frees a B tile may need y tiles.
+    // A full ring is not freed before the kernels that this one hangs on are done, and those may run on for longer than a bounded
+    // wait lasts (a CTA starts here as soon as its SM is free, and tiles that hundreds of adapters meet in keep others busy): so
+    // every role waits for them first, without a limit, and counts only from there.
     if (warp == 0) {
         tc::Ring yr;
         uint32_t issued = 0;
@@ -740,6 +743,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
             const int begin = begin_of(tile), end = end_of(tile);
             if (in_place && tile_count(tile) == 0) continue;
             for (int unit = begin * kU; unit < end * kU; ++unit) {
+                if (issued == (uint32_t)plan.y_stages) tc::wait_for_dependency();   // (see above)
                 ok = tc::mbar_wait(&y_empty[yr.at], yr.round ^ 1u, s_abort, &g_lora_status, kWaitYFree);
                 if (!ok) break;
                 if (tc::elect_one()) {
@@ -765,6 +769,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 for (int j = 0; j < count && ok; ++j) {
                     const int which = s_list[j];
                     for (int k = 0; k < plan.blocks; ++k) {
+                        if (issued == (uint32_t)plan.b_stages) tc::wait_for_dependency();
                         ok = tc::mbar_wait(&b_empty[br.at], br.round ^ 1u, s_abort, &g_lora_status, kWaitEmpty);
                         if (!ok) break;
                         if (tc::elect_one()) {
