@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(96) lora_count_kernel(const LoraArgs p) {
             const int wide = (hi + 1 - (lo & ~7) + 15) & ~15;
             if (lane == 0) { l.id[j] = which; l.wide[j] = (int16_t)wide; l.from[j] = (int16_t)min(lo & ~7, kShrinkRows - wide); }
         });
-        if (lane == 0) { l.count = n; p.asked256[tile] = n; }
+        // (no blocks, until the first product's kernel says otherwise: one that gives up may not)
+        if (lane == 0) { l.count = n; p.asked256[tile] = n; p.first_block[tile] = 0; p.last_block[tile] = -1; }
     }
 }
 
@@ -614,6 +615,8 @@ __global__ void __launch_bounds__(kJoinThreads) lora_join_kernel(const LoraArgs 
     const int id = place >= 0 ? __ldcg(p.list128 + row / kTile * kTile + place) : -1;
     const float scale = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.0f;
     tc::wait_for_dependency();
+    // (where the first product's kernel has given up on a tile, either may still be what the count kernel has set: no blocks, or some
+    // of another tile's, but none outside `partial`; the status word says that the result is none)
     const int tile = (int)(row / kShrinkRows), block0 = id >= 0 ? __ldcg(p.first_block + tile) : 0, block1 = id >= 0 ? __ldcg(p.last_block + tile) : -1;
     float v[kMaxRank / 64][8];
 #pragma unroll

@@ -226,3 +226,28 @@ def test_lora_nothing_to_add_in_place_then_another(ck, rows):
     from comfy_kitchen.backends import cuda
 
     assert cuda.lora_device_status() == 0
+
+
+@pytest.mark.parametrize("rows,k,n,rank", [(700, 512, 264, 64), (520, 264, 1032, 200), (5000, 1032, 520, 24), (17000, 256, 136, 128)])
+def test_lora_workspace_needs_no_value(ck, rows, k, n, rank):
+    """Through the C entry: whatever lies in the scratch, nothing behind its end is touched, and it is the call's own again the next time."""
+    from comfy_kitchen import _native
+
+    g = _gen(rows + n)
+    a, b, scales = _randn(g, 5, rank, k, scale=k ** -0.5), _randn(g, 5, n, rank, scale=0.1), 0.5 + torch.rand(5, generator=g, device="cuda")
+    x, y = _randn(g, rows, k), _randn(g, rows, n)
+    ids = (torch.arange(rows, device="cuda") // 150 * 7) % 9 - 2           # tiles of several adapters, of one, of none
+    want = ck.lora_add(y, x, a, b, ids, scales)
+    need = _native.load().ck_lora_workspace_bytes(rows, k, n, rank)
+    assert need > 0
+    work, tail = torch.empty(need + 4096, dtype=torch.uint8, device="cuda"), 0x5A
+    for fill in (0x00, 0xFF, 0x7F, 0x80, "random", "last"):
+        if fill == "random":
+            work.copy_(torch.randint(0, 256, work.shape, generator=g, device="cuda").to(torch.uint8))
+        elif fill != "last":
+            work.fill_(fill)
+        work[need:] = tail
+        out = torch.empty_like(y)
+        _native.call("launch_lora_add_kernel", y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), scales.data_ptr(), out.data_ptr(),
+                     work.data_ptr(), rows, k, n, rank, 5, n, k, n, 1, 2, True, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out, want) and bool((work[need:] == tail).all())
