@@ -78,7 +78,10 @@ constexpr int kSmemSfA = 4 * 512;           // up to four 512-byte tiles (NVFP4)
 constexpr int kSmemSfB = 2 * 4 * 512;       // two row tiles x four: all 256 columns
 constexpr int kStageBytes = kSmemA + kSmemB + kSmemSfA + kSmemSfB;   // 38 KB
 constexpr int kSmemOut = kEpiWarps * 2048;   // per-epilogue-warp staging: 32 rows x 64 bytes, 64-byte swizzle
+// barriers (full, empty, sf_full; tmem_full, tmem_empty, tile_open, drain[2]), then the TMEM address and the abort flag
+constexpr int kSmemBars = 8 * (3 * kStages + 2 * kSfBufs + 5) + 8;
 constexpr int kSmemBytes = kStages * kStageBytes + kSmemOut + 256 /*barriers*/ + 1024 /*alignment slack*/;
+static_assert(kSmemBars <= 256, "the barriers do not fit the room kept for them");
 static_assert(kStageBytes % 1024 == 0, "operand tiles need 1024-byte alignment");
 static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 
@@ -529,7 +532,8 @@ gemm_blockscaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         // Issuing one block-scaled MMA keeps a thread ~100 clocks and the bookkeeping of a k-tile (barrier
         // look-ahead, commit) another ~150, while the tensor cores need 128 clocks per MMA: a single issuer
         // cannot keep them fed.  Two warps therefore take the k-tiles in turn (of all tiles: warp 1 the even ones).  The
-        // accumulation order does not matter except for the first MMA of a tile, which overwrites: the second
+        // accumulation order does not matter (it shows in the last bit of an MXFP8 result: some 200 of 42 M bf16
+        // elements differ from launch to launch) except for the first MMA of a tile, which overwrites: the second
         // issuer of a tile waits (tile_open) until the first has issued it.  A commit covers the committing thread's own
         // MMAs, so each issuer releases the stages it consumed and both commit to tmem_full.
         const uint32_t which = warp == 1 ? 0u : 1u;
