@@ -97,7 +97,7 @@ class FunctionConstraints:
                      self.min_compute_capability))
 
 
-@dataclass
+@dataclass(frozen=True)
 class ValidationResult:
     success: bool
     failed_param: str | None = None

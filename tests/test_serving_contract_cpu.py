@@ -219,3 +219,19 @@ def test_given_outputs_under_a_fake_mode(same):
             assert q.shape == (2, 64) and s.shape == (128, 4) and h is sum_out and [t.shape for t in y] == [norm["x"].shape] * keep
             q, h, *y = ck.add_rmsnorm_quantize_fp8(**norm, scale=torch.ones(1), return_norm=keep, sum_out=sum_out)
             assert q.shape == (2, 64) and q.dtype == torch.float8_e4m3fn and h is sum_out and [t.shape for t in y] == [norm["x"].shape] * keep
+
+
+# ---- the registry's answers
+
+
+def test_a_validation_result_cannot_be_changed():
+    """One answer serves every call that is in order: a caller that could write to it would change all later ones."""
+    import dataclasses
+
+    from comfy_kitchen.constraints import FunctionConstraints, validate_function_call
+
+    good = validate_function_call(FunctionConstraints(), {})
+    for field, value in (("success", False), ("failed_param", "x"), ("failure_reason", "y")):
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            setattr(good, field, value)
+    assert validate_function_call(FunctionConstraints(), {}).success
