@@ -251,3 +251,102 @@ def test_lora_workspace_needs_no_value(ck, rows, k, n, rank):
         _native.call("launch_lora_add_kernel", y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), scales.data_ptr(), out.data_ptr(),
                      work.data_ptr(), rows, k, n, rank, 5, n, k, n, 1, 2, True, torch.cuda.current_stream().cuda_stream)
         assert torch.equal(out, want) and bool((work[need:] == tail).all())
+
+
+# ------------------------------------------------------------------ large tensors, several callers
+
+
+def _same(u, v):
+    return torch.equal(u.contiguous().view(torch.uint8), v.contiguous().view(torch.uint8))
+
+
+def test_norm_past_32_bit_offsets(ck):
+    g, rows, width = _gen(20), 140001, 16384                               # 2.3 G elements
+    x, res, w = (torch.empty(s, dtype=BF16, device="cuda").normal_(generator=g) for s in ((rows, width), (rows, width), (width,)))
+    scale = torch.tensor([0.02], device="cuda")
+    whole = ck.add_rmsnorm_quantize_mxfp8(x, res, w, return_norm=True)
+    fp8 = ck.add_rmsnorm_quantize_fp8(x, res, w, scale)[0]
+    for first in (0, 131008, rows - 97):
+        part = slice(first, first + 97)
+        q, _, h, y = ck.add_rmsnorm_quantize_mxfp8(x[part].clone(), res[part].clone(), w, return_norm=True)
+        for got, want in zip((q, h, y), (whole[0], whole[2], whole[3])):
+            assert _same(got, want[part])
+        assert _same(ck.add_rmsnorm_quantize_fp8(x[part].clone(), res[part].clone(), w, scale)[0], fp8[part])
+    assert _same(whole[1], ck.quantize_mxfp8(whole[3])[1])
+
+
+@pytest.mark.parametrize("tokens_dim", [1, 2])
+@pytest.mark.parametrize("unaligned", [0, 1])
+def test_rope_past_32_bit_offsets(ck, tokens_dim, unaligned):
+    g, n, heads, dim, axes = _gen(21), 140001, 128, 128, (32, 48, 48)
+    x = torch.empty(n * heads * dim + unaligned, dtype=BF16, device="cuda").normal_(generator=g)[unaligned:]
+    x = x.view((1, n, heads, dim) if tokens_dim == 1 else (1, heads, n, dim))
+    pos, freqs = torch.randint(0, 1 << 20, (n, 3), generator=g, device="cuda"), ck.rope_axes_freqs(axes)
+    out = ck.apply_rope_axes1(x, pos, freqs, axes, tokens_dim=tokens_dim)
+    for first in (0, 131060, n - 40):
+        part = slice(first, first + 40)
+        cut = lambda t: (t[:, part] if tokens_dim == 1 else t[:, :, part]).contiguous()  # noqa: E731
+        if unaligned:     # (the one-pair kernel: the same angles, another order of roundings)
+            small = ck.apply_rope_axes1(cut(x), pos[part], freqs, axes, tokens_dim=tokens_dim).double()
+            size = cut(x).double().abs().view(*small.shape[:-1], -1, 2).sum(-1, keepdim=True).expand(*small.shape[:-1], -1, 2).reshape(small.shape)
+            assert bool(((cut(out).double() - small).abs() <= 2 * (2.0 ** -8 * 1.01 * small.abs() + 2.0 ** -20 * size)).all())
+        else:
+            assert torch.equal(cut(out), ck.apply_rope_axes1(cut(x), pos[part], freqs, axes, tokens_dim=tokens_dim))
+
+
+def test_lora_past_32_bit_offsets(ck):
+    g, rows, k, n, rank = _gen(22), 300001, 8192, 8200, 24
+    x, y = (torch.empty(rows, c, dtype=BF16, device="cuda").normal_(generator=g) for c in (k, n))
+    a, b = _randn(g, 5, rank, k, scale=k ** -0.5), _randn(g, 5, n, rank, scale=0.1)
+    ids = torch.arange(rows, device="cuda") // 777 % 6
+    out = ck.lora_add(y, x, a, b, ids)
+    for first in (0, 131000, 262000, rows - 300):
+        part = slice(first, first + 300)
+        low = torch.stack([x[t].double() @ a[i].double().T if i < 5 else torch.zeros(rank, device="cuda", dtype=torch.float64) for t, i in zip(range(first, first + 300), ids[part].tolist())])
+        more = torch.einsum("tr,tnr->tn", low, b.double()[ids[part].clamp(max=4)])
+        want = y[part].double() + more
+        size = torch.einsum("tr,tnr->tn", low.abs(), b.double().abs()[ids[part].clamp(max=4)])
+        # k products of unit variance over sqrt(k) in fp32, then rank; the low-rank vector as two bf16 parts; one rounding to bf16
+        bound = 2.0 ** -8 * 1.01 * want.abs() + size * 2.0 ** -16 + (k + rank) * 2.0 ** -23 * k ** 0.5 * b.double().abs().sum(-1).max()
+        assert bool(((out[part].double() - want).abs() <= bound).all())
+    own = y.clone()
+    ck.lora_add(own, x, a, b, ids, out=own)
+    assert torch.equal(own, out)
+
+
+def test_several_threads_at_once(ck):
+    """Four threads, each on a stream of its own, with operators of every kind between one another."""
+    import threading
+
+    def case(seed):
+        g = _gen(seed)
+        rows, k, n = 700 + 300 * seed, 512, 1032
+        return dict(x=_randn(g, rows, k), y=_randn(g, rows, n), a=_randn(g, 4, 64, k, scale=0.05), b=_randn(g, 4, n, 64, scale=0.1),
+                    ids=torch.arange(rows, device="cuda") // (90 + seed) % 5, q=_randn(g, 1, rows, 4, 64), pos=torch.randint(0, 5000, (rows, 2), generator=g, device="cuda"))
+
+    def run(c):
+        q, s, h, norm = ck.add_rmsnorm_quantize_mxfp8(c["x"], c["x"], None, return_norm=True)
+        few = ck.lora_add(c["y"][:40], norm[:40], c["a"], c["b"], c["ids"][:40])
+        return [q, s, h, norm, few, ck.lora_add(c["y"], norm, c["a"], c["b"], c["ids"]), ck.apply_rope_axes1(c["q"], c["pos"], freqs, (24, 40), tokens_dim=1)]
+
+    freqs = ck.rope_axes_freqs((24, 40))
+    cases = [case(s) for s in range(4)]
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def worker(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(100):
+                    if not all(_same(u, v) for u, v in zip(run(cases[i]), want[i])):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001 - told below
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
