@@ -101,9 +101,10 @@ def adaln_quantize_mxfp8(x, scale, shift, eps: float = 1e-6):
 def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
                                return_norm: bool = False, sum_out: torch.Tensor | None = None):
     """h = x + residual; ``quantize_mxfp8(rmsnorm(h, weight, eps).reshape(-1, D))`` in one pass.
-    -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``residual`` and h
-    have x's dtype or float32; ``sum_out``: a contiguous tensor to write h to; ``residual`` itself (or x, where it has h's dtype),
-    or memory that no input lies in."""
+    -> (data, block scales, h), and the normalised h in x's dtype behind them with ``return_norm``.  ``weight`` is taken in x's
+    dtype (a float32 one beside 16-bit x is rounded to it, as ``rmsnorm`` does).  ``residual`` and h have x's dtype or float32;
+    ``sum_out``: a contiguous tensor to write h to: ``residual`` itself (or x, where it has h's dtype), or memory that no input
+    lies in."""
     if not _Ops._plain((x, residual, weight, sum_out)):
         if sum_out is None:
             got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)

@@ -701,9 +701,9 @@ def add_rmsnorm_quantize_mxfp8(
     """h = x + residual; quantize_mxfp8(rmsnorm(h, weight, eps)) in one pass -> (data, block scales, h), and with
     ``return_norm`` the normalised h behind them.
 
-    ``residual`` (and h) has x's dtype or float32; the norm is taken of h as stored and rounded to x's dtype before it
-    is quantized.  ``sum_out``: a contiguous tensor for h, which may be ``residual`` itself (or x, where it has h's dtype); any
-    other overlap with an input is refused.
+    ``residual`` (and h) has x's dtype or float32; ``weight`` is taken in x's dtype, whatever it has; the norm is taken of h as
+    stored and rounded to x's dtype before it is quantized.  ``sum_out``: a contiguous tensor for h, which may be ``residual`` itself
+    (or x, where it has h's dtype); any other overlap with an input is refused.
     """
     q, sx, h, norm = _add_rmsnorm("add_rmsnorm_quantize_mxfp8", x, residual, weight, eps, None, torch.float8_e4m3fn, return_norm, sum_out)
     return (q, sx, h, norm) if return_norm else (q, sx, h)
@@ -823,7 +823,8 @@ def lora_add(
     y: [..., N], what the shared projection made of x: [..., K].  a: [L, R, K], b: [L, N, R] (adapters of a lower rank are
     padded with zeros).  adapter_ids: int32 or int64 in the shape of x's leading dimensions, or of the first of them
     (one per batch entry); an id outside [0, L) means no adapter, and the row of y is passed on.  scales: float32 [L].
-    ``out``: where to write, in y's shape; may be y itself, any other overlap with an input is refused.  K, N and R are multiples of 8, R at most 256.
+    ``out``: where to write, in y's shape; may be y itself, any other overlap with an input is refused.
+    K, N and R are multiples of 8, R at most 256.
     """
     what = "lora_add"
     _no_grad(what, y, x, a, b, scales, out)

@@ -14,7 +14,7 @@
 // back from where the same thread has just written it.
 //
 // Measured: 16384 x 8192 bf16 to MXFP8 in 152.8 us back to back (6.18 TB/s, 96 % of the copy rate; 141 in a short burst),
-// 4608 x 8192 bf16 with an fp32 residual to per-tensor FP8 in 68.9 us (6.03 TB/s, 93 %), one row of 4096 in 2.2 us of a graph.  The MXFP8
+// 4608 x 8192 bf16 with an fp32 residual to per-tensor FP8 in 68.2 us (6.09 TB/s, 94 %), one row of 4096 in 2.1 us of a graph.  The MXFP8
 // form has instructions to spare only since pairs are worked on together (add, squares, products, maximum) and the
 // scale needs no division: 28.5 instructions an element took 74 % of the issue slots and 164 us, 21 take 58 %.
 #include "ck_common.cuh"

@@ -6,7 +6,7 @@
 //
 // Bound by HBM in either direction: x is read once, y read and out written once (2 K + 4 N bytes a row), each used adapter
 // once; the products' 2 R (K + N) flop a row stay below that up to a rank of about 128.  Two forms:
-//   few rows:   one CTA per row.
+//   few rows:   a cluster of eight CTAs per row, one launch.
 //   many rows:  four kernels, two of them on the tensor cores (tcgen05):
 //               count:   which adapters each tile of rows asks for; by their number the others share out their work;
 //               shrink:  low[t, :] = A x[t], equal shares of the tiles' K steps for every SM, partial sums in fp32;
@@ -18,8 +18,8 @@
 // one another cost nothing extra; a tile of 128 different adapters reads 128 adapters, as it must.
 //
 // Measured, back to back: 16384 rows, 8192 -> 8192, rank 128, 8 requests: 204 us (64 % of the copy rate; 186 in a short burst:
-// the first product at 8, x done at 71, the sums joined at 81, the first output at 87); 4608 rows, 4096 -> 12288, rank 64, 7 requests: 76 us (54 %), of which about 20 are
-// the four kernels' beginnings and ends; one row 4.2 us, 64 rows of 16 adapters 16.7 us on the device.
+// the first product at 8, x done at 71, the sums joined at 81, the first output at 87); 4608 rows, 4096 -> 12288, rank 64, 7 requests: 76 us (54 %), of which
+// about 30 are the four kernels' beginnings and ends; one row 4.0 us, 64 rows of 16 adapters 16.9 us on the device.
 //
 // Rounding: sums in fp32.  The low-rank vector is the second product's 16-bit operand: it goes in as two parts, the
 // rounded value and what the rounding left (for fp16 scaled by a power of two per row, which keeps large and small vectors
