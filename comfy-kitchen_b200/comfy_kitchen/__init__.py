@@ -138,7 +138,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
              scales: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y + scales[i] * (x @ a[i].T) @ b[i].T with i the row's adapter id: the low-rank adapters of many requests beside
     a shared projection y [..., N] of x [..., K].  a: [L, R, K]; b: [L, N, R]; adapter_ids: int32 or int64, one per row
-    or per leading index (outside [0, L): no adapter); ``out``: y itself, or memory that no input lies in."""
+    or per leading index (outside [0, L): no adapter); ``out``: y (or x) itself, or memory that no input lies in."""
     if not _Ops._plain((y, x, a, b, adapter_ids, scales, out)):
         if out is None:
             return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)

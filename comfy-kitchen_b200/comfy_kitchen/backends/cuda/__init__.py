@@ -823,7 +823,7 @@ def lora_add(
     y: [..., N], what the shared projection made of x: [..., K].  a: [L, R, K], b: [L, N, R] (adapters of a lower rank are
     padded with zeros).  adapter_ids: int32 or int64 in the shape of x's leading dimensions, or of the first of them
     (one per batch entry); an id outside [0, L) means no adapter, and the row of y is passed on.  scales: float32 [L].
-    ``out``: where to write, in y's shape; may be y itself, any other overlap with an input is refused.
+    ``out``: where to write, in y's shape; may be y (or x) itself, any other overlap with an input is refused.
     K, N and R are multiples of 8, R at most 256.
     """
     what = "lora_add"

@@ -58,6 +58,13 @@ inline Memory memory_of(const void* at, int64_t bytes) { return Memory{at, 1, 0,
 inline bool same_place(const Memory& a, const Memory& b) {
     return a.at == b.at && a.rows == b.rows && a.bytes == b.bytes && (a.rows == 1 || a.stride == b.stride);
 }
+// Whether no run of one shares a byte with any but the same run of the other.
+inline bool row_by_row(const Memory& a, const Memory& b) {
+    if (a.rows != b.rows) return false;
+    if (a.rows == 1) return true;
+    const int64_t ahead = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at));
+    return a.stride == b.stride && ahead + b.bytes <= a.stride && a.bytes - ahead <= a.stride;
+}
 // Whether two of them share a byte.  Runs of one buffer that lie between one another (columns of it, every second row) do not;
 // where the spans meet, the runs are compared modulo the strides' common divisor (exact but for runs that would meet only
 // behind an end).

@@ -1132,14 +1132,14 @@ extern "C" int launch_lora_add_kernel(const void* y, const void* x, const void* 
     if (rank <= 0 || rank % 8 != 0 || rank > kMaxRank) CK_FAIL(CK_ERR_SHAPE, "lora_add: rank %lld (a multiple of 8, at most %d)", (long long)rank, kMaxRank);
     if (!aligned16(y) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out) || ((x_row_stride | y_row_stride | out_row_stride) & 7))
         CK_FAIL(CK_ERR_ALIGN, "lora_add: tensors and row strides must be 16-byte aligned");
-    // a row's columns are read and written by several CTAs, in no order: what is read stays, but y in its own place
-    const Memory written{out, rows, out_row_stride * 2, N * 2}, added{y, rows, y_row_stride * 2, N * 2};
-    if (!same_place(written, added) && overlap(written, added))
-        CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: out overlaps y and is not y");
-    if (overlap(written, Memory{x, rows, x_row_stride * 2, K * 2}) || overlap(written, memory_of(a, adapters * rank * K * 2)) ||
+    // A row's columns are written by several CTAs and other rows by others, in no order, so what they read stays, but for y in its own
+    // place and x's same row (every kernel is done with a row of x before it writes that row).
+    const Memory written{out, rows, out_row_stride * 2, N * 2}, added{y, rows, y_row_stride * 2, N * 2}, taken{x, rows, x_row_stride * 2, K * 2};
+    if (overlap(written, added) && !same_place(written, added)) CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: out overlaps y and is not y");
+    if ((overlap(written, taken) && !row_by_row(written, taken)) || overlap(written, memory_of(a, adapters * rank * K * 2)) ||
         overlap(written, memory_of(b, adapters * rank * N * 2)) || overlap(written, memory_of(scales, adapters * 4)) ||
         overlap(written, memory_of(ids, ceil_div(rows, rows_per_id) * (ids_64bit ? 8 : 4))))
-        CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: out overlaps an input other than y");
+        CK_FAIL(CK_ERR_UNSUPPORTED, "lora_add: out overlaps an input");
     const LoraArgs p{y, x, a, b, ids, scales, out, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, K, N, rank, adapters, y_row_stride, x_row_stride, out_row_stride, rows_per_id, ids_64bit};
     if (few_rows(rows, K, N, rank)) {
         const dim3 grid(kFewCluster, (unsigned)rows);

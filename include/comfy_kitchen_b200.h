@@ -245,7 +245,8 @@ int ck_norm_device_status(void);
  * out[t] = y[t] + scales[a] * B_a (A_a x[t]) for every row, a = ids[t / rows_per_id]; out[t] = y[t] where a lies outside
  * [0, adapters).  y: [rows, N], the shared projection's output; x: [rows, K]; a: [adapters, rank, K]; b: [adapters, N, rank];
  * all bf16 or all fp16, 16-byte aligned, row strides (elements) multiples of 8; ids: int32 or int64; scales: fp32
- * [adapters] or NULL (ones); out may be y (same address and stride), any other overlap of it with an input is refused
+ * [adapters] or NULL (ones); out may be y (same address and stride), and a row of it may lie over the same row of x (same
+ * stride); any other overlap with an input is refused
  * (CK_ERR_UNSUPPORTED).  K, N, rank multiples of 8, rank at most 256.  workspace: scratch of
  * ck_lora_workspace_bytes(), 16-byte aligned, used by this call only until it ends on the stream (need not be set). */
 int launch_lora_add_kernel(const void* y, const void* x, const void* a, const void* b, const void* ids, const float* scales,

@@ -117,12 +117,23 @@ def test_lora_out_beside_its_inputs(ck, rows):
     assert torch.equal(buf[:, 2 * n:], want) and torch.equal(buf[:, :2 * n], kept[:, :2 * n])
     ck.lora_add(y, x, a, b, ids, out=y)                                    # y's own
     assert torch.equal(y, want) and torch.equal(x, kept[:, n:2 * n])
+    one = x.clone()                                                        # x, y and out in one place: h + B A h
+    want_one = ck.lora_add(one, one, a, b, ids)
+    ck.lora_add(one, one, a, b, ids, out=one)
+    assert torch.equal(one, want_one)
+    of_x = x.clone()                                                       # x's place
+    ck.lora_add(kept[:, :n], of_x, a, b, ids, out=of_x)
+    assert torch.equal(of_x, want)
+    wide = _randn(g, rows, n + 64)                                         # out's row over part of x's
+    x_part = wide[:, 64:].clone()
+    ck.lora_add(kept[:, :n], wide[:, 64:], a, b, ids, out=wide[:, :n])
+    assert torch.equal(wide[:, :n], ck.lora_add(kept[:, :n], x_part, a, b, ids))
     every = _randn(g, 3 * rows, n)
     every[0::3], every[1::3] = kept[:, :n], kept[:, n:2 * n]
     ck.lora_add(every[0::3], every[1::3], a, b, ids, out=every[2::3])      # every third row
     assert torch.equal(every[2::3], want) and torch.equal(every[0::3], kept[:, :n])
     rest = _randn(g, rows + 1, n)
-    for yy, xx, out in ((rest[:-1], x, rest[1:]), (rest[1:], x, rest[:-1]), (kept[:, :n], rest[:-1], rest[:-1]), (kept[:, :n], rest[1:], rest[:-1]),
+    for yy, xx, out in ((rest[:-1], x, rest[1:]), (rest[1:], x, rest[:-1]), (kept[:, :n], rest[1:], rest[:-1]),
                         (buf[:, :n], x, buf[:, 64:n + 64])):
         before = out.clone()
         with pytest.raises(RuntimeError, match="overlaps"):

@@ -141,9 +141,10 @@ OVERLAPS = [
     dict(y=P, out=P + 16),                          # half a row on
     dict(y=P, out=P, os=24),                        # the same address, rows further apart
     dict(y=P, ys=48, out=P + 16, os=48),            # columns that meet, of one buffer
-    dict(x=P, out=P),                               # x is read by CTAs that do not write these columns
+    dict(x=P, out=P),                               # rows of another width: not the same rows
     dict(x=P, out=P + 48),
-    dict(x=P, xs=40, out=P + 32, os=40),
+    dict(x=P, xs=40, out=P + 64, os=40),            # out's row reaches the next one of x
+    dict(x=P + 64, xs=40, out=P, os=40),
     dict(a=P, out=P + 2 * 8 * 24 * 2 - 16),         # the end of the adapters
     dict(b=P, out=P - 16),
     dict(ids=P + 112, out=P),                       # the last of four rows
