@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _ops  # noqa: F401  (defines torch.ops.comfy_kitchen.*)
-from ._ops import DTYPE_CODE_TO_DTYPE, DTYPE_TO_CODE  # noqa: F401
+from ._ops import DTYPE_CODE_TO_DTYPE, DTYPE_TO_CODE, refuse_derivatives  # noqa: F401
 from .exceptions import BackendError, BackendNotFoundError, BackendNotImplementedError, NoCapableBackendError
 from .float_utils import from_blocked, swap_nibbles, to_blocked
 from .registry import registry
@@ -109,6 +109,7 @@ def add_rmsnorm_quantize_mxfp8(x: torch.Tensor, residual: torch.Tensor, weight: 
         if sum_out is None:
             got = _ops_ns.add_rmsnorm_quantize_mxfp8(x, residual, weight, eps, return_norm)
         else:
+            refuse_derivatives("add_rmsnorm_quantize_mxfp8", x, residual, weight, sum_out)
             data, scales, norm = _ops_ns.add_rmsnorm_quantize_mxfp8_out(x, residual, weight, eps, return_norm, sum_out)
             got = data, scales.view(torch.float8_e8m0fnu), sum_out, norm
         return got if return_norm else got[:-1]
@@ -126,6 +127,7 @@ def add_rmsnorm_quantize_fp8(x: torch.Tensor, residual: torch.Tensor, weight: to
         if sum_out is None:
             got = _ops_ns.add_rmsnorm_quantize_fp8(x, residual, weight, scale, eps, code, return_norm)
         else:
+            refuse_derivatives("add_rmsnorm_quantize_fp8", x, residual, weight, scale, sum_out)
             data, norm = _ops_ns.add_rmsnorm_quantize_fp8_out(x, residual, weight, scale, eps, code, return_norm, sum_out)
             got = data, sum_out, norm
         return got if return_norm else got[:-1]
@@ -142,6 +144,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     if not _Ops._plain((y, x, a, b, adapter_ids, scales, out)):
         if out is None:
             return _ops_ns.lora_add(y, x, a, b, adapter_ids, scales)
+        refuse_derivatives("lora_add", y, x, a, b, scales, out)   # (an op that only writes returns nothing that could ask for one later)
         _ops_ns.lora_add_out(y, x, a, b, adapter_ids, scales, out)
         return out
     impl = registry.get_implementation("lora_add", kwargs={"y": y, "x": x, "a": a, "b": b, "adapter_ids": adapter_ids, "scales": scales})

@@ -8,6 +8,7 @@ that fixes the output shapes for ``torch.compile``.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .float_utils import roundup
 from .registry import registry
@@ -24,6 +25,19 @@ DTYPE_TO_CODE = {v: k for k, v in DTYPE_CODE_TO_DTYPE.items()}
 
 def _dispatch(name: str, **kwargs):
     return registry.get_implementation(name, kwargs=kwargs)(**kwargs)
+
+
+def refuse_derivatives(what: str, *tensors) -> None:
+    """The serving operators record no gradient; a call that would drop one is refused.  Asked of the tensors as the caller gave
+    them: a parameter's data wants none any more."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:   # inside forward_ad.dual_level(), where torch.no_grad() does not apply
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: call it with forward_ad.unpack_dual(t).primal")
 
 
 # ------------------------------------------------------------------ FP8 per tensor

@@ -18,9 +18,9 @@ import ctypes
 import functools
 
 import torch
-from torch.autograd import forward_ad
 
 from comfy_kitchen import _native
+from comfy_kitchen._ops import refuse_derivatives as _no_grad
 from comfy_kitchen.backends._modulation import adaln_prep_modulation
 from comfy_kitchen.float_utils import roundup
 
@@ -599,19 +599,6 @@ def rmsnorm_quantize_nvfp4(
 
 # A call of these runs for a few microseconds on the GPU when one token is served, so their host side is kept short: shapes
 # are read once, addresses go to ctypes as plain integers, and the checks that format a message do so only when they fail.
-
-
-def _no_grad(what: str, *tensors) -> None:
-    """These entry points record no gradient; a call that would drop one is refused.  Asked of the tensors as the caller gave
-    them: a parameter that _plain() has seen wants none any more."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
-    if forward_ad._current_level >= 0:   # inside forward_ad.dual_level(), where torch.no_grad() does not apply
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{what} has no forward-mode derivative: call it with forward_ad.unpack_dual(t).primal")
 
 
 def _same_device(what: str, device, *tensors) -> None:

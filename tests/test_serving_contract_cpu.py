@@ -236,3 +236,28 @@ def test_a_validation_result_cannot_be_changed():
         with pytest.raises(dataclasses.FrozenInstanceError):
             setattr(good, field, value)
     assert validate_function_call(FunctionConstraints(), {}).success
+
+
+@pytest.mark.parametrize("name,argument", [("lora_add", "a"), ("lora_add", "x"), ("mxfp8", "weight"), ("fp8", "weight"), ("fp8", "scale")])
+def test_no_derivative_is_dropped_by_a_traced_write(name, argument):
+    """An op that only writes to an argument returns nothing that could ask for a gradient later: the call itself is refused."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    entry = {"lora_add": ck.lora_add, "mxfp8": ck.add_rmsnorm_quantize_mxfp8, "fp8": ck.add_rmsnorm_quantize_fp8}[name]
+
+    def call(args):
+        given = torch.empty_like(args["y" if name == "lora_add" else "residual"])
+        return entry(**args, **{"out" if name == "lora_add" else "sum_out": given})
+
+    args = _calls()[name][1]
+    args[argument] = torch.nn.Parameter(args[argument])
+    with pytest.raises(RuntimeError, match="no backward"):
+        torch.compile(call, backend="aot_eager")(args)
+    torch._dynamo.reset()
+    with FakeTensorMode():
+        args = _calls()[name][1]
+        args[argument] = torch.nn.Parameter(args[argument])
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(args)
+        with torch.no_grad():
+            call(args)
